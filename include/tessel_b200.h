@@ -108,6 +108,33 @@ int tb200_host_free(tb200_ctx* ctx, void* ptr);
  * path with f32 accumulation, the product scaled by sx[row] * sw[column] before
  * the epilogue's own arithmetic; K a multiple of 16, N a multiple of 8.
  *
+ * 4-bit KV cache (no counterpart in the reference; results differ from the f16
+ * cache's by the quantisation). A cache is u8 [NP,G,P,RB], RB = D/2 + 2*ceil(D/64):
+ * the bytes of one (page, KV head) are P rows of D/2 bytes of codes, then P rows
+ * of ceil(D/64) 16-bit headers, one for each 64 elements of a token's row: an f16
+ * scale of seven significant bits with the zero point in its low four bits.
+ * value = scale * (code - zero point), which an f16 holds exactly. Eight elements
+ * e0..e7 are one little-endian 32-bit word, nibbles e0 e2 e4 e6 e1 e3 e5 e7 from
+ * the low end. Quantising: lo = min(0, min x), hi = max(0, max x), scale =
+ * (hi - lo) / 15 rounded up to seven bits (below 2^-14 to a multiple of 2^-20),
+ * zero point = rint(-lo / scale), code = rint(x / scale) + zero point, kept to
+ * 0..15; a group that holds an infinity or a NaN stands for NaN throughout. D is a
+ * multiple of 16, at most 256, P even; Q, K, V, O and the caches 16-byte aligned.
+ * rope_kv_q4 takes rope_kv's arrays with such caches (QKV, pos, slot, C, S, Q, Kc,
+ * Vc, K, V; the slots of a call that lie inside the cache must differ from one
+ * another). kv_unpack_q4 (Kc, Vc, slot[N], K f16[N,G,D], V f16[N,G,D]) reads rows
+ * back; a slot outside the cache gives zeros. decode_attention_q4 and
+ * chunk_attention_q4 are decode_attention and chunk_attention over such caches;
+ * positions beyond the block table lie on page 0, a page outside the cache reads
+ * as zeros.
+ *
+ * page_copy (caches i64[A], pairs i32[N,2], then the i32 scalars n, NP and bytes):
+ * for each of the A caches, whose device addresses (16-byte aligned) `caches` holds,
+ * and each of the first n pairs (src, dst): page dst = page src, pages of `bytes`
+ * bytes (a multiple of 16) in caches of NP pages. A pair with a page outside the
+ * cache is skipped. All pairs run at once: a page may be the source of several
+ * pairs, but a page that one pair writes must not be in any other pair.
+ *
  * The reference's `meta` and `warps` arguments have no equivalent: tile shapes
  * are chosen inside. */
 int tb200_kernel(tb200_ctx* ctx, const char* name, const int64_t* shapes, const int32_t* ranks, int n_arrays,

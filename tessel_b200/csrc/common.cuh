@@ -52,6 +52,12 @@ enum Kind : int {
   K_LINEAR_Q8,           // Y f16 = (Xq sx) (Wq sw)^T
   K_LINEAR_RESIDUAL_Q8,  // R f32 += (Xq sx) (Wq sw)^T
   K_GATE_UP_Q8,          // Y f16 = silu((Xq sx)(Wgq sg)^T) * ((Xq sx)(Wuq su)^T)
+  // The KV cache in 4 bits (non-parity), and copies of cache pages.
+  K_ROPE_KV_Q4,           // rope_q and the cache write, K and V quantised into their slots
+  K_KV_UNPACK_Q4,         // rows of a 4-bit cache as f16
+  K_DECODE_ATTENTION_Q4,  // decode_attention over a 4-bit cache
+  K_CHUNK_ATTENTION_Q4,   // chunk_attention over a 4-bit cache
+  K_PAGE_COPY,            // pages copied within every cache of a list
   K_COUNT
 };
 

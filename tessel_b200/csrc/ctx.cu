@@ -7,7 +7,7 @@
 #include <sstream>
 
 #include "../../include/tessel_b200.h"
-#include "common.cuh"
+#include "kv_q4.cuh"
 
 struct tb200_ctx {
   tb::Ctx c;
@@ -94,6 +94,11 @@ static const KindInfo KINDS[] = {
     {"linear_q8", K_LINEAR_Q8, 5, 5},
     {"linear_residual_q8", K_LINEAR_RESIDUAL_Q8, 5, 5},
     {"gate_up_q8", K_GATE_UP_Q8, 7, 7},
+    {"rope_kv_q4", K_ROPE_KV_Q4, 10, 10},
+    {"kv_unpack_q4", K_KV_UNPACK_Q4, 5, 5},
+    {"decode_attention_q4", K_DECODE_ATTENTION_Q4, 6, 7},
+    {"chunk_attention_q4", K_CHUNK_ATTENTION_Q4, 6, 7},
+    {"page_copy", K_PAGE_COPY, 2, 5},
 };
 
 static std::string shape_text(const std::vector<int64_t>& s) {
@@ -120,6 +125,11 @@ static bool is_gemm(Kind k) {
   return k == K_LINEAR || k == K_LINEAR_RESIDUAL || k == K_LOGITS || k == K_GATE_UP || k == K_MATMUL ||
          k == K_LINEAR_F32 || k == K_LINEAR_SCATTER || k == K_LINEAR_ROPE_KV || k == K_LINEAR_Q8 ||
          k == K_LINEAR_RESIDUAL_Q8 || k == K_GATE_UP_Q8;
+}
+
+static bool is_kv_q4(Kind k) {
+  return k == K_ROPE_KV_Q4 || k == K_KV_UNPACK_Q4 || k == K_DECODE_ATTENTION_Q4 || k == K_CHUNK_ATTENTION_Q4 ||
+         k == K_PAGE_COPY;
 }
 
 }  // namespace tb
@@ -335,6 +345,8 @@ int tb200_kernel(tb200_ctx* h, const char* name, const int64_t* shapes, const in
     r = make_prefill(c, op);
   else if (op.kind == K_TP_REDUCE_NORM)
     r = make_tp(c, op);
+  else if (is_kv_q4(op.kind))
+    r = make_kv_q4(c, op);
   else
     r = make_glue(c, op);
   if (r) return r;
@@ -365,6 +377,8 @@ int tb200_launch(tb200_ctx* h, tb200_op id, const uint64_t* args, int n_args) {
     r = launch_prefill(c, op, args);
   else if (op.kind == K_TP_REDUCE_NORM)
     r = launch_tp(c, op, args);
+  else if (is_kv_q4(op.kind))
+    r = launch_kv_q4(c, op, args);
   else
     r = launch_glue(c, op, args);
   if (r || !timed) return r;

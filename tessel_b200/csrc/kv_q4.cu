@@ -1,0 +1,384 @@
+// The 4-bit KV cache: rope_q and the cache write of a step's rows (rope_kv_q4), rows read back as
+// f16 (kv_unpack_q4), attention over it for every shape (the tensor-core kernels of
+// decode_attention_q4.cu and chunk_attention_q4.cu take the common ones), and page_copy, which
+// moves pages of any cache. The format is described in kv_q4.cuh.
+#include "kv_q4.cuh"
+
+namespace tb {
+
+namespace {
+
+union H8 {
+  uint4 u;
+  __half h[8];
+};
+
+// One step's QKV rows: Q rotated; K rotated, V as it is, both stored densely and, quantised, into
+// their cache slots. The rotation rounds after every operation, as rope_kv does, so Q, K and V are
+// that kernel's bit for bit.
+//
+// HBM-bound (at decode sizes: launch latency): the QKV row is read and the Q, K, V rows are written
+// once, plus 4.25 bits per cached element. Eight lanes own the 64 elements of a group, eight
+// elements each, so the bounds are three shuffles, and a lane's codes are one 32-bit store. A lane's
+// rotation partner lies D/2 away in the same row: both halves are loaded by both lanes (from L1).
+__global__ void rope_kv_q4_kernel(const __half* __restrict__ QKV, const int* __restrict__ pos,
+                                  const int* __restrict__ slot, const float* __restrict__ Ct,
+                                  const float* __restrict__ St, __half* __restrict__ Q, unsigned char* __restrict__ Kc,
+                                  unsigned char* __restrict__ Vc, __half* __restrict__ Kd, __half* __restrict__ Vd,
+                                  int T, int H, int NPOS, Q4Shape s) {
+  pdl_launch();
+  pdl_wait();
+  const int G = s.G, D = s.D, d2 = D >> 1, W = (H + 2 * G) * D, ng = s.ng();
+  const long long kv = ((long long)T * G * ng * 8 + 31) / 32 * 32;  // whole warps: the shuffles below are warp-wide
+  const int per = D >> 4;
+  const long long total = kv + (long long)T * H * per;
+  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    if (i < kv) {
+      const long long unit = i >> 3;
+      const int gi = (int)(unit % ng), g = (int)((unit / ng) % G), t = (int)(unit / ((long long)ng * G));
+      const int e = gi * Q4_GROUP + (int)(i & 7) * 8;  // this lane's first element
+      const bool live = t < T && e < D;
+      H8 k, v;
+      k.u = v.u = make_uint4(0, 0, 0, 0);
+      if (live) {
+        const int p = pos[t];
+        const bool in = p >= 0 && p < NPOS;
+        const __half* src = QKV + (size_t)t * W + (size_t)(H + g) * D;
+        const bool first = e < d2;
+        const int ec = first ? e : e - d2;
+        H8 x1, x2;
+        x1.u = *reinterpret_cast<const uint4*>(src + ec);
+        x2.u = *reinterpret_cast<const uint4*>(src + ec + d2);
+        v.u = *reinterpret_cast<const uint4*>(src + (size_t)G * D + e);
+        const size_t to = (size_t)(in ? p : 0) * d2 + ec;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float c = in ? Ct[to + j] : 0.f, sn = in ? St[to + j] : 0.f;
+          const float a = __half2float(x1.h[j]), b = __half2float(x2.h[j]);
+          const float y = first ? __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, sn)) : __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, sn));
+          k.h[j] = __float2half_rn(y);
+        }
+        const size_t dd = ((size_t)t * G + g) * D + e;
+        *reinterpret_cast<uint4*>(Kd + dd) = k.u;
+        *reinterpret_cast<uint4*>(Vd + dd) = v.u;
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const H8& x = w ? v : k;
+        float lo = 0.f, hi = 0.f;
+        bool odd = false;  // an infinity or a NaN
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float y = __half2float(x.h[j]);
+          odd |= !(fabsf(y) <= 65504.0f);
+          lo = fminf(lo, y);
+          hi = fmaxf(hi, y);
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+          odd |= __shfl_xor_sync(0xffffffffu, (int)odd, o) != 0;
+        }
+        uint32_t head = odd ? 0x7e00u : q4_scale_bits(lo, hi);
+        const float scale = q4_scale(head);
+        uint32_t word = 0;
+        if (!odd && scale > 0.f) {
+          const float zp = fminf(rintf(__fdiv_rn(-lo, scale)), 15.f);
+          const float most = floorf(__fdiv_rn(65504.f, scale));
+          head |= (uint32_t)zp;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float q = fminf(fmaxf(rintf(__fdiv_rn(__half2float(x.h[j]), scale)), -most), most) + zp;
+            word |= (uint32_t)fminf(fmaxf(q, 0.f), 15.f) << (4 * ((j >> 1) + 4 * (j & 1)));
+          }
+        }
+        if (live) {
+          const int at = slot[t];
+          if (at >= 0 && at < s.NP * s.P) {
+            unsigned char* rec = (w ? Vc : Kc) + ((size_t)(at / s.P) * G + g) * s.record();
+            const int row = at % s.P;
+            *reinterpret_cast<uint32_t*>(rec + (size_t)row * d2 + (e >> 1)) = word;
+            if ((i & 7) == 0)
+              *reinterpret_cast<unsigned short*>(rec + (size_t)s.P * d2 + 2 * (row * ng + gi)) = (unsigned short)head;
+          }
+        }
+      }
+    } else {
+      const long long q = i - kv;
+      const int ch = (int)(q % per), h = (int)((q / per) % H), t = (int)(q / ((long long)per * H));
+      const int p = pos[t];
+      const bool in = p >= 0 && p < NPOS;
+      const __half* src = QKV + (size_t)t * W + (size_t)h * D + ch * 8;
+      H8 x1, x2, y1, y2;
+      x1.u = *reinterpret_cast<const uint4*>(src);
+      x2.u = *reinterpret_cast<const uint4*>(src + d2);
+      const size_t to = (size_t)(in ? p : 0) * d2 + ch * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float c = in ? Ct[to + j] : 0.f, sn = in ? St[to + j] : 0.f;
+        const float a = __half2float(x1.h[j]), b = __half2float(x2.h[j]);
+        y1.h[j] = __float2half_rn(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, sn)));
+        y2.h[j] = __float2half_rn(__fadd_rn(__fmul_rn(b, c), __fmul_rn(a, sn)));
+      }
+      __half* dst = Q + ((size_t)t * H + h) * D + ch * 8;
+      *reinterpret_cast<uint4*>(dst) = y1.u;
+      *reinterpret_cast<uint4*>(dst + d2) = y2.u;
+    }
+  }
+}
+
+// Rows of the cache as f16 (exactly what they stand for); zeros for a slot outside the cache.
+// A thread reads eight elements' codes and writes them as one 16-byte store: HBM-bound.
+__global__ void kv_unpack_q4_kernel(const unsigned char* __restrict__ Kc, const unsigned char* __restrict__ Vc,
+                                    const int* __restrict__ slot, __half* __restrict__ K, __half* __restrict__ V, int N,
+                                    Q4Shape s) {
+  pdl_launch();
+  pdl_wait();
+  const int per = s.D >> 3, G = s.G, ng = s.ng();
+  const long long half = (long long)N * G * per, total = 2 * half;
+  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const bool isv = i >= half;
+    const long long j = isv ? i - half : i;
+    const int ch = (int)(j % per), g = (int)((j / per) % G), n = (int)(j / ((long long)per * G));
+    const int at = slot[n];
+    H8 y;
+    y.u = make_uint4(0, 0, 0, 0);
+    if (at >= 0 && at < s.NP * s.P) {
+      const unsigned char* rec = (isv ? Vc : Kc) + ((size_t)(at / s.P) * G + g) * s.record();
+      const int row = at % s.P;
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + (size_t)row * (s.D >> 1) + ch * 4);
+      const uint32_t head = *reinterpret_cast<const unsigned short*>(rec + (size_t)s.P * (s.D >> 1) + 2 * (row * ng + (ch >> 3)));
+      const float sc = q4_scale(head), zp = q4_zero(head);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y.h[e] = __float2half_rn(sc * ((float)q4_code(w, e) - zp));
+    }
+    *reinterpret_cast<uint4*>((isv ? V : K) + ((size_t)n * G + g) * s.D + ch * 8) = y.u;
+  }
+}
+
+// Attention of one query row and head over its first `n` cached tokens, by one warp, for any page
+// size and head_dim: a key at a time, an f32 online softmax. A lane owns the elements of words
+// lane, lane + 32, ... that is, at most one word of eight (D <= 256).
+// Tokens beyond the block table lie on page 0 (as decode_attention reads them); a page outside the
+// cache reads as zeros.
+__device__ __forceinline__ void attend_q4(const __half* __restrict__ q, const unsigned char* __restrict__ Kc,
+                                          const unsigned char* __restrict__ Vc, const int* __restrict__ row, int MP,
+                                          long long n, int g, float scale, const Q4Shape& s, __half* __restrict__ o) {
+  const int lane = threadIdx.x & 31, words = s.D >> 3, ng = s.ng();
+  const bool mine = lane < words;
+  float qv[8], acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    qv[e] = mine ? __half2float(q[lane * 8 + e]) : 0.f;
+    acc[e] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  for (long long t = 0; t < n; ++t) {
+    const long long col = t / s.P;
+    const int at = (int)(t % s.P), page = col < MP ? row[col] : 0;
+    const bool in = mine && page >= 0 && page < s.NP;
+    const size_t rec = ((size_t)(in ? page : 0) * s.G + g) * s.record();
+    const size_t cw = rec + (size_t)at * (s.D >> 1) + lane * 4, hw = rec + (size_t)s.P * (s.D >> 1) + 2 * (at * ng + (lane >> 3));
+    float x = 0.f, v[8];
+    uint32_t vw = 0;
+    float vs = 0.f, vz = 0.f;
+    if (in) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(Kc + cw);
+      const uint32_t head = *reinterpret_cast<const unsigned short*>(Kc + hw);
+      const float zp = q4_zero(head);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x += ((float)q4_code(w, e) - zp) * qv[e];
+      x *= q4_scale(head);
+      vw = *reinterpret_cast<const uint32_t*>(Vc + cw);
+      const uint32_t vh = *reinterpret_cast<const unsigned short*>(Vc + hw);
+      vs = q4_scale(vh), vz = q4_zero(vh);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = vs * ((float)q4_code(vw, e) - vz);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    x *= scale;
+    const float m2 = fmaxf(m, x), a = expf(m - m2), p = expf(x - m2);
+    l = l * a + p;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = acc[e] * a + p * v[e];
+    m = m2;
+  }
+  if (mine) {
+    H8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y.h[e] = __float2half_rn(acc[e] / l);  // n == 0: 0/0, NaN
+    *reinterpret_cast<uint4*>(o + lane * 8) = y.u;
+  }
+}
+
+__global__ void decode_q4_generic_kernel(const __half* __restrict__ Q, const unsigned char* __restrict__ Kc,
+                                         const unsigned char* __restrict__ Vc, const int* __restrict__ table,
+                                         const int* __restrict__ lens, __half* __restrict__ O, float scale, int B, int H,
+                                         int MP, Q4Shape s) {
+  pdl_launch();
+  pdl_wait();
+  const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  if (w >= (long long)B * H) return;
+  const int b = (int)(w / H), h = (int)(w % H);
+  attend_q4(Q + w * s.D, Kc, Vc, table + (size_t)b * MP, MP, lens[b], h / (H / s.G), scale, s, O + w * s.D);
+}
+
+__global__ void chunk_q4_generic_kernel(const __half* __restrict__ Q, const unsigned char* __restrict__ Kc,
+                                        const unsigned char* __restrict__ Vc, const int* __restrict__ table,
+                                        const int* __restrict__ meta, __half* __restrict__ O, float scale, int T, int H,
+                                        int MP, Q4Shape s) {
+  pdl_launch();
+  pdl_wait();
+  const int* m = meta + 4 * blockIdx.y;
+  const int row0 = m[0], nrows = m[1], pos0 = m[2];
+  if (row0 < 0 || nrows <= 0 || pos0 < 0 || nrows > T - row0) return;  // a descriptor outside the step is skipped
+  const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  if (w >= (long long)nrows * H) return;
+  const int r = (int)(w / H), h = (int)(w % H);
+  const size_t at = ((size_t)(row0 + r) * H + h) * s.D;
+  attend_q4(Q + at, Kc, Vc, table + (size_t)row0 * MP, MP, (long long)pos0 + r + 1, h / (H / s.G), scale, s, O + at);
+}
+
+// For every cache a and pair n: page pairs[n][1] of caches[a] = page pairs[n][0]. One block per
+// (pair, cache) at a time, 16-byte loads, several in flight per thread before the first store.
+__global__ void page_copy_kernel(const unsigned long long* __restrict__ caches, const int* __restrict__ pairs, int A,
+                                 int n, int NP, int words) {
+  pdl_launch();
+  pdl_wait();
+  const long long jobs = (long long)n * A;
+  for (long long j = blockIdx.x; j < jobs; j += gridDim.x) {
+    const int pair = (int)(j / A), a = (int)(j % A);
+    const int src = pairs[2 * pair], dst = pairs[2 * pair + 1];
+    if (src < 0 || src >= NP || dst < 0 || dst >= NP || src == dst) continue;
+    const uint4* from = (const uint4*)caches[a] + (size_t)src * words;
+    uint4* to = (uint4*)caches[a] + (size_t)dst * words;
+    for (int i = threadIdx.x; i < words; i += blockDim.x) to[i] = from[i];
+  }
+}
+
+int blocks_for(long long threads, int block, int sms) {
+  const long long g = (threads + block - 1) / block, cap = (long long)sms * 16;
+  return (int)(g < 1 ? 1 : g > cap ? cap : g);
+}
+
+}  // namespace
+
+int make_kv_q4(Ctx* c, Op& op) {
+  const auto& s = op.shapes;
+  auto bad = [&](const char* why) { return fail(c, op.name + ": " + why); };
+  for (const auto& a : s)
+    for (int64_t d : a)
+      if (d > 0x7fffffffLL) return bad("a dimension is beyond 2^31 - 1");
+  Q4Shape q;
+  const char* why = nullptr;
+  switch (op.kind) {
+    case K_ROPE_KV_Q4: {
+      // QKV[T,W], pos[T], slot[T], C, S [NPOS,D/2], Q[T,H,D], Kc, Vc, K, V [T,G,D]
+      if (s[0].size() != 2 || s[1].size() != 1 || s[2].size() != 1 || s[3].size() != 2 || s[4] != s[3] || s[5].size() != 3 ||
+          s[8].size() != 3 || s[9] != s[8])
+        return bad("shapes are QKV[T,W], pos[T], slot[T], C, S[NPOS,D/2], Q[T,H,D], Kc, Vc, K, V[T,G,D]");
+      const int64_t T = s[0][0], H = s[5][1], D = s[5][2];
+      if ((why = q4_shape(op, 6, D, &q))) return bad(why);
+      if (s[1][0] != T || s[2][0] != T || s[5][0] != T || s[8][0] != T) return bad("QKV, pos, slot, Q, K and V have T rows");
+      if (s[3][1] != D / 2) return bad("the rotation tables are [NPOS, D/2]");
+      if (s[8][1] != q.G || s[8][2] != D) return bad("K and V are [T,G,D]");
+      if (s[0][1] != (H + 2 * q.G) * D) return bad("W must be (H + 2G) * D");
+      return 0;
+    }
+    case K_KV_UNPACK_Q4:
+      if (s[2].size() != 1 || s[3].size() != 3 || s[4] != s[3] || s[3][0] != s[2][0])
+        return bad("shapes are Kc, Vc, slot[N], K, V[N,G,D]");
+      if ((why = q4_shape(op, 0, s[3][2], &q))) return bad(why);
+      if (s[3][1] != q.G) return bad("K and V are [N,G,D]");
+      return 0;
+    case K_DECODE_ATTENTION_Q4:
+    case K_CHUNK_ATTENTION_Q4: {
+      const bool chunk = op.kind == K_CHUNK_ATTENTION_Q4;
+      const char* shapes = chunk ? "shapes are Q[T,H,D], Kc, Vc, table[T,MP], meta[C,4], O[T,H,D]"
+                                 : "shapes are Q[B,H,D], Kc, Vc, table[B,MP], lens[B], O[B,H,D]";
+      if (s[0].size() != 3 || s[5] != s[0] || s[3].size() != 2 || s[3][0] != s[0][0]) return bad(shapes);
+      if (chunk ? s[4].size() != 2 || s[4][1] != 4 : s[4].size() != 1 || s[4][0] != s[0][0]) return bad(shapes);
+      if ((why = q4_shape(op, 1, s[0][2], &q))) return bad(why);
+      if (s[0][1] < 1 || s[0][1] % q.G) return bad("heads must be a multiple of kv heads");
+      if (chunk && s[4][0] > 65535) return bad("at most 65535 chunks");
+      return 0;
+    }
+    case K_PAGE_COPY:
+      if (s[0].size() != 1 || s[1].size() != 2 || s[1][1] != 2) return bad("shapes are caches i64[A], pairs[N,2]");
+      return 0;
+    default:
+      return bad("not a 4-bit cache kernel");
+  }
+}
+
+int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
+  const auto& s = op.shapes;
+  auto bad = [&](const char* why) { return fail(c, op.name + ": " + why); };
+  Q4Shape q;
+  switch (op.kind) {
+    case K_ROPE_KV_Q4: {
+      const int T = (int)s[0][0], H = (int)s[5][1], D = (int)s[5][2], NPOS = (int)s[3][0];
+      q4_shape(op, 6, D, &q);
+      if (T == 0) return 0;
+      for (int i : {0, 5, 6, 7, 8, 9})
+        if (!aligned_to(a[i], 16)) return bad("QKV, Q, K, V and the caches must be 16-byte aligned");
+      const long long n = ((long long)T * q.G * q.ng() * 8 + 31) / 32 * 32 + (long long)T * H * (D / 16);
+      TB_CUDA(c, launch_k(c, rope_kv_q4_kernel, dim3(blocks_for(n, 128, c->sm_count)), dim3(128), 0, 1, (const __half*)a[0],
+                          (const int*)a[1], (const int*)a[2], (const float*)a[3], (const float*)a[4], (__half*)a[5],
+                          (unsigned char*)a[6], (unsigned char*)a[7], (__half*)a[8], (__half*)a[9], T, H, NPOS, q));
+      break;
+    }
+    case K_KV_UNPACK_Q4: {
+      const int N = (int)s[2][0], D = (int)s[3][2];
+      q4_shape(op, 0, D, &q);
+      if (N == 0) return 0;
+      for (int i : {0, 1, 3, 4})
+        if (!aligned_to(a[i], 16)) return bad("K, V and the caches must be 16-byte aligned");
+      const long long n = 2LL * N * q.G * (D / 8);
+      TB_CUDA(c, launch_k(c, kv_unpack_q4_kernel, dim3(blocks_for(n, 256, c->sm_count)), dim3(256), 0, 1,
+                          (const unsigned char*)a[0], (const unsigned char*)a[1], (const int*)a[2], (__half*)a[3],
+                          (__half*)a[4], N, q));
+      break;
+    }
+    case K_DECODE_ATTENTION_Q4:
+    case K_CHUNK_ATTENTION_Q4: {
+      const int T = (int)s[0][0], H = (int)s[0][1], D = (int)s[0][2], MP = (int)s[3][1];
+      q4_shape(op, 1, D, &q);
+      for (int i : {0, 1, 2, 5})
+        if (!aligned_to(a[i], 16)) return bad("Q, O and the caches must be 16-byte aligned");
+      const unsigned blocks = (unsigned)(((long long)T * H + 3) / 4);
+      if (T == 0) return 0;
+      if (op.kind == K_DECODE_ATTENTION_Q4) {
+        TB_CUDA(c, launch_k(c, decode_q4_generic_kernel, dim3(blocks), dim3(128), 0, 1, (const __half*)a[0],
+                            (const unsigned char*)a[1], (const unsigned char*)a[2], (const int*)a[3], (const int*)a[4],
+                            (__half*)a[5], bits_f32(a[6]), T, H, MP, q));
+      } else {
+        if (s[4][0] == 0) return 0;
+        TB_CUDA(c, launch_k(c, chunk_q4_generic_kernel, dim3(blocks, (unsigned)s[4][0]), dim3(128), 0, 1,
+                            (const __half*)a[0], (const unsigned char*)a[1], (const unsigned char*)a[2], (const int*)a[3],
+                            (const int*)a[4], (__half*)a[5], bits_f32(a[6]), T, H, MP, q));
+      }
+      break;
+    }
+    case K_PAGE_COPY: {
+      const int A = (int)s[0][0], n = (int)(uint32_t)a[2], NP = (int)(uint32_t)a[3], bytes = (int)(uint32_t)a[4];
+      if (n < 0 || n > s[1][0]) return bad("0 <= n <= N pairs");
+      if (NP < 0 || bytes < 16 || bytes % 16) return bad("the page size must be a positive multiple of 16 bytes, NP not negative");
+      if (!aligned_to(a[0], 8) || !aligned_to(a[1], 4)) return bad("the address table must be 8-byte aligned");
+      if (A == 0 || n == 0) return 0;
+      const long long jobs = (long long)A * n, cap = (long long)c->sm_count * 8;
+      TB_CUDA(c, launch_k(c, page_copy_kernel, dim3((unsigned)(jobs < cap ? jobs : cap)), dim3(256), 0, 1,
+                          (const unsigned long long*)a[0], (const int*)a[1], A, n, NP, bytes / 16));
+      break;
+    }
+    default:
+      return bad("not a 4-bit cache kernel");
+  }
+  c->launches += 1;
+  TB_CUDA(c, cudaGetLastError());
+  return 0;
+}
+
+}  // namespace tb

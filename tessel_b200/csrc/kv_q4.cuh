@@ -1,0 +1,75 @@
+// The 4-bit KV cache's format, shared by the kernels that write it (kv_q4.cu) and attend over it
+// (decode_attention_q4.cu, chunk_attention_q4.cu).
+//
+// A cache is u8 [NP, G, P, RB] with RB = D/2 + 2 ceil(D/64) bytes per token and KV head. The P * RB
+// bytes of one (page, head) hold first the P tokens' codes, D/2 bytes each, then their headers,
+// ceil(D/64) 16-bit words each, one for every 64 elements (the last group may be shorter).
+//
+// Header: an f16 scale of seven significant bits, its low four mantissa bits replaced by the zero
+// point zp. value = scale * (code - zp) with code in 0..15: |code - zp| has four bits, so the
+// product has at most eleven and an f16 holds it exactly. Every kernel can therefore choose where
+// it multiplies (in f16 tiles, or in f32 after the dot product) and still compute on the same numbers.
+//
+// Codes: eight elements e0..e7 take one 32-bit word, nibbles e0 e2 e4 e6 e1 e3 e5 e7 from the low
+// end, so that masking a word with 0x000f000f << 4k leaves a pair of neighbours in the two halves.
+//
+// Quantising 64 f16 numbers x: lo = min(0, min x), hi = max(0, max x); scale = (hi - lo) / 15 rounded
+// UP to seven significant bits (below 2^-14: to a multiple of 2^-20), so 15 steps reach across;
+// zp = rint(-lo / scale), code = clamp(rint(x / scale) + zp, 0, 15), where rint(x / scale) is kept to
+// floor(65504 / scale) steps, so that no value passes the largest f16 number. All zeros: scale 0. A
+// group that holds an infinity or a NaN gets a NaN scale and stands for NaN throughout.
+#pragma once
+
+#include "common.cuh"
+
+namespace tb {
+
+constexpr int Q4_GROUP = 64;
+
+struct Q4Shape {
+  int NP, G, P, D;
+  __host__ __device__ int ng() const { return (D + Q4_GROUP - 1) / Q4_GROUP; }
+  __host__ __device__ int row_bytes() const { return D / 2 + 2 * ng(); }
+  __host__ __device__ int record() const { return P * row_bytes(); }
+};
+
+// The cache shape of an op (array `i`) whose head_dim is `D`; null, or what is wrong with it.
+inline const char* q4_shape(const Op& op, int i, int64_t D, Q4Shape* out) {
+  const auto& s = op.shapes[i];
+  if (s.size() != 4 || op.shapes[i + 1] != s) return "the caches are two arrays [NP,G,P,D/2 + 2*ceil(D/64)]";
+  if (D < 16 || D % 16 || D > 256) return "head_dim must be a multiple of 16, at most 256";
+  if (s[3] != D / 2 + 2 * ((D + Q4_GROUP - 1) / Q4_GROUP)) return "a cache row has D/2 + 2*ceil(D/64) bytes";
+  if (s[2] < 2 || s[2] % 2 || s[2] > 1024) return "the page size must be even, at most 1024";
+  if (s[1] < 1) return "at least one kv head";
+  if (s[0] * s[1] > 0x7fffffffLL || s[0] * s[2] > 0x7fffffffLL) return "the cache has too many pages";
+  *out = Q4Shape{(int)s[0], (int)s[1], (int)s[2], (int)D};
+  return nullptr;
+}
+
+inline bool aligned_to(uint64_t p, uint64_t n) { return (p & (n - 1)) == 0; }
+
+int make_kv_q4(Ctx* c, Op& op);
+int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a);
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ float q4_scale(uint32_t head) { return __half2float(__ushort_as_half((unsigned short)(head & 0xfff0u))); }
+__device__ __forceinline__ float q4_zero(uint32_t head) { return (float)(head & 15u); }
+
+// Element `i` (0..7) of a word of codes.
+__device__ __forceinline__ int q4_code(uint32_t word, int i) { return (word >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15; }
+
+// The header for a group with these bounds (lo <= 0 <= hi).
+__device__ __forceinline__ uint32_t q4_scale_bits(float lo, float hi) {
+  const float r = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+  float s;
+  if (r < 6.103515625e-05f)  // 2^-14: f16 subnormals, four low bits of 2^-24 units kept free
+    s = ceilf(r * 1048576.0f) * 9.5367431640625e-07f;
+  else
+    s = __uint_as_float((__float_as_uint(r) + 0x1ffffu) & ~0x1ffffu);
+  return __half_as_ushort(__float2half_rn(s));  // exact: seven bits, at most 2 * 65504 / 15 rounded up
+}
+
+#endif  // __CUDACC__
+
+}  // namespace tb

@@ -29,7 +29,8 @@ from typing import Dict, List, Optional, Sequence
 
 import numpy as np
 
-from .gpu import Buf, F32, Gpu, K
+from . import kv4 as kv4_format
+from .gpu import Buf, F32, Gpu, I32, K
 from .model import Config, Weights, rope_tables
 
 
@@ -132,7 +133,7 @@ class Engine:
     """``w`` holds the full model; with ``nranks > 1`` this engine keeps rank ``rank``'s shard of it."""
 
     def __init__(self, gpu: Gpu, w: Weights, lim: Limits, rank: int = 0, nranks: int = 1, sharded: bool = False,
-                 exchange=None, fp8: bool = False):
+                 exchange=None, fp8: bool = False, kv4: bool = False):
         """``sharded``: ``w`` already is this rank's shard (its ``cfg`` the local shape).
         ``exchange``: with ``nranks > 1``, a function that takes this rank's list of byte strings and
         returns every rank's list (an all-gather on the host). When given, the ranks map each
@@ -143,11 +144,18 @@ class Engine:
         layer are quantised to E4M3 with one f32 scale per output row when they are uploaded,
         activations are quantised per row on the device in front of each projection, and the
         projections run on the tensor cores' 8-bit path. Attention, RoPE, the cache, the norms'
-        arithmetic and the LM head stay as they are."""
+        arithmetic and the LM head stay as they are.
+        ``kv4``: a separate, NON-PARITY mode (any number of ranks, with or without ``fp8``): the cache
+        holds K and V in 4 bits with one scale and zero point for 64 elements (``tessel_b200.kv4``),
+        0.27 of the f16 cache's bytes. Decode steps and prompts fed in chunks attend to the
+        quantised keys and values; a prompt's own prefill step attends to its rows in f16."""
         full = w.cfg
         if fp8 and nranks != 1:
             raise ValueError("the FP8 mode runs on a single rank")
         self.fp8 = fp8
+        self.kv4 = kv4
+        if kv4 and (full.head_dim % 16 or full.head_dim > 256 or lim.page % 2):
+            raise ValueError("a 4-bit cache takes a head_dim that is a multiple of 16, at most 256, and an even page size")
         if full.heads % full.kv_heads or full.head_dim % 2:
             raise ValueError("heads must be a multiple of kv_heads, head_dim even")
         if not sharded:
@@ -178,7 +186,12 @@ class Engine:
         self.head = up(w.lm_head) if w.lm_head is not None else self.embed
         self.norm = up(w.norm)
         slots = lim.pages * lim.page
-        kv_bytes = slots * cfg.kv_heads * cfg.head_dim * 2
+        row = kv4_format.row_bytes(cfg.head_dim) if kv4 else cfg.head_dim * 2
+        kv_bytes = slots * cfg.kv_heads * row
+        # The cache as the attention kernels see it, and bytes of one page of K (or V) of one layer.
+        self.cache_shape = [lim.pages, cfg.kv_heads, lim.page, row] if kv4 else [lim.pages, lim.page, cfg.kv_heads, cfg.head_dim]
+        self.page_bytes = lim.page * cfg.kv_heads * row
+        self._page_tables: Optional[tuple] = None
         self.layers: List[_DevLayer] = []
         self.q8: List[Dict[str, Buf]] = []
         for l in w.layers:
@@ -499,12 +512,11 @@ class Engine:
         if prefill:
             att = k("prefill_attention", [[t, nh, hd], [t, ng, hd], [t, ng, hd], [t], [t, nh, hd]])
         else:
-            att = k("decode_attention", [[t, nh, hd], [lim.pages, lim.page, ng, hd], [lim.pages, lim.page, ng, hd],
-                                         [t, mp], [t], [t, nh, hd]])
+            cache, q4 = self.cache_shape, "_q4" if self.kv4 else ""
+            att = k("decode_attention" + q4, [[t, nh, hd], cache, cache, [t, mp], [t], [t, nh, hd]])
         chunk_att = None
         if not prefill and self._chunks:
-            cache = [lim.pages, lim.page, ng, hd]
-            chunk_att = k("chunk_attention", [[t, nh, hd], cache, cache, [t, mp], [self._chunks, 4], [t, nh, hd]])
+            chunk_att = k("chunk_attention" + q4, [[t, nh, hd], cache, cache, [t, mp], [self._chunks, 4], [t, nh, hd]])
         if self.fp8:
             g.launch(embed, [self.tok, self.embed, self.x])
             self._launch_layers_q8(t, prefill, att, chunk_att, eps, scale)
@@ -516,7 +528,11 @@ class Engine:
         fused_shapes = [[t, dm], [w, dm]] + rope_shapes + [[t, w]] + kv_shapes
         fused_args = [self.h, l0.wqkv, self.pos, self.slot, self.cos, self.sin, self.qkv, self.q, l0.kc, l0.vc,
                       self.k, self.v]
-        if self._fuse_rope_for(t, fused_shapes, fused_args, rope_shapes, kv_shapes):
+        if self.kv4:
+            # The quantiser needs whole groups of a row, so the rotation and the cache write stay behind the projection.
+            qkv = self._mm("linear", [[t, dm], [w, dm], [t, w]], [self.h, l0.wqkv, self.qkv], t)
+            ropekv = self._rope_kv_q4(t)
+        elif self._fuse_rope_for(t, fused_shapes, fused_args, rope_shapes, kv_shapes):
             # The QKV projection rotates and scatters its own output (src/llm/engine.rs:473-488 as
             # one kernel): Q, the dense K and V and the cache pages come straight from the accumulators.
             qkv = self._mm("linear_rope_kv", fused_shapes, fused_args, t)
@@ -568,6 +584,12 @@ class Engine:
             project(down, self.mlp, l.wd)
         self._launch_head(t, bw, greedy, eps)
 
+    def _rope_kv_q4(self, t: int) -> K:
+        cfg = self.cfg
+        nh, ng, hd = cfg.heads, cfg.kv_heads, cfg.head_dim
+        return self.gpu.kernel("rope_kv_q4", [[t, cfg.qkv()], [t], [t], [cfg.max_pos, hd // 2], [cfg.max_pos, hd // 2],
+                                              [t, nh, hd], self.cache_shape, self.cache_shape, [t, ng, hd], [t, ng, hd]])
+
     def _launch_qkv(self, qkv: K, ropekv: Optional[K], l: _DevLayer) -> None:
         """QKV projection, rotary embedding and the KV-cache write of one layer: one kernel, or
         (``ropekv`` given) the projection followed by ``rope_kv``."""
@@ -588,8 +610,8 @@ class Engine:
         ns, npos = lim.pages * lim.page, cfg.max_pos
         normq = k("rmsnorm_q8", [[t, dm], [dm], [t, dm], [t]])
         qkv = k("linear_q8", [[t, dm], [t], [w, dm], [w], [t, w]])
-        ropekv = k("rope_kv", [[t, w], [t], [t], [npos, hd // 2], [npos, hd // 2], [t, nh, hd], [ns, ng, hd],
-                               [ns, ng, hd], [t, ng, hd], [t, ng, hd]])
+        ropekv = self._rope_kv_q4(t) if self.kv4 else k("rope_kv", [
+            [t, w], [t], [t], [npos, hd // 2], [npos, hd // 2], [t, nh, hd], [ns, ng, hd], [ns, ng, hd], [t, ng, hd], [t, ng, hd]])
         quant_o = k("quant_rows", [[t, nh * hd], [t, nh * hd], [t]])
         oproj = k("linear_residual_q8", [[t, nh * hd], [t], [dm, nh * hd], [dm], [t, dm]])
         gu = k("gate_up_q8", [[t, dm], [t], [f, dm], [f], [f, dm], [f], [t, f]])
@@ -665,9 +687,41 @@ class Engine:
             pick = k("argmax_rows", [[bw, v], [bw]])
             g.launch(pick, [self.logits, self.picked])
 
+    # -- pages ------------------------------------------------------------------------
+    def copy_pages(self, pairs: Sequence[Sequence[int]]) -> None:
+        """Copies cache pages, in every layer's K and V: ``pairs`` of (source, destination). Every copy reads its
+        source as it was before the call, so pages may be moved along (5 -> 2 with 9 -> 5): copies that have to wait
+        for others go into launches of their own, usually there is one. A page outside the cache, a page written twice
+        and pages exchanged in a circle are refused (ValueError) before anything is copied."""
+        waves = kv4_format.copy_waves(pairs, self.lim.pages)
+        if not waves:
+            return
+        g = self.gpu
+        if self._page_tables is None:
+            caches = np.array([b.ptr for l in self.layers for b in (l.kc, l.vc)], np.uint64)
+            self._page_tables = (g.tensor(caches), len(caches), g.alloc(self.lim.pages * 8))
+        caches, n, buf = self._page_tables
+        copy = g.kernel("page_copy", [[n], [self.lim.pages, 2]])
+        g.write(buf, 0, np.array([p for w in waves for p in w], np.int32))
+        at = 0
+        for w in waves:
+            g.launch(copy, [caches, Buf(buf.ptr + at * 8, buf.bytes - at * 8), I32(len(w)), I32(self.lim.pages), I32(self.page_bytes)])
+            at += len(w)
+
     # -- inspection (tests, parity checks) ------------------------------------------
     def read_cache(self, layer: int):
-        """The K and V caches of one layer as f16 ``[pages, page, kv_heads, head_dim]`` arrays."""
+        """The K and V caches of one layer as f16 ``[pages, page, kv_heads, head_dim]`` arrays (of a 4-bit cache: the
+        values it stands for, which an f16 holds exactly)."""
         shape = (self.lim.pages, self.lim.page, self.cfg.kv_heads, self.cfg.head_dim)
         l = self.layers[layer]
+        if self.kv4:
+            g, ns = self.gpu, shape[0] * shape[1]
+            rows = [ns, shape[2], shape[3]]
+            slot = g.tensor(np.arange(ns, dtype=np.int32))
+            out = [g.alloc(ns * shape[2] * shape[3] * 2) for _ in range(2)]
+            g.launch(g.kernel("kv_unpack_q4", [self.cache_shape, self.cache_shape, [ns], rows, rows]), [l.kc, l.vc, slot] + out)
+            k, v = (g.fetch(b, np.float16, shape) for b in out)
+            for b in [slot] + out:
+                g.free(b)
+            return k, v
         return self.gpu.fetch(l.kc, np.float16, shape), self.gpu.fetch(l.vc, np.float16, shape)

@@ -17,6 +17,12 @@ keys before its attention runs). The step says which rows are such pieces
 (``engine.Mixed``), and the engine runs them through ``chunk_attention``: the
 prefill kernel's tensor-core pipeline with the paged cache as K and V, one CTA
 per 256 rows and head, instead of one decode query per token.
+
+Another: ``prefix``, tokens that every request's prompt starts with (a shared system prompt).
+They are computed once, into pages that all sequences' block tables then share; a prefix
+that ends inside a page is forked: that one page is copied into each sequence's first page of
+its own (``Engine.copy_pages``, all layers in one launch). A request's own prompt is then fed in
+chunks behind the prefix. ``Scheduler.compact`` moves the pages in use to the front of the cache.
 """
 from __future__ import annotations
 
@@ -64,6 +70,8 @@ class _Seq:
     last: int
     left: int
     todo: int = 0  # prompt tokens not yet in the cache (a prompt fed in chunks)
+    base: int = 0  # tokens in front of the request's own prompt (a shared prefix)
+    shared: int = 0  # leading pages that belong to the prefix, not to this sequence
 
 
 class Scheduler:
@@ -71,9 +79,15 @@ class Scheduler:
     one call admits and prefills what fits, or decodes one token for every running sequence."""
 
     def __init__(self, e: Engine, reqs: Sequence[Request], max_batch: int, packed: bool = True,
-                 device_argmax: bool = False, chunk: int = 0):
+                 device_argmax: bool = False, chunk: int = 0, prefix: Sequence[int] = ()):
         self.e, self.reqs, self.packed, self.device_argmax = e, reqs, packed, device_argmax
+        self.prefix = list(prefix)
+        if self.prefix and not chunk:
+            chunk = e.lim.max_tokens
         self.chunk = max(0, min(chunk, e.lim.max_tokens - 1))
+        if self.prefix and not self.chunk:
+            raise ValueError("a shared prefix needs steps of at least two tokens")
+        self.prefix_pages: List[int] = []  # the prefix's pages, once it is in the cache
         self.feeding: List[_Seq] = []  # sequences whose (long) prompt is still being fed in chunks
         self.start = time.perf_counter()
         # Pops yield pages 0, 1, 2, ...
@@ -96,18 +110,62 @@ class Scheduler:
             return [int(t) for t in self.e.step_greedy(toks, pos, slots, attn, want)]
         return [argmax(row) for row in self.e.step(toks, pos, slots, attn, want)]
 
+    def _feed_prefix(self) -> None:
+        """Computes the shared prefix into pages of its own."""
+        e, p, n = self.e, self.e.lim.page, len(self.prefix)
+        need = -(-n // p)
+        if need > len(self.free) or need > e.lim.max_seq_pages or n > e.cfg.max_pos:
+            raise ValueError(f"shared prefix of {n} tokens does not fit")
+        pages = [self.free.pop() for _ in range(need)]
+        pg = np.asarray(pages, np.int64)
+        size = n if n <= e.lim.max_tokens else self.chunk
+        for a in range(0, n, size):
+            i = np.arange(a, min(a + size, n))
+            tables = np.zeros((len(i), need), np.int32)
+            tables[0] = pages
+            attn = Prefill() if size == n else Mixed(tables, (i + 1).tolist(), [(0, len(i), a)])
+            e.step(self.prefix[a:a + len(i)], i.tolist(), (pg[i // p] * p + i % p).tolist(), attn, [])
+        self.st.prompt_tokens += n
+        self.prefix_pages = pages
+
+    def _free_pages(self, s: _Seq) -> None:
+        self.free.extend(s.pages[s.shared:])
+
+    def compact(self) -> int:
+        """Moves the pages in use to the lowest page numbers (``Engine.copy_pages``) and points the block tables at them;
+        returns how many are in use. Call it between steps: pages from that number on hold nothing any more."""
+        seqs = self.running + self.feeding
+        live = set(self.prefix_pages)
+        for s in seqs:
+            live.update(s.pages)
+        n = len(live)
+        moves = dict(zip(sorted(pg for pg in live if pg >= n), (pg for pg in range(n) if pg not in live)))
+        if moves:
+            self.e.copy_pages(list(moves.items()))
+        at = lambda pages: [moves.get(pg, pg) for pg in pages]
+        self.prefix_pages = at(self.prefix_pages)
+        for s in seqs:
+            s.pages = at(s.pages)
+        self.free = list(range(self.e.lim.pages - 1, n - 1, -1))
+        self._table_ids = ()
+        return n
+
     def _admit(self) -> List[Tuple[int, List[int]]]:
         """As many waiting prompts as the step's token budget, the batch and the free cache pages
         allow. Pages for a whole sequence are reserved up front."""
         e, p = self.e, self.e.lim.page
         admit: List[Tuple[int, List[int]]] = []
         tokens = 0
+        if self.prefix and not self.prefix_pages and self.waiting:
+            self._feed_prefix()
+        base, shared = len(self.prefix), len(self.prefix) // p
+        forks = []  # (the prefix's last, partly filled page, a sequence's copy of it)
         while self.waiting:
             rid = self.waiting[0]
             r = self.reqs[rid]
-            need = -(-(len(r.prompt) + r.max_new) // p)
-            long = len(r.prompt) > e.lim.max_tokens
-            if len(r.prompt) == 0 or (long and not self.chunk) or need > e.lim.max_seq_pages:
+            need = -(-(base + len(r.prompt) + r.max_new) // p) - shared
+            long = len(r.prompt) > e.lim.max_tokens or base > 0
+            if len(r.prompt) == 0 or (long and not self.chunk) or shared + need > e.lim.max_seq_pages:
                 raise ValueError(f"request {rid}: prompt of {len(r.prompt)} tokens does not fit")
             busy = len(self.running) + len(self.feeding) + len(admit)
             if long:
@@ -115,8 +173,11 @@ class Scheduler:
                 if busy >= self.max_batch or need > len(self.free):
                     break
                 self.waiting.popleft()
-                self.feeding.append(_Seq(rid, [self.free.pop() for _ in range(need)], 0, -1, r.max_new,
-                                         len(r.prompt)))
+                own = [self.free.pop() for _ in range(need)]
+                if base % p:
+                    forks.append((self.prefix_pages[shared], own[0]))
+                self.feeding.append(_Seq(rid, self.prefix_pages[:shared] + own, base, -1, r.max_new, len(r.prompt),
+                                         base, shared))
                 continue
             room = busy < self.max_batch and tokens + len(r.prompt) <= e.lim.max_tokens
             if not room or need > len(self.free) or (not self.packed and admit):
@@ -124,6 +185,8 @@ class Scheduler:
             self.waiting.popleft()
             tokens += len(r.prompt)
             admit.append((rid, [self.free.pop() for _ in range(need)]))
+        if forks:
+            e.copy_pages(forks)
         return admit
 
     def decode_inputs(self):
@@ -157,7 +220,7 @@ class Scheduler:
             self.out[s.id].tokens.append(t)
             if s.left == 0 or t == eos:
                 self.out[s.id].done_s = time.perf_counter() - self.start
-                self.free.extend(s.pages)
+                self._free_pages(s)
             else:
                 keep.append(s)
         self.running = keep
@@ -188,7 +251,7 @@ class Scheduler:
                 s = _Seq(rid, pages, len(reqs[rid].prompt), t, reqs[rid].max_new - 1)
                 if s.left == 0 or t == e.cfg.eos:
                     self.out[rid].done_s = time.perf_counter() - self.start
-                    self.free.extend(s.pages)
+                    self._free_pages(s)
                 else:
                     self.running.append(s)
             return "prefill"
@@ -224,7 +287,7 @@ class Scheduler:
             chunks.append((len(toks), c, s.len))
             first_rows.append((len(toks), s.pages))
             i = np.arange(s.len, s.len + c)
-            toks.extend(pr[s.len:s.len + c])
+            toks.extend(pr[s.len - s.base:s.len - s.base + c])
             pos.extend(i.tolist())
             slots.extend((np.asarray(s.pages, np.int64)[i // p] * p + i % p).tolist())
             lens.extend((i + 1).tolist())
@@ -258,7 +321,7 @@ class Scheduler:
             s.last, s.left = t, s.left - 1
             if s.left == 0 or t == e.cfg.eos:
                 self.out[s.id].done_s = time.perf_counter() - self.start
-                self.free.extend(s.pages)
+                self._free_pages(s)
             else:
                 self.running.append(s)
         return "mixed"
@@ -276,12 +339,13 @@ def generate(e: Engine, reqs: Sequence[Request], max_batch: int) -> Tuple[List[O
 
 
 def generate_with(e: Engine, reqs: Sequence[Request], max_batch: int, packed: bool,
-                  device_argmax: bool = False, chunk: int = 0) -> Tuple[List[Output], Stats]:
+                  device_argmax: bool = False, chunk: int = 0, prefix: Sequence[int] = ()) -> Tuple[List[Output], Stats]:
     """``generate``, choosing whether new prompts share prefill steps (``packed``) or each takes
     its own. ``device_argmax`` picks the tokens on the GPU (``Engine.step_greedy``) instead of
     reading the logits back and choosing on the host as the reference does. ``chunk > 0`` admits
-    prompts longer than a step and feeds them that many tokens at a time (see the module text)."""
-    s = Scheduler(e, reqs, max_batch, packed, device_argmax, chunk)
+    prompts longer than a step and feeds them that many tokens at a time; ``prefix`` are tokens in
+    front of every request's prompt, computed once and shared (see the module text for both)."""
+    s = Scheduler(e, reqs, max_batch, packed, device_argmax, chunk, prefix)
     while not s.done():
         if s.step() == "idle" and s.waiting:
             raise ValueError(f"request {s.waiting[0]} cannot be admitted: not enough cache pages")

@@ -42,6 +42,10 @@ class EmuGpu:
         self._bufs[base] = np.zeros(max(nbytes, 1), np.uint8)
         return Buf(base, nbytes)
 
+    def free(self, b: Buf) -> None:
+        self._bases.remove(b.ptr)
+        del self._bufs[b.ptr]
+
     def _view(self, ptr: int, nbytes: int) -> np.ndarray:
         i = bisect.bisect_right(self._bases, ptr) - 1
         base = self._bases[i]
@@ -137,6 +141,8 @@ class EmuGpu:
             kc, vc, kd, vd = oracle.kv_write(qkv, A(2, i), A(3, i), A(4, f), A(5, f), A(8, h), A(9, h), sh[8][1],
                                              sh[8][2])
             A(8, h)[:], A(9, h)[:], A(10, h)[:], A(11, h)[:] = kc, vc, kd, vd
+        elif name in ("rope_kv_q4", "kv_unpack_q4", "decode_attention_q4", "chunk_attention_q4", "page_copy"):
+            self._q4(name, args, sh, A, sc)
         elif name in ("quant_rows", "rmsnorm_q8", "linear_q8", "linear_residual_q8", "gate_up_q8"):
             self._q8(name, A, sc)
         elif name == "prefill_attention":
@@ -185,6 +191,49 @@ class EmuGpu:
                 out[m] = 0 if best[1] < 0 else int(best[1])
         else:
             raise GpuError(f"no kernel {name}")
+
+    def _q4(self, name, args, sh, A, sc) -> None:
+        """The 4-bit cache's kernels in numpy: the host quantiser (tessel_b200/kv4.py), and the oracle's attention on the f16
+        values that the cache stands for."""
+        from tessel_b200 import kv4
+        h, f, i, u8 = np.float16, np.float32, np.int32, np.uint8
+        if name == "rope_kv_q4":
+            # QKV, pos, slot, C, S, Q, Kc, Vc, K, V: the f16 form's rows (every slot dropped), then the quantised writes.
+            T, G, D = sh[8]
+            A(5, h)[:] = oracle.rope_q(A(0, h), A(1, i), A(3, f), A(4, f), sh[5][1], D)
+            none = np.zeros((1, G, D), h)
+            _, _, kd, vd = oracle.kv_write(A(0, h), A(1, i), np.full(T, 1, i), A(3, f), A(4, f), none, none, G, D)
+            A(8, h)[:], A(9, h)[:] = kd, vd
+            kv4.write(A(6, u8), A(2, i), kd)
+            kv4.write(A(7, u8), A(2, i), vd)
+        elif name == "kv_unpack_q4":
+            N, G, D = sh[3]
+            slot, ns = A(2, i), sh[0][0] * sh[0][2]
+            keep = (slot >= 0) & (slot < ns)
+            for c, o in ((0, 3), (1, 4)):
+                rows = kv4.read(A(c, u8), D).reshape(ns, G, D)
+                A(o, h)[:] = np.where(keep[:, None, None], rows[np.where(keep, slot, 0)], h(0))
+        elif name == "page_copy":
+            bases, pairs = A(0, np.uint64), A(1, i)
+            n, pages, nbytes = sc(2), sc(3), sc(4)
+            for b in bases:
+                c = self._view(int(b), pages * nbytes).reshape(pages, nbytes)
+                for s, d in pairs[:n]:
+                    if 0 <= s < pages and 0 <= d < pages:
+                        c[d] = c[s]
+        else:
+            D = sh[0][2]
+            kc, vc = kv4.read(A(1, u8), D), kv4.read(A(2, u8), D)
+            q, o, table = A(0, h), A(5, h), A(3, i)
+            if name == "decode_attention_q4":
+                o[:] = oracle.decode_attention(q, kc, vc, table, A(4, i), sc(6))
+                return
+            for row0, nrows, pos0, _ in A(4, i):
+                if nrows > 0:
+                    rows = np.arange(row0, row0 + nrows)
+                    tb = np.repeat(table[row0:row0 + 1], nrows, axis=0)
+                    ln = (pos0 + 1 + np.arange(nrows)).astype(np.int32)
+                    o[rows] = oracle.decode_attention(q[rows], kc, vc, tb, ln, sc(6))
 
     @staticmethod
     def _q8(name, A, sc) -> None:
