@@ -1,0 +1,577 @@
+// Paged grouped-query decode attention over the 4-bit cache (format: kv_q4.cuh), for pages of 16
+// tokens and head_dim 64 or 128; other shapes run on kv_q4.cu's one-warp kernel.
+//
+// Mathematics. With a key's code u, zero point z and scale s (64 elements share z and s), and a
+// query q: q.k = sum over groups of s (q.u - z sum(q)); so the tensor cores multiply q by the raw
+// codes and the scale and zero point come in afterwards, once per (token, head, group). For the
+// values, o = sum_t p_t s_t (u_t - z_t) = sum_t P_t (u_t - 8) + sum_t P_t (8 - z_t) with P = p s:
+// the scale rides on the weight, the second sum is one number per (head, group). Codes are centred
+// by 8 because all-positive products would make the accumulator hundreds of times larger than the
+// result of a long context, and the tensor cores' sums are not rounded to nearest.
+//
+// A code becomes an f16 operand by one AND: the nibble in the low bits of an f16 is the subnormal
+// u 2^-24, the next nibble 16 u 2^-24, and the tensor cores take subnormals as they are; the powers
+// of two are taken out of the accumulators. q enters as the f16 it is. P is split in two f16 (hi +
+// lo), so the second product keeps f32 accuracy; with four or fewer query heads per KV head the
+// eight columns of the product hold hi and lo side by side, else lo is a second product.
+//
+// Bound: HBM bytes, 2 (D/2 + 2 D/64) per token and KV head, with the issue slots close behind.
+//
+// Work split. A CTA takes an equal share of the step's (sequence, KV head, page) list, whatever the
+// lengths are: it finds its place from the lengths, walks through as many (sequence, head) units as
+// its share covers, and writes O itself for units that lie wholly inside. A unit that is cut leaves
+// one partial in each CTA; a second, tiny kernel joins them.
+#include "kv_q4.cuh"
+
+namespace tb {
+
+namespace {
+
+constexpr int DQ_WARPS = 4;                       // consumer warps
+constexpr int DQ_THREADS = (DQ_WARPS + 1) * 32;   // + one producer warp
+constexpr int DQ_STAGES = 8;                      // pages in flight per CTA
+constexpr int DQ_CTAS = 4;                        // per SM
+constexpr int DQ_LEAST = 8;                       // pages a CTA takes at least: two per warp
+constexpr int DQ_SLOT = 8;                        // heads of a partial
+static_assert(DQ_STAGES % DQ_WARPS == 0, "a slot is always read by the same warp");
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float TWO24 = 16777216.0f;
+constexpr float GROW = 8.0f;        // the running maximum is renewed when a score passes it by this (log2): p <= 2^8
+constexpr float SCALE_MOST = 128.f; // and the values' running scale when s F passes this: P = p s F < 2^15 fits an f16
+
+// What a table entry outside the cache reads as.
+__device__ __align__(128) unsigned char g_zero_record[2048];
+
+struct DqParams {
+  const __half* Q;
+  const unsigned char* Kc;
+  const unsigned char* Vc;
+  const int* table;
+  const int* lens;
+  __half* O;
+  float* part;  // [CTA][2][8][D + 2]: accumulators, then maximum and sum, per head
+  int* desc;    // [CTA][4]: sequence, head group, CTAs that hold a piece of the unit cut at this CTA's end (0: none)
+  float scale;
+  int B, H, G, NP, MP, hgroups, least;
+  unsigned int* status;
+};
+
+template <int D>
+struct DqSmem {
+  static constexpr int REC = 16 * (D / 2 + 2 * (D / 64));
+  static constexpr int KV = (REC + 127) / 128 * 128;
+  static constexpr int STAGE = 2 * KV;
+  static constexpr int RING = DQ_STAGES * STAGE;
+  static constexpr int WARP = 8 * D + 16;  // floats a warp leaves for the merge: acc[head][d], m[8], l[8]
+  static constexpr int BARS = RING + DQ_WARPS * WARP * 4;
+  static constexpr int SCAN = BARS + 2 * DQ_STAGES * 8;  // long long [DQ_THREADS + 1], then the CTA's start
+  static constexpr int TOTAL = SCAN + (DQ_THREADS + 4) * 8 + 128;
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"((uint64_t)src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ uint32_t movm_t(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  unsigned short v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t add_h2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ float lo_f32(uint32_t h2) { return __low2float(*reinterpret_cast<__half2*>(&h2)); }
+__device__ __forceinline__ float hi_f32(uint32_t h2) { return __high2float(*reinterpret_cast<__half2*>(&h2)); }
+
+// A place in the list of (sequence, head group, page): sequences in order, the head groups of one
+// after another, its pages within.
+struct Place {
+  int b, hg;
+  long long page;
+};
+
+__device__ __forceinline__ long long pages_of(int n) { return n > 0 ? ((long long)n + 15) / 16 : 0; }
+
+// The number of (unit, page) items, the share of a CTA, and where CTA `cta` begins. All threads call it.
+__device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, long long cta, long long* total,
+                                            long long* share) {
+  const int units = p.G * p.hgroups;
+  const int per = (p.B + DQ_THREADS - 1) / DQ_THREADS;
+  const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
+  long long sum = 0;
+  for (int b = b0; b < b1; ++b) sum += pages_of(p.lens[b]);
+  scan[threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    // Exclusive prefix of the threads' sums: a lane owns DQ_WARPS + 1 neighbours.
+    constexpr int OWN = DQ_THREADS / 32;
+    long long own = 0;
+    for (int i = 0; i < OWN; ++i) own += scan[threadIdx.x * OWN + i];
+    long long inc = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+      if ((int)threadIdx.x >= o) inc += up;
+    }
+    long long at = inc - own;
+    for (int i = 0; i < OWN; ++i) {
+      const long long v = scan[threadIdx.x * OWN + i];
+      scan[threadIdx.x * OWN + i] = at;
+      at += v;
+    }
+    if (threadIdx.x == 31) scan[DQ_THREADS] = at;
+  }
+  __syncthreads();
+  const long long all = scan[DQ_THREADS] * units;
+  const long long w = max((all + gridDim.x - 1) / gridDim.x, (long long)p.least);
+  const long long start = cta * w;
+  *total = all;
+  *share = w;
+  // The thread whose sequences hold `start` says which one.
+  if (start < all) {
+    long long at = scan[threadIdx.x] * units;
+    for (int b = b0; b < b1; ++b) {
+      const long long np = pages_of(p.lens[b]);
+      if (start >= at && start < at + np * units) {
+        scan[DQ_THREADS + 1] = b;
+        scan[DQ_THREADS + 2] = start - at;
+      }
+      at += np * units;
+    }
+  }
+  __syncthreads();
+  Place r = {0, 0, 0};
+  if (start < all) {
+    r.b = (int)scan[DQ_THREADS + 1];
+    const long long np = pages_of(p.lens[r.b]), in = scan[DQ_THREADS + 2];
+    r.hg = (int)(in / np);
+    r.page = in % np;
+  }
+  return r;
+}
+
+template <int D, bool SIDE>
+__global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const DqParams p) {
+  pdl_launch();
+  pdl_wait();
+  using SM = DqSmem<D>;
+  constexpr int NG = D / 64;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 127) & ~(uintptr_t)127);
+  uint64_t* full = (uint64_t*)(smem + SM::BARS);
+  uint64_t* empty = full + DQ_STAGES;
+  long long* scan = (long long*)(smem + SM::SCAN);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < DQ_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    fence_barrier_init();
+    p.desc[4 * blockIdx.x + 2] = 0;
+  }
+  long long total, share;
+  Place at = find_place(p, scan, blockIdx.x, &total, &share);
+  const long long first = blockIdx.x * share;
+  long long left = first < total ? min(share, total - first) : 0;
+  const int units = p.G * p.hgroups, hq = p.H / p.G;
+
+  if (warp == DQ_WARPS) {
+    // ---- producer: walks the block tables and brings one record of K and of V per page ------------
+    const size_t rec_page = (size_t)p.G * SM::REC;
+    int j = 0;  // pages issued; a slot's phase follows from it
+    for (; left > 0; at.page = 0, ++at.hg) {
+      if (at.hg == units) at.hg = 0, ++at.b;
+      long long np = pages_of(p.lens[at.b]);
+      while (np == 0) np = pages_of(p.lens[++at.b]);  // (only at the start of a sequence; `left` says that one follows)
+      const long long count = min(np - at.page, left);
+      const size_t head = (size_t)(at.hg / p.hgroups) * SM::REC;
+      for (long long j0 = 0; j0 < count; j0 += 32) {
+        const long long col = at.page + j0 + lane;  // beyond the table: page 0
+        const int mine = (j0 + lane < count && col < p.MP) ? p.table[(size_t)at.b * p.MP + col] : 0;
+        const int lim = (int)min(32LL, count - j0);
+        for (int i = 0; i < lim; ++i, ++j) {
+          const int page = __shfl_sync(0xffffffffu, mine, i);
+          if (lane == 0) {
+            const int s = j % DQ_STAGES;
+            mbar_wait(&empty[s], ((j / DQ_STAGES) & 1) ^ 1, p.status, 501);
+            mbar_expect_tx(&full[s], 2 * SM::REC);
+            unsigned char* dst = smem + s * SM::STAGE;
+            const bool in = page >= 0 && page < p.NP;
+            const size_t off = (size_t)page * rec_page + head;
+            bulk_load(dst, in ? p.Kc + off : g_zero_record, SM::REC, &full[s]);
+            bulk_load(dst + SM::KV, in ? p.Vc + off : g_zero_record, SM::REC, &full[s]);
+          }
+        }
+      }
+      left -= count;
+    }
+    return;
+  }
+
+  // ---- consumers -----------------------------------------------------------------------------------
+  const int gq = lane >> 2, t = lane & 3;
+  // Rows of the K tile (and columns of the V tile) are the page's tokens in the order that lets a
+  // lane's four V tokens be t, 4 + t, 8 + t, 12 + t: row r is token (r & 7) / 2 + 4 (r & 1) + (r & 8).
+  const int tok_a = (gq >> 1) + 4 * (gq & 1), tok_b = tok_a + 8;
+  const float sc2 = p.scale * LOG2E * TWO24;
+  const uint32_t ring = smem_u32(smem);
+  int base = 0;  // pages of the CTA before this segment
+  for (; left > 0; at.page = 0, ++at.hg) {
+    if (at.hg == units) at.hg = 0, ++at.b;
+    int n = p.lens[at.b];
+    while (n <= 0) n = p.lens[++at.b];
+    const long long np = pages_of(n);
+    const int count = (int)min(np - at.page, left);
+    const int g = at.hg / p.hgroups, h0 = g * hq + (at.hg % p.hgroups) * 8, nh = min(8, hq - (at.hg % p.hgroups) * 8);
+
+    // Q as the B operand: column gq is head gq (SIDE: heads 0..3 twice), the rows of step k of group
+    // x are elements 64 x + 16 t + 2 k, + 1 and the same + 8, as the words of codes hold them.
+    uint32_t qf[NG][4][2];
+    float qsum[NG][2];
+    {
+      const int hc = SIDE ? gq & 3 : gq;
+      const bool live = hc < nh;
+      const __half* q = p.Q + ((size_t)at.b * p.H + h0 + (live ? hc : 0)) * D + 16 * t;
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if (live) {
+          lo = *reinterpret_cast<const uint4*>(q + 64 * x);
+          hi = *reinterpret_cast<const uint4*>(q + 64 * x + 8);
+        }
+        qf[x][0][0] = lo.x, qf[x][1][0] = lo.y, qf[x][2][0] = lo.z, qf[x][3][0] = lo.w;
+        qf[x][0][1] = hi.x, qf[x][1][1] = hi.y, qf[x][2][1] = hi.z, qf[x][3][1] = hi.w;
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s += lo_f32(qf[x][k][0]) + hi_f32(qf[x][k][0]) + lo_f32(qf[x][k][1]) + hi_f32(qf[x][k][1]);
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        qsum[x][0] = __shfl_sync(0xffffffffu, s, 8 * t);      // of head 2t
+        qsum[x][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);  // of head 2t + 1
+      }
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float F = 4294967296.0f * 64.0f / 4096.0f;  // for the smallest scale, 2^-20: the first page sets it
+    float acc[4 * NG][4], zacc[NG][2];
+#pragma unroll
+    for (int i = 0; i < 4 * NG; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+#pragma unroll
+    for (int x = 0; x < NG; ++x) zacc[x][0] = zacc[x][1] = 0.f;
+
+    for (int j = base + ((warp - base) & (DQ_WARPS - 1)); j < base + count; j += DQ_WARPS) {
+      const int s = j % DQ_STAGES;
+      mbar_wait(&full[s], (j / DQ_STAGES) & 1, p.status, 502);
+      const uint32_t kb = ring + s * SM::STAGE, vb = kb + SM::KV;
+      // Headers of this lane's two tokens: a pair of f16 (or one), scales and zero points (2^-24 units).
+      uint32_t hka, hkb, hva, hvb;
+      if (NG == 2) {
+        hka = lds32(kb + 8 * D + 4 * tok_a), hkb = lds32(kb + 8 * D + 4 * tok_b);
+        hva = lds32(vb + 8 * D + 4 * tok_a), hvb = lds32(vb + 8 * D + 4 * tok_b);
+      } else {
+        hka = lds16(kb + 8 * D + 2 * tok_a), hkb = lds16(kb + 8 * D + 2 * tok_b);
+        hva = lds16(vb + 8 * D + 2 * tok_a), hvb = lds16(vb + 8 * D + 2 * tok_b);
+      }
+      // Tokens behind the last one: stale headers may be NaN, and the scores are masked below.
+      const long long tok0 = (at.page + j - base) * 16;
+      const bool tail = tok0 + 16 > n;
+      const bool ok_a = !tail || tok0 + tok_a < n, ok_b = !tail || tok0 + tok_b < n;
+      if (tail) {
+        if (!ok_a) hka = hva = 0;
+        if (!ok_b) hkb = hvb = 0;
+      }
+      float xa[2] = {0.f, 0.f}, xb[2] = {0.f, 0.f};  // scores of heads 2t, 2t + 1 in the log2 domain
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        const uint2 wa = lds64(kb + tok_a * (D / 2) + 32 * x + 8 * t), wb = lds64(kb + tok_b * (D / 2) + 32 * x + 8 * t);
+        float e[4] = {0.f, 0.f, 0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};  // nibbles of weight 1, and of weight 16
+        mma16816(e, wa.x & 0x000f000fu, wb.x & 0x000f000fu, wa.y & 0x000f000fu, wb.y & 0x000f000fu, qf[x][0][0], qf[x][0][1]);
+        mma16816(o, wa.x & 0x00f000f0u, wb.x & 0x00f000f0u, wa.y & 0x00f000f0u, wb.y & 0x00f000f0u, qf[x][1][0], qf[x][1][1]);
+        const uint32_t ax = wa.x >> 8, bx = wb.x >> 8, ay = wa.y >> 8, by = wb.y >> 8;
+        mma16816(e, ax & 0x000f000fu, bx & 0x000f000fu, ay & 0x000f000fu, by & 0x000f000fu, qf[x][2][0], qf[x][2][1]);
+        mma16816(o, ax & 0x00f000f0u, bx & 0x00f000f0u, ay & 0x00f000f0u, by & 0x00f000f0u, qf[x][3][0], qf[x][3][1]);
+        const uint32_t sa = hka & 0xfff0fff0u, za = hka & 0x000f000fu, sb = hkb & 0xfff0fff0u, zb = hkb & 0x000f000fu;
+        const float ka = (x ? hi_f32(sa) : lo_f32(sa)) * sc2, kza = x ? hi_f32(za) : lo_f32(za);
+        const float kbs = (x ? hi_f32(sb) : lo_f32(sb)) * sc2, kzb = x ? hi_f32(zb) : lo_f32(zb);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          xa[c] = fmaf(ka, fmaf(-kza, qsum[x][c], fmaf(o[c], 0.0625f, e[c])), xa[c]);
+          xb[c] = fmaf(kbs, fmaf(-kzb, qsum[x][c], fmaf(o[2 + c], 0.0625f, e[2 + c])), xb[c]);
+        }
+      }
+      if (tail) {
+        if (!ok_a) xa[0] = xa[1] = -INFINITY;
+        if (!ok_b) xb[0] = xb[1] = -INFINITY;
+      }
+      // The running maximum is lazy: renewed (and the sums rescaled) only when a score outgrew it by 2^8.
+      if (__any_sync(0xffffffffu, fmaxf(xa[0], xb[0]) > m[0] + GROW || fmaxf(xa[1], xb[1]) > m[1] + GROW)) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(xa[c], xb[c]);
+#pragma unroll
+          for (int d = 4; d <= 16; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          mx = fmaxf(m[c], mx);
+          const float f = m[c] == -INFINITY ? 0.f : ex2(m[c] - mx);  // (nothing to rescale before the first page)
+          m[c] = mx;
+          l[c] *= f;
+#pragma unroll
+          for (int i = 0; i < 4 * NG; ++i) acc[i][c] *= f, acc[i][2 + c] *= f;
+#pragma unroll
+          for (int x = 0; x < NG; ++x) zacc[x][c] *= f;
+        }
+      }
+      const float pa[2] = {ex2(xa[0] - m[0]), ex2(xa[1] - m[1])}, pb[2] = {ex2(xb[0] - m[0]), ex2(xb[1] - m[1])};
+      l[0] += pa[0] + pb[0];
+      l[1] += pa[1] + pb[1];
+      // P = p s F: F, a power of two, keeps it in f16's range whatever the values' size. It follows the
+      // largest scale seen.
+      float va[NG], vbs[NG];
+      {
+        const uint32_t sa = hva & 0xfff0fff0u, sb = hvb & 0xfff0fff0u;
+        va[0] = lo_f32(sa), vbs[0] = lo_f32(sb);
+        if (NG == 2) va[NG - 1] = hi_f32(sa), vbs[NG - 1] = hi_f32(sb);
+        float most = fmaxf(va[0], vbs[0]);
+        if (NG == 2) most = fmaxf(most, fmaxf(va[NG - 1], vbs[NG - 1]));
+        if (__any_sync(0xffffffffu, most * F >= SCALE_MOST)) {
+#pragma unroll
+          for (int d = 1; d <= 16; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+          const float to = __uint_as_float((260u - (__float_as_uint(most) >> 23)) << 23);  // the largest scale in [64, 128)
+          const float f = to / F;
+          F = to;
+#pragma unroll
+          for (int i = 0; i < 4 * NG; ++i) acc[i][0] *= f, acc[i][1] *= f, acc[i][2] *= f, acc[i][3] *= f;
+#pragma unroll
+          for (int x = 0; x < NG; ++x) zacc[x][0] *= f, zacc[x][1] *= f;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        const uint32_t za = hva & 0x000f000fu, zb = hvb & 0x000f000fu;
+        const float sa = va[x] * F, sb = vbs[x] * F;
+        const float ca = 8.f / TWO24 - (x ? hi_f32(za) : lo_f32(za)), cb = 8.f / TWO24 - (x ? hi_f32(zb) : lo_f32(zb));
+        const float a0 = pa[0] * sa, a1 = pa[1] * sa, b0 = pb[0] * sb, b1 = pb[1] * sb;
+        zacc[x][0] = fmaf(b0, cb, fmaf(a0, ca, zacc[x][0]));
+        zacc[x][1] = fmaf(b1, cb, fmaf(a1, ca, zacc[x][1]));
+        uint32_t pha = pack_h2(a0, a1), phb = pack_h2(b0, b1);
+        const uint32_t pla = pack_h2(a0 - lo_f32(pha), a1 - hi_f32(pha)), plb = pack_h2(b0 - lo_f32(phb), b1 - hi_f32(phb));
+        if (SIDE && t >= 2) pha = pla, phb = plb;  // columns 4..7: the same heads' low parts
+        const uint32_t bh0 = movm_t(pha), bh1 = movm_t(phb);
+        uint32_t bl0 = 0, bl1 = 0;
+        if (!SIDE) bl0 = movm_t(pla), bl1 = movm_t(plb);
+        // V^T: a lane's word gq of the group, for its four tokens; two tokens' halves side by side.
+        const uint32_t v = vb + 32 * x + 4 * gq + t * (D / 2);
+        const uint32_t w0 = lds32(v), w1 = lds32(v + 2 * D), w2 = lds32(v + 4 * D), w3 = lds32(v + 6 * D);
+        const uint32_t lo01 = __byte_perm(w0, w1, 0x5410), hi01 = __byte_perm(w0, w1, 0x7632);
+        const uint32_t lo23 = __byte_perm(w2, w3, 0x5410), hi23 = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // elements 2k, 2k + 1 of the word: rows gq, gq + 8
+          const int sh = (k >> 1) * 8;
+          const uint32_t mask = (k & 1) ? 0x00f000f0u : 0x000f000fu, centre = (k & 1) ? 0x80808080u : 0x80088008u;
+          const uint32_t a_0 = add_h2((lo01 >> sh) & mask, centre), a_1 = add_h2((hi01 >> sh) & mask, centre);
+          const uint32_t a_2 = add_h2((lo23 >> sh) & mask, centre), a_3 = add_h2((hi23 >> sh) & mask, centre);
+          mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bh0, bh1);
+          if (!SIDE) mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bl0, bl1);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+    }
+
+    // ---- the four warps' sums of this segment, merged ---------------------------------------------
+    float z[NG][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int d = 4; d <= 16; d <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], d);
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        z[x][c] = zacc[x][c];
+#pragma unroll
+        for (int d = 4; d <= 16; d <<= 1) z[x][c] += __shfl_xor_sync(0xffffffffu, z[x][c], d);
+      }
+    }
+    float* mine = (float*)(smem + SM::RING) + warp * SM::WARP;
+    const float unit = TWO24 / F;
+#pragma unroll
+    for (int i = 0; i < 4 * NG; ++i) {
+      const int d = 64 * (i >> 2) + 8 * gq + 2 * (i & 3);
+      const float w = (i & 1) ? 0.0625f * unit : unit;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        // SIDE: columns 4..7 are the low parts of heads 0..3; the zero points count once.
+        const float zz = SIDE && t >= 2 ? 0.f : z[i >> 2][c] * unit;
+        mine[(2 * t + c) * D + d] = fmaf(acc[i][c], w, zz);
+        mine[(2 * t + c) * D + d + 1] = fmaf(acc[i][2 + c], w, zz);
+      }
+    }
+    if (gq == 0) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) mine[8 * D + 2 * t + c] = m[c], mine[8 * D + 8 + 2 * t + c] = l[c];
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(DQ_WARPS * 32) : "memory");
+    const float* all = (const float*)(smem + SM::RING);
+    const bool whole = at.page == 0 && count == np;
+    float* part = p.part + ((size_t)blockIdx.x * 2 + (at.page == 0 ? 1 : 0)) * DQ_SLOT * (D + 2);
+    for (int i = threadIdx.x; i < nh * D; i += DQ_WARPS * 32) {
+      const int hh = i / D, d = i % D;
+      float mt = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < DQ_WARPS; ++w) mt = fmaxf(mt, all[w * SM::WARP + 8 * D + hh]);
+      float lt = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < DQ_WARPS; ++w) {
+        const float* a = all + w * SM::WARP;
+        const float mw = a[8 * D + hh], lw = a[8 * D + 8 + hh];
+        // A warp without a page has nothing; one whose scores were all NaN has a NaN sum.
+        const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2(mw - mt);
+        float v = a[hh * D + d];
+        if (SIDE) v += a[(hh + 4) * D + d];
+        if (f != 0.f || v != v) o = fmaf(v, f, o);
+        lt = fmaf(lw, f, lt);
+      }
+      if (whole) {
+        p.O[((size_t)at.b * p.H + h0 + hh) * D + d] = __float2half_rn(o / lt);
+      } else {
+        part[hh * D + d] = o;
+        if (d == 0) part[DQ_SLOT * D + hh] = mt, part[DQ_SLOT * (D + 1) + hh] = lt;
+      }
+    }
+    if (threadIdx.x == 0 && !whole && at.page == 0) {
+      // The unit is cut at this CTA's end: the next CTAs go on with it.
+      int* d = p.desc + 4 * blockIdx.x;
+      d[0] = at.b, d[1] = at.hg;
+      d[2] = 1 + (int)((np - count + share - 1) / share);
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(DQ_WARPS * 32) : "memory");
+    base += count;
+    left -= count;
+  }
+
+  // Rows without a cached token: 0/0, as decode_attention gives.
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x)
+    if (p.lens[b] <= 0)
+      for (int i = threadIdx.x; i < p.H * D; i += DQ_WARPS * 32)
+        p.O[(size_t)b * p.H * D + i] = __float2half_rn(__int_as_float(0x7fc00000));
+}
+
+// Joins the partials of the unit that is cut at the end of CTA blockIdx.x, if there is one: that
+// CTA's second slot and the first slots of the CTAs that follow. One warp per head.
+template <int D>
+__global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p) {
+  pdl_launch();
+  pdl_wait();
+  const int* d = p.desc + 4 * blockIdx.x;
+  const int b = d[0], hg = d[1], pieces = d[2];
+  if (pieces < 2) return;
+  const int hq = p.H / p.G, h0 = (hg / p.hgroups) * hq + (hg % p.hgroups) * 8, nh = min(8, hq - (hg % p.hgroups) * 8);
+  const int hh = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (hh >= nh) return;
+  auto slot = [&](int i) { return p.part + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * DQ_SLOT * (D + 2); };
+  float m = -INFINITY;
+  for (int i = lane; i < pieces; i += 32) m = fmaxf(m, slot(i)[DQ_SLOT * D + hh]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float l = 0.f, a[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) a[i] = 0.f;
+  for (int i = 0; i < pieces; ++i) {
+    const float* s = slot(i);
+    const float mi = s[DQ_SLOT * D + hh];
+    const float f = mi == -INFINITY ? 1.f : ex2(mi - m);  // (only where its scores were all NaN, and so are its sums)
+    l = fmaf(s[DQ_SLOT * (D + 1) + hh], f, l);
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) a[k] = fmaf(s[hh * D + lane + 32 * k], f, a[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k)
+    p.O[((size_t)b * p.H + h0 + hh) * D + lane + 32 * k] = __float2half_rn(a[k] / l);
+}
+
+template <int D, bool SIDE>
+int run(Ctx* c, Op& op, DqParams p, const Q4Shape& q) {
+  const int grid = op.p1;
+  TB_CUDA(c, launch_k(c, decode_q4_kernel<D, SIDE>, dim3(grid), dim3(DQ_THREADS), DqSmem<D>::TOTAL, 1, p));
+  c->launches += 1;
+  TB_CUDA(c, launch_k(c, decode_q4_join_kernel<D>, dim3(grid), dim3(256), 0, 1, p));
+  c->launches += 1;
+  return 0;
+}
+
+}  // namespace
+
+bool decode_q4_takes(const Q4Shape& q, int B, int MP) {
+  return q.P == 16 && (q.D == 64 || q.D == 128) && q.NP > 0 && B > 0 && MP > 0;
+}
+
+int make_decode_q4(Ctx* c, Op& op, const Q4Shape& q) {
+  const int B = (int)op.shapes[0][0], H = (int)op.shapes[0][1];
+  const int units = q.G * ((H / q.G + 7) / 8);
+  // As many CTAs as stay resident, and no more than have DQ_LEAST pages to work on. (Lengths beyond
+  // the table only make the shares larger.)
+  const long long most = ((long long)B * units * op.shapes[3][1] + DQ_LEAST - 1) / DQ_LEAST;
+  const long long fit = (long long)c->sm_count * DQ_CTAS;
+  op.p1 = (int)(most < fit ? most : fit);
+  op.scratch_bytes = (size_t)op.p1 * (2 * DQ_SLOT * (q.D + 2) * sizeof(float) + 16);
+  TB_CUDA(c, cudaMalloc(&op.scratch, op.scratch_bytes));
+  auto attr = [&](auto kern, int bytes) { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); };
+  TB_CUDA(c, attr(decode_q4_kernel<128, true>, DqSmem<128>::TOTAL));
+  TB_CUDA(c, attr(decode_q4_kernel<128, false>, DqSmem<128>::TOTAL));
+  TB_CUDA(c, attr(decode_q4_kernel<64, true>, DqSmem<64>::TOTAL));
+  TB_CUDA(c, attr(decode_q4_kernel<64, false>, DqSmem<64>::TOTAL));
+  return 0;
+}
+
+int launch_decode_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
+  DqParams p;
+  p.Q = (const __half*)a[0];
+  p.Kc = (const unsigned char*)a[1];
+  p.Vc = (const unsigned char*)a[2];
+  p.table = (const int*)a[3];
+  p.lens = (const int*)a[4];
+  p.O = (__half*)a[5];
+  p.scale = bits_f32(a[6]);
+  p.B = (int)op.shapes[0][0], p.H = (int)op.shapes[0][1], p.G = q.G, p.NP = q.NP, p.MP = (int)op.shapes[3][1];
+  p.hgroups = (p.H / p.G + 7) / 8;
+  p.least = DQ_LEAST;
+  p.status = c->status;
+  p.part = (float*)op.scratch;
+  p.desc = (int*)(p.part + (size_t)op.p1 * 2 * DQ_SLOT * (q.D + 2));
+  const bool side = p.H / p.G <= 4;
+  int r;
+  if (q.D == 128)
+    r = side ? run<128, true>(c, op, p, q) : run<128, false>(c, op, p, q);
+  else
+    r = side ? run<64, true>(c, op, p, q) : run<64, false>(c, op, p, q);
+  return r;
+}
+
+}  // namespace tb

@@ -303,7 +303,8 @@ int make_kv_q4(Ctx* c, Op& op) {
       if ((why = q4_shape(op, 1, s[0][2], &q))) return bad(why);
       if (s[0][1] < 1 || s[0][1] % q.G) return bad("heads must be a multiple of kv heads");
       if (chunk && s[4][0] > 65535) return bad("at most 65535 chunks");
-      return 0;
+      op.p0 = !chunk && decode_q4_takes(q, (int)s[0][0], (int)s[3][1]);
+      return op.p0 ? make_decode_q4(c, op, q) : 0;
     }
     case K_PAGE_COPY:
       if (s[0].size() != 1 || s[1].size() != 2 || s[1][1] != 2) return bad("shapes are caches i64[A], pairs[N,2]");
@@ -350,6 +351,7 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
         if (!aligned_to(a[i], 16)) return bad("Q, O and the caches must be 16-byte aligned");
       const unsigned blocks = (unsigned)(((long long)T * H + 3) / 4);
       if (T == 0) return 0;
+      if (op.p0) return launch_decode_q4(c, op, a, q);
       if (op.kind == K_DECODE_ATTENTION_Q4) {
         TB_CUDA(c, launch_k(c, decode_q4_generic_kernel, dim3(blocks), dim3(128), 0, 1, (const __half*)a[0],
                             (const unsigned char*)a[1], (const unsigned char*)a[2], (const int*)a[3], (const int*)a[4],

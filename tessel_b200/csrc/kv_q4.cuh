@@ -50,6 +50,10 @@ inline bool aligned_to(uint64_t p, uint64_t n) { return (p & (n - 1)) == 0; }
 
 int make_kv_q4(Ctx* c, Op& op);
 int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a);
+// The tensor-core kernels behind decode_attention_q4 (decode_attention_q4.cu), for the shapes they take.
+bool decode_q4_takes(const Q4Shape& q, int B, int MP);
+int make_decode_q4(Ctx* c, Op& op, const Q4Shape& q);
+int launch_decode_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q);
 
 #ifdef __CUDACC__
 
