@@ -10,10 +10,16 @@
 // result of a long context, and the tensor cores' sums are not rounded to nearest.
 //
 // A code becomes an f16 operand by one AND: the nibble in the low bits of an f16 is the subnormal
-// u 2^-24, the next nibble 16 u 2^-24, and the tensor cores take subnormals as they are; the powers
-// of two are taken out of the accumulators. q enters as the f16 it is. P is split in two f16 (hi +
-// lo), so the second product keeps f32 accuracy; with four or fewer query heads per KV head the
-// eight columns of the product hold hi and lo side by side, else lo is a second product.
+// u 2^-24, the next nibble 16 u 2^-24, and the tensor cores take subnormals as they are. For the
+// keys the 16 is taken out of q (q / 16 is exact, or off by 2^-25 where |q| < 2^-10), for the
+// values out of the accumulators. P is split in two f16 (hi + lo), so the second product keeps f32
+// accuracy.
+//
+// The eight columns of a product. With four or fewer query heads per KV head (SIDE) a warp takes two
+// pages at a time: the first page's scores come out in columns 0..3, the second's in 4..7 (the
+// operand q has zeros in the other page's columns), so no lane of the softmax idles; and the hi and
+// lo parts of P share a product, side by side. With five to eight heads a page fills the columns,
+// and lo is a second product.
 //
 // Bound: HBM bytes, 2 (D/2 + 2 D/64) per token and KV head, with the issue slots close behind.
 //
@@ -29,8 +35,8 @@ namespace {
 
 constexpr int DQ_WARPS = 4;                       // consumer warps
 constexpr int DQ_THREADS = (DQ_WARPS + 1) * 32;   // + one producer warp
-constexpr int DQ_STAGES = 8;                      // pages in flight per CTA
-constexpr int DQ_CTAS = 4;                        // per SM
+constexpr int DQ_STAGES = 8;                      // pairs of pages in flight per CTA
+constexpr int DQ_CTAS = 3;                        // per SM
 constexpr int DQ_LEAST = 8;                       // pages a CTA takes at least: two per warp
 constexpr int DQ_SLOT = 8;                        // heads of a partial
 static_assert(DQ_STAGES % DQ_WARPS == 0, "a slot is always read by the same warp");
@@ -60,7 +66,8 @@ template <int D>
 struct DqSmem {
   static constexpr int REC = 16 * (D / 2 + 2 * (D / 64));
   static constexpr int KV = (REC + 127) / 128 * 128;
-  static constexpr int STAGE = 2 * KV;
+  static constexpr int PAGE = 2 * KV;    // K and V of a page
+  static constexpr int STAGE = 2 * PAGE;
   static constexpr int RING = DQ_STAGES * STAGE;
   static constexpr int WARP = 8 * D + 16;  // floats a warp leaves for the merge: acc[head][d], m[8], l[8]
   static constexpr int BARS = RING + DQ_WARPS * WARP * 4;
@@ -108,6 +115,11 @@ __device__ __forceinline__ uint32_t lds16(uint32_t a) {
 __device__ __forceinline__ uint32_t add_h2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 __device__ __forceinline__ float lo_f32(uint32_t h2) { return __low2float(*reinterpret_cast<__half2*>(&h2)); }
@@ -181,7 +193,6 @@ __device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, 
 
 template <int D, bool SIDE>
 __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const DqParams p) {
-  pdl_launch();
   pdl_wait();
   using SM = DqSmem<D>;
   constexpr int NG = D / 64;
@@ -208,7 +219,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
   if (warp == DQ_WARPS) {
     // ---- producer: walks the block tables and brings one record of K and of V per page ------------
     const size_t rec_page = (size_t)p.G * SM::REC;
-    int j = 0;  // pages issued; a slot's phase follows from it
+    int j = 0;  // pairs issued; a slot's phase follows from it
     for (; left > 0; at.page = 0, ++at.hg) {
       if (at.hg == units) at.hg = 0, ++at.b;
       long long np = pages_of(p.lens[at.b]);
@@ -219,17 +230,20 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
         const long long col = at.page + j0 + lane;  // beyond the table: page 0
         const int mine = (j0 + lane < count && col < p.MP) ? p.table[(size_t)at.b * p.MP + col] : 0;
         const int lim = (int)min(32LL, count - j0);
-        for (int i = 0; i < lim; ++i, ++j) {
-          const int page = __shfl_sync(0xffffffffu, mine, i);
+        for (int i = 0; i < lim; i += 2, ++j) {
+          const int pa = __shfl_sync(0xffffffffu, mine, i), pb = __shfl_sync(0xffffffffu, mine, i + 1);
           if (lane == 0) {
-            const int s = j % DQ_STAGES;
+            const int s = j % DQ_STAGES, n = min(2, lim - i);
             mbar_wait(&empty[s], ((j / DQ_STAGES) & 1) ^ 1, p.status, 501);
-            mbar_expect_tx(&full[s], 2 * SM::REC);
+            mbar_expect_tx(&full[s], n * 2 * SM::REC);
             unsigned char* dst = smem + s * SM::STAGE;
-            const bool in = page >= 0 && page < p.NP;
-            const size_t off = (size_t)page * rec_page + head;
-            bulk_load(dst, in ? p.Kc + off : g_zero_record, SM::REC, &full[s]);
-            bulk_load(dst + SM::KV, in ? p.Vc + off : g_zero_record, SM::REC, &full[s]);
+            for (int e = 0; e < n; ++e, dst += SM::PAGE) {
+              const int page = e ? pb : pa;
+              const bool in = page >= 0 && page < p.NP;
+              const size_t off = (size_t)page * rec_page + head;
+              bulk_load(dst, in ? p.Kc + off : g_zero_record, SM::REC, &full[s]);
+              bulk_load(dst + SM::KV, in ? p.Vc + off : g_zero_record, SM::REC, &full[s]);
+            }
           }
         }
       }
@@ -245,18 +259,22 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
   const int tok_a = (gq >> 1) + 4 * (gq & 1), tok_b = tok_a + 8;
   const float sc2 = p.scale * LOG2E * TWO24;
   const uint32_t ring = smem_u32(smem);
-  int base = 0;  // pages of the CTA before this segment
+  const int side = SIDE ? t >> 1 : 0;  // the page of a pair whose scores this lane holds
+  int base = 0;  // pairs of the CTA before this segment
   for (; left > 0; at.page = 0, ++at.hg) {
     if (at.hg == units) at.hg = 0, ++at.b;
     int n = p.lens[at.b];
     while (n <= 0) n = p.lens[++at.b];
     const long long np = pages_of(n);
-    const int count = (int)min(np - at.page, left);
+    const int count = (int)min(np - at.page, left), pairs = (count + 1) / 2;
+    // Tokens of this segment: those behind it are another CTA's, or do not exist.
+    const int tokens = (int)min((long long)count * 16, (long long)n - at.page * 16);
     const int g = at.hg / p.hgroups, h0 = g * hq + (at.hg % p.hgroups) * 8, nh = min(8, hq - (at.hg % p.hgroups) * 8);
 
-    // Q as the B operand: column gq is head gq (SIDE: heads 0..3 twice), the rows of step k of group
-    // x are elements 64 x + 16 t + 2 k, + 1 and the same + 8, as the words of codes hold them.
-    uint32_t qf[NG][4][2];
+    // Q as the B operand: column gq is head gq (SIDE: head gq & 3, for page gq >> 2 of the pair), the
+    // rows of step k of group x are elements 64 x + 16 t + 2 k, + 1 and the same + 8, as the words of
+    // codes hold them; odd steps' nibbles weigh 16.
+    uint32_t qf[SIDE ? 2 : 1][NG][4][2];
     float qsum[NG][2];
     {
       const int hc = SIDE ? gq & 3 : gq;
@@ -269,63 +287,80 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
           lo = *reinterpret_cast<const uint4*>(q + 64 * x);
           hi = *reinterpret_cast<const uint4*>(q + 64 * x + 8);
         }
-        qf[x][0][0] = lo.x, qf[x][1][0] = lo.y, qf[x][2][0] = lo.z, qf[x][3][0] = lo.w;
-        qf[x][0][1] = hi.x, qf[x][1][1] = hi.y, qf[x][2][1] = hi.z, qf[x][3][1] = hi.w;
+        uint32_t w[4][2] = {{lo.x, hi.x}, {lo.y, hi.y}, {lo.z, hi.z}, {lo.w, hi.w}};
         float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s += lo_f32(qf[x][k][0]) + hi_f32(qf[x][k][0]) + lo_f32(qf[x][k][1]) + hi_f32(qf[x][k][1]);
+        for (int k = 0; k < 4; ++k) {
+          s += lo_f32(w[k][0]) + hi_f32(w[k][0]) + lo_f32(w[k][1]) + hi_f32(w[k][1]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t v = (k & 1) ? mul_h2(w[k][e], 0x2c002c00u) : w[k][e];  // 1/16
+            if (SIDE) {
+              qf[0][x][k][e] = gq < 4 ? v : 0u;
+              qf[SIDE][x][k][e] = gq < 4 ? 0u : v;
+            } else {
+              qf[0][x][k][e] = v;
+            }
+          }
+        }
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
-        qsum[x][0] = __shfl_sync(0xffffffffu, s, 8 * t);      // of head 2t
-        qsum[x][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);  // of head 2t + 1
+        qsum[x][0] = __shfl_sync(0xffffffffu, s, 8 * t);      // of column 2t
+        qsum[x][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);  // of column 2t + 1
       }
     }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    float F = 4294967296.0f * 64.0f / 4096.0f;  // for the smallest scale, 2^-20: the first page sets it
+    float F = 67108864.0f;  // fits the smallest scale, 2^-20: the first page sets it
     float acc[4 * NG][4], zacc[NG][2];
 #pragma unroll
     for (int i = 0; i < 4 * NG; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
     for (int x = 0; x < NG; ++x) zacc[x][0] = zacc[x][1] = 0.f;
 
-    for (int j = base + ((warp - base) & (DQ_WARPS - 1)); j < base + count; j += DQ_WARPS) {
-      const int s = j % DQ_STAGES;
-      mbar_wait(&full[s], (j / DQ_STAGES) & 1, p.status, 502);
-      const uint32_t kb = ring + s * SM::STAGE, vb = kb + SM::KV;
-      // Headers of this lane's two tokens: a pair of f16 (or one), scales and zero points (2^-24 units).
-      uint32_t hka, hkb, hva, hvb;
+    // One product's worth of tokens: a page, or (SIDE) a pair of pages at `pg`, `limit` tokens of them.
+    auto tile = [&](uint32_t pg, int limit) {
+      const uint32_t own = pg + side * SM::PAGE;  // the page of this lane's scores
+      uint32_t hka, hkb, hva, hvb;  // headers of its two tokens: a pair of f16 (or one)
       if (NG == 2) {
-        hka = lds32(kb + 8 * D + 4 * tok_a), hkb = lds32(kb + 8 * D + 4 * tok_b);
-        hva = lds32(vb + 8 * D + 4 * tok_a), hvb = lds32(vb + 8 * D + 4 * tok_b);
+        hka = lds32(own + 8 * D + 4 * tok_a), hkb = lds32(own + 8 * D + 4 * tok_b);
+        hva = lds32(own + SM::KV + 8 * D + 4 * tok_a), hvb = lds32(own + SM::KV + 8 * D + 4 * tok_b);
       } else {
-        hka = lds16(kb + 8 * D + 2 * tok_a), hkb = lds16(kb + 8 * D + 2 * tok_b);
-        hva = lds16(vb + 8 * D + 2 * tok_a), hvb = lds16(vb + 8 * D + 2 * tok_b);
+        hka = lds16(own + 8 * D + 2 * tok_a), hkb = lds16(own + 8 * D + 2 * tok_b);
+        hva = lds16(own + SM::KV + 8 * D + 2 * tok_a), hvb = lds16(own + SM::KV + 8 * D + 2 * tok_b);
       }
       // Tokens behind the last one: stale headers may be NaN, and the scores are masked below.
-      const long long tok0 = (at.page + j - base) * 16;
-      const bool tail = tok0 + 16 > n;
-      const bool ok_a = !tail || tok0 + tok_a < n, ok_b = !tail || tok0 + tok_b < n;
+      const bool tail = limit < (SIDE ? 32 : 16);
+      const bool ok_a = 16 * side + tok_a < limit, ok_b = 16 * side + tok_b < limit;
       if (tail) {
         if (!ok_a) hka = hva = 0;
         if (!ok_b) hkb = hvb = 0;
       }
-      float xa[2] = {0.f, 0.f}, xb[2] = {0.f, 0.f};  // scores of heads 2t, 2t + 1 in the log2 domain
+      float e[NG][4];
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
-        const uint2 wa = lds64(kb + tok_a * (D / 2) + 32 * x + 8 * t), wb = lds64(kb + tok_b * (D / 2) + 32 * x + 8 * t);
-        float e[4] = {0.f, 0.f, 0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};  // nibbles of weight 1, and of weight 16
-        mma16816(e, wa.x & 0x000f000fu, wb.x & 0x000f000fu, wa.y & 0x000f000fu, wb.y & 0x000f000fu, qf[x][0][0], qf[x][0][1]);
-        mma16816(o, wa.x & 0x00f000f0u, wb.x & 0x00f000f0u, wa.y & 0x00f000f0u, wb.y & 0x00f000f0u, qf[x][1][0], qf[x][1][1]);
-        const uint32_t ax = wa.x >> 8, bx = wb.x >> 8, ay = wa.y >> 8, by = wb.y >> 8;
-        mma16816(e, ax & 0x000f000fu, bx & 0x000f000fu, ay & 0x000f000fu, by & 0x000f000fu, qf[x][2][0], qf[x][2][1]);
-        mma16816(o, ax & 0x00f000f0u, bx & 0x00f000f0u, ay & 0x00f000f0u, by & 0x00f000f0u, qf[x][3][0], qf[x][3][1]);
+        e[x][0] = e[x][1] = e[x][2] = e[x][3] = 0.f;
+#pragma unroll
+        for (int s = 0; s < (SIDE ? 2 : 1); ++s) {
+          const uint32_t kb = pg + s * SM::PAGE + 32 * x + 8 * t;
+          const uint2 wa = lds64(kb + tok_a * (D / 2)), wb = lds64(kb + tok_b * (D / 2));
+          mma16816(e[x], wa.x & 0x000f000fu, wb.x & 0x000f000fu, wa.y & 0x000f000fu, wb.y & 0x000f000fu, qf[s][x][0][0], qf[s][x][0][1]);
+          mma16816(e[x], wa.x & 0x00f000f0u, wb.x & 0x00f000f0u, wa.y & 0x00f000f0u, wb.y & 0x00f000f0u, qf[s][x][1][0], qf[s][x][1][1]);
+          const uint32_t ax = wa.x >> 8, bx = wb.x >> 8, ay = wa.y >> 8, by = wb.y >> 8;
+          mma16816(e[x], ax & 0x000f000fu, bx & 0x000f000fu, ay & 0x000f000fu, by & 0x000f000fu, qf[s][x][2][0], qf[s][x][2][1]);
+          mma16816(e[x], ax & 0x00f000f0u, bx & 0x00f000f0u, ay & 0x00f000f0u, by & 0x00f000f0u, qf[s][x][3][0], qf[s][x][3][1]);
+        }
+      }
+      float xa[2], xb[2];  // scores of columns 2t, 2t + 1 in the log2 domain
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
         const uint32_t sa = hka & 0xfff0fff0u, za = hka & 0x000f000fu, sb = hkb & 0xfff0fff0u, zb = hkb & 0x000f000fu;
         const float ka = (x ? hi_f32(sa) : lo_f32(sa)) * sc2, kza = x ? hi_f32(za) : lo_f32(za);
         const float kbs = (x ? hi_f32(sb) : lo_f32(sb)) * sc2, kzb = x ? hi_f32(zb) : lo_f32(zb);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          xa[c] = fmaf(ka, fmaf(-kza, qsum[x][c], fmaf(o[c], 0.0625f, e[c])), xa[c]);
-          xb[c] = fmaf(kbs, fmaf(-kzb, qsum[x][c], fmaf(o[2 + c], 0.0625f, e[2 + c])), xb[c]);
+          const float ya = fmaf(-kza, qsum[x][c], e[x][c]), yb = fmaf(-kzb, qsum[x][c], e[x][2 + c]);
+          xa[c] = x ? fmaf(ka, ya, xa[c]) : ka * ya;
+          xb[c] = x ? fmaf(kbs, yb, xb[c]) : kbs * yb;
         }
       }
       if (tail) {
@@ -338,7 +373,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
         for (int c = 0; c < 2; ++c) {
           float mx = fmaxf(xa[c], xb[c]);
 #pragma unroll
-          for (int d = 4; d <= 16; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           mx = fmaxf(m[c], mx);
           const float f = m[c] == -INFINITY ? 0.f : ex2(m[c] - mx);  // (nothing to rescale before the first page)
           m[c] = mx;
@@ -381,27 +416,41 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
         const float a0 = pa[0] * sa, a1 = pa[1] * sa, b0 = pb[0] * sb, b1 = pb[1] * sb;
         zacc[x][0] = fmaf(b0, cb, fmaf(a0, ca, zacc[x][0]));
         zacc[x][1] = fmaf(b1, cb, fmaf(a1, ca, zacc[x][1]));
-        uint32_t pha = pack_h2(a0, a1), phb = pack_h2(b0, b1);
-        const uint32_t pla = pack_h2(a0 - lo_f32(pha), a1 - hi_f32(pha)), plb = pack_h2(b0 - lo_f32(phb), b1 - hi_f32(phb));
-        if (SIDE && t >= 2) pha = pla, phb = plb;  // columns 4..7: the same heads' low parts
+        const uint32_t pha = pack_h2(a0, a1), phb = pack_h2(b0, b1);
         const uint32_t bh0 = movm_t(pha), bh1 = movm_t(phb);
-        uint32_t bl0 = 0, bl1 = 0;
-        if (!SIDE) bl0 = movm_t(pla), bl1 = movm_t(plb);
-        // V^T: a lane's word gq of the group, for its four tokens; two tokens' halves side by side.
-        const uint32_t v = vb + 32 * x + 4 * gq + t * (D / 2);
-        const uint32_t w0 = lds32(v), w1 = lds32(v + 2 * D), w2 = lds32(v + 4 * D), w3 = lds32(v + 6 * D);
-        const uint32_t lo01 = __byte_perm(w0, w1, 0x5410), hi01 = __byte_perm(w0, w1, 0x7632);
-        const uint32_t lo23 = __byte_perm(w2, w3, 0x5410), hi23 = __byte_perm(w2, w3, 0x7632);
+        const uint32_t bl0 = movm_t(pack_h2(a0 - lo_f32(pha), a1 - hi_f32(pha)));
+        const uint32_t bl1 = movm_t(pack_h2(b0 - lo_f32(phb), b1 - hi_f32(phb)));
+        // SIDE: columns 0..3 of (bh, bl) are the first page's, 4..7 the second's. The first page's
+        // product takes its hi in columns 0..3 and its lo in 4..7, the second's the other way round.
+        uint32_t ol0 = 0, ol1 = 0;
+        if (SIDE) ol0 = __shfl_xor_sync(0xffffffffu, bl0, 16), ol1 = __shfl_xor_sync(0xffffffffu, bl1, 16);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // elements 2k, 2k + 1 of the word: rows gq, gq + 8
-          const int sh = (k >> 1) * 8;
-          const uint32_t mask = (k & 1) ? 0x00f000f0u : 0x000f000fu, centre = (k & 1) ? 0x80808080u : 0x80088008u;
-          const uint32_t a_0 = add_h2((lo01 >> sh) & mask, centre), a_1 = add_h2((hi01 >> sh) & mask, centre);
-          const uint32_t a_2 = add_h2((lo23 >> sh) & mask, centre), a_3 = add_h2((hi23 >> sh) & mask, centre);
-          mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bh0, bh1);
-          if (!SIDE) mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bl0, bl1);
+        for (int s = 0; s < (SIDE ? 2 : 1); ++s) {
+          const bool hi = !SIDE || (gq < 4) == (s == 0);
+          const uint32_t b_0 = hi ? bh0 : ol0, b_1 = hi ? bh1 : ol1;
+          // V^T: a lane's word gq of the group, for its four tokens; two tokens' halves side by side.
+          const uint32_t v = pg + s * SM::PAGE + SM::KV + 32 * x + 4 * gq + t * (D / 2);
+          const uint32_t w0 = lds32(v), w1 = lds32(v + 2 * D), w2 = lds32(v + 4 * D), w3 = lds32(v + 6 * D);
+          const uint32_t lo01 = __byte_perm(w0, w1, 0x5410), hi01 = __byte_perm(w0, w1, 0x7632);
+          const uint32_t lo23 = __byte_perm(w2, w3, 0x5410), hi23 = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // elements 2k, 2k + 1 of the word: rows gq, gq + 8
+            const int sh = (k >> 1) * 8;
+            const uint32_t mask = (k & 1) ? 0x00f000f0u : 0x000f000fu, centre = (k & 1) ? 0x80808080u : 0x80088008u;
+            const uint32_t a_0 = add_h2((lo01 >> sh) & mask, centre), a_1 = add_h2((hi01 >> sh) & mask, centre);
+            const uint32_t a_2 = add_h2((lo23 >> sh) & mask, centre), a_3 = add_h2((hi23 >> sh) & mask, centre);
+            mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, b_0, b_1);
+            if (!SIDE) mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bl0, bl1);
+          }
         }
       }
+    };
+
+    for (int j = base + ((warp - base) & (DQ_WARPS - 1)); j < base + pairs; j += DQ_WARPS) {
+      const int s = j % DQ_STAGES, limit = tokens - 32 * (j - base);
+      mbar_wait(&full[s], (j / DQ_STAGES) & 1, p.status, 502);
+      tile(ring + s * SM::STAGE, min(limit, 32));
+      if (!SIDE && limit > 16) tile(ring + s * SM::STAGE + SM::PAGE, min(limit - 16, 16));
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
     }
@@ -422,15 +471,17 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
     float* mine = (float*)(smem + SM::RING) + warp * SM::WARP;
     const float unit = TWO24 / F;
 #pragma unroll
-    for (int i = 0; i < 4 * NG; ++i) {
+    for (int i = 0; i < 4 * NG; i += 2) {
       const int d = 64 * (i >> 2) + 8 * gq + 2 * (i & 3);
-      const float w = (i & 1) ? 0.0625f * unit : unit;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        // SIDE: columns 4..7 are the low parts of heads 0..3; the zero points count once.
-        const float zz = SIDE && t >= 2 ? 0.f : z[i >> 2][c] * unit;
-        mine[(2 * t + c) * D + d] = fmaf(acc[i][c], w, zz);
-        mine[(2 * t + c) * D + d + 1] = fmaf(acc[i][2 + c], w, zz);
+        const float zz = z[i >> 2][c] * unit;
+        float4 v;
+        v.x = fmaf(acc[i][c], unit, zz);
+        v.y = fmaf(acc[i][2 + c], unit, zz);
+        v.z = fmaf(acc[i + 1][c], 0.0625f * unit, zz);
+        v.w = fmaf(acc[i + 1][2 + c], 0.0625f * unit, zz);
+        *reinterpret_cast<float4*>(mine + (2 * t + c) * D + d) = v;
       }
     }
     if (gq == 0) {
@@ -450,7 +501,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 #pragma unroll
       for (int w = 0; w < DQ_WARPS; ++w) {
         const float* a = all + w * SM::WARP;
-        const float mw = a[8 * D + hh], lw = a[8 * D + 8 + hh];
+        const float mw = a[8 * D + hh], lw = SIDE ? a[8 * D + 8 + hh] + a[8 * D + 12 + hh] : a[8 * D + 8 + hh];
         // A warp without a page has nothing; one whose scores were all NaN has a NaN sum.
         const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2(mw - mt);
         float v = a[hh * D + d];
@@ -472,10 +523,13 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       d[2] = 1 + (int)((np - count + share - 1) / share);
     }
     asm volatile("bar.sync 1, %0;" ::"r"(DQ_WARPS * 32) : "memory");
-    base += count;
+    base += pairs;
     left -= count;
   }
 
+  // Only now: the next kernel's CTAs, let in earlier, would take the places of this one's and make the
+  // equal shares unequal (256 sequences back to back: 229 us per launch instead of 149).
+  pdl_launch();
   // Rows without a cached token: 0/0, as decode_attention gives.
   for (int b = blockIdx.x; b < p.B; b += gridDim.x)
     if (p.lens[b] <= 0)
@@ -487,8 +541,8 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 // CTA's second slot and the first slots of the CTAs that follow. One warp per head.
 template <int D>
 __global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p) {
-  pdl_launch();
   pdl_wait();
+  pdl_launch();
   const int* d = p.desc + 4 * blockIdx.x;
   const int b = d[0], hg = d[1], pieces = d[2];
   if (pieces < 2) return;
