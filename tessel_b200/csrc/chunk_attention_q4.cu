@@ -1,0 +1,682 @@
+// Causal attention of pieces of prompts over the 4-bit cache (format: kv_q4.cuh), for pages of 16
+// tokens, head_dim 64 or 128 and at most 128 query heads per KV head; other shapes run on kv_q4.cu's
+// one-warp kernel.
+//
+// Mathematics: softmax(scale q K^T) V with an online softmax over 64 keys at a time, as
+// chunk_attention computes it: S = Q K^T and O += P V on tcgen05, O in tensor memory, rescaled only
+// when a row's maximum grew by more than 2^8; P is rounded to f16 for the second product (as
+// chunk_attention and prefill_attention round it; its relative error, 2^-11 at most and independent
+// from key to key, adds to the result about what the result's own rounding to f16 does), its sum is
+// kept in f32. K and V enter as f16 tiles; every value of the cache is an f16 number, so unpacking
+// rounds nothing.
+//
+// Roles of a CTA's sixteen warps: warp 0 brings Q (TMA) and the pages' 4-bit records (bulk copies);
+// warp 1 issues the MMAs; warps 4-7 unpack a 128-key tile of K or V into the 128-byte-swizzled layout
+// the tensor cores read; warps 8-15 are two softmax warpgroups, one query row per thread.
+//
+// Rows. The M = 128 rows of a tile are (token, query head) pairs of ONE KV head: 128 / hq tokens times
+// its hq heads. So a KV head's keys are unpacked once for all heads that share it, and a piece of a
+// few tokens still fills a tile hq times better than a tile per head would.
+//
+// Work split. A unit is (piece, KV head, block of two tiles); its work is the 128-key tiles its last
+// row sees. The units' tiles form one list, a CTA takes an equal, contiguous share of it (one CTA per
+// SM), whatever the pieces' lengths are. A unit that is cut leaves one partial in each CTA (f32
+// numerator, maximum and sum), which a second kernel joins.
+//
+// NaN. A weight of zero times a NaN is a NaN, so a spoilt V row would reach rows that do not see it.
+// The unpacking warps store zeros for it instead and note the least such position of each 64-column
+// group; a row at or behind it gets its NaN at the end.
+#include "kv_q4.cuh"
+
+namespace tb {
+
+namespace {
+
+constexpr int CQ_BM = 128;       // rows of a tile
+constexpr int CQ_BN = 128;       // keys of a K / V tile
+constexpr int CQ_SN = 64;        // keys of a sub-block: the unit of S, softmax and P V
+constexpr int CQ_THREADS = 512;  // 0 TMA, 1 MMA, (2, 3 idle), 4-7 unpack, 8-15 softmax
+constexpr int CQ_LEAST = 2;      // tiles a CTA takes at least
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float RESCALE_STEP = 8.0f;
+
+// What a table entry outside the cache reads as.
+__device__ __align__(128) unsigned char g_zero_record[2048];
+
+struct CqParams {
+  const unsigned char* Kc;
+  const unsigned char* Vc;
+  const int* table;
+  const int* meta;
+  __half* O;
+  float* part;  // [CTA][2][256][D + 2]: numerator, maximum, sum of a row
+  int* desc;    // [CTA][4]: piece, KV head, block, CTAs that hold a part of the unit cut at this CTA's end (0: none)
+  float scale;
+  int T, H, G, hq, tm, C, NP, MP, least;  // tm: tokens of a tile
+  unsigned int* status;
+};
+
+template <int D>
+struct CqSmem {
+  static constexpr int SUB = D / 64;
+  static constexpr int REC = 16 * (D / 2 + 2 * SUB);
+  static constexpr int Q_TILE = CQ_BM * D * 2;
+  static constexpr int KV_BYTES = CQ_BN * D * 2;
+  static constexpr int RAW = 8 * REC;  // a tile's records
+  static constexpr int NSLOT = 4;
+  static constexpr int NRAW = D == 128 ? 3 : 4;
+  static constexpr int OFF_KV = 2 * Q_TILE;
+  static constexpr int OFF_RAW = OFF_KV + NSLOT * KV_BYTES;
+  static constexpr int OFF_BAR = OFF_RAW + NRAW * RAW;
+  static constexpr int TOTAL = OFF_BAR + 40 * 8 + 1024;
+  static constexpr int TMEM_COLS = 512;
+  static_assert(TOTAL <= 227 * 1024, "shared memory");
+  static_assert(RAW % 128 == 0 && OFF_BAR % 8 == 0, "alignment");
+  static_assert((CQ_THREADS + 8) * 8 <= KV_BYTES, "the prefix sums use the first K / V slot");
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"((uint64_t)src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A piece of the step, empty if its descriptor does not lie inside it.
+struct Piece {
+  int row0, nrows, pos0, blocks;
+};
+__device__ __forceinline__ Piece piece_of(const CqParams& p, int c) {
+  const int* m = p.meta + 4 * c;
+  Piece r = {m[0], m[1], m[2], 0};
+  if (r.row0 < 0 || r.nrows <= 0 || r.pos0 < 0 || r.nrows > p.T - r.row0 || r.nrows > 0x7fffffff - 256 - r.pos0)
+    r.nrows = 0;
+  r.blocks = (r.nrows + 2 * p.tm - 1) / (2 * p.tm);
+  return r;
+}
+// Tiles of keys that block `i` of a piece sees.
+__device__ __forceinline__ int tiles_of(const CqParams& p, const Piece& r, int i) {
+  return (r.pos0 + min((i + 1) * 2 * p.tm, r.nrows) + CQ_BN - 1) / CQ_BN;
+}
+
+// Walks a CTA's share of the list: `k0`, `k1` are the tiles of the current unit that are its own.
+struct Walk {
+  int c, g, i, left, share;
+  Piece r;
+  int tiles, k0, k1;
+
+  __device__ __forceinline__ void set(const CqParams& p, int from) {
+    tiles = tiles_of(p, r, i);
+    k0 = from;
+    k1 = left < tiles - from ? from + left : tiles;
+    left -= k1 - k0;
+  }
+  // To the next unit; false at the end of the share.
+  __device__ __forceinline__ bool next(const CqParams& p) {
+    if (left <= 0) return false;
+    if (++i == r.blocks) {
+      i = 0;
+      if (++g == p.G) {
+        g = 0;
+        do r = piece_of(p, ++c);
+        while (r.blocks == 0);  // `left` says that one follows
+      }
+    }
+    set(p, 0);
+    return true;
+  }
+};
+
+// Where this CTA begins. All threads call it. False: it has no share.
+__device__ __forceinline__ bool find_walk(const CqParams& p, long long* scan, Walk* w) {
+  const int per = (p.C + CQ_THREADS - 1) / CQ_THREADS;
+  const int c0 = min(p.C, (int)threadIdx.x * per), c1 = min(p.C, c0 + per);
+  auto tiles_in = [&](int c) {
+    const Piece r = piece_of(p, c);
+    long long s = 0;
+    for (int i = 0; i < r.blocks; ++i) s += tiles_of(p, r, i);
+    return s;
+  };
+  long long sum = 0;
+  for (int c = c0; c < c1; ++c) sum += tiles_in(c);
+  scan[threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    constexpr int OWN = CQ_THREADS / 32;
+    long long own = 0;
+    for (int i = 0; i < OWN; ++i) own += scan[threadIdx.x * OWN + i];
+    long long inc = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+      if ((int)threadIdx.x >= o) inc += up;
+    }
+    long long at = inc - own;
+    for (int i = 0; i < OWN; ++i) {
+      const long long v = scan[threadIdx.x * OWN + i];
+      scan[threadIdx.x * OWN + i] = at;
+      at += v;
+    }
+    if (threadIdx.x == 31) scan[CQ_THREADS] = at;
+  }
+  __syncthreads();
+  const long long all = scan[CQ_THREADS] * p.G;
+  const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)p.least);
+  const long long start = blockIdx.x * share;
+  if (start >= all) return false;  // uniform for the CTA
+  long long at = scan[threadIdx.x] * p.G;
+  for (int c = c0; c < c1; ++c) {
+    const long long n = tiles_in(c);
+    if (start >= at && start < at + n * p.G) {
+      const Piece r = piece_of(p, c);
+      long long in = (start - at) % n;
+      int i = 0;
+      for (; in >= tiles_of(p, r, i); ++i) in -= tiles_of(p, r, i);
+      scan[CQ_THREADS + 1] = c, scan[CQ_THREADS + 2] = (start - at) / n, scan[CQ_THREADS + 3] = i, scan[CQ_THREADS + 4] = in;
+    }
+    at += n * p.G;
+  }
+  __syncthreads();
+  w->c = (int)scan[CQ_THREADS + 1], w->g = (int)scan[CQ_THREADS + 2], w->i = (int)scan[CQ_THREADS + 3];
+  w->share = (int)share;  // (2^31 tiles would be hours of work)
+  w->left = (int)min(share, all - start);
+  w->r = piece_of(p, w->c);
+  w->set(p, (int)scan[CQ_THREADS + 4]);
+  return true;
+}
+
+// Sub-blocks of keys that tile `t` of the current unit visits in this CTA's part, and its last key + 1.
+__device__ __forceinline__ int subs_of(const CqParams& p, const Walk& w, int t) {
+  const int first = w.i * 2 * p.tm + t * p.tm;
+  if (first >= w.r.nrows) return 0;
+  const int end = min(CQ_BN * w.k1, w.r.pos0 + min(first + p.tm, w.r.nrows));
+  return max(0, (end - CQ_BN * w.k0 + CQ_SN - 1) / CQ_SN);
+}
+
+template <int D>
+__global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_constant__ CUtensorMap mapQ, const CqParams p) {
+  pdl_wait();
+  using SM = CqSmem<D>;
+  constexpr int SUB = SM::SUB, NSLOT = SM::NSLOT, NRAW = SM::NRAW;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = (uint64_t*)(smem + SM::OFF_BAR);
+  uint64_t* q_full = bars;              // a unit's Q has landed
+  uint64_t* q_free = bars + 1;          // and its last S has been computed
+  uint64_t* raw_full = bars + 2;        // [NRAW]
+  uint64_t* raw_empty = bars + 6;       // [NRAW]
+  uint64_t* kv_full = bars + 10;        // [NSLOT]
+  uint64_t* kv_empty = bars + 14;       // [NSLOT]
+  uint64_t* s_full = bars + 18;         // [tile][buffer]
+  uint64_t* p_ready = bars + 22;        // [tile][buffer]
+  uint64_t* o_done = bars + 26;         // [tile][parity]
+  uint32_t* tmem_slot = (uint32_t*)(bars + 30);
+  int* nan_at = (int*)(bars + 31);      // [unit & 3][group]: least position of a spoilt V row
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) p.desc[4 * blockIdx.x + 3] = 0;
+  Walk w;
+  if (!find_walk(p, (long long*)(smem + SM::OFF_KV), &w)) {
+    pdl_launch();
+    return;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_free, 1);
+    for (int i = 0; i < NRAW; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 4);
+    }
+    for (int i = 0; i < NSLOT; ++i) {
+      mbar_init(&kv_full[i], 128);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], CQ_BM);
+      mbar_init(&o_done[i], 1);
+      nan_at[i] = nan_at[4 + i] = 0x7fffffff;
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, SM::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    if (warp == 0) {
+      // ---- Q and the records of K and V tiles, in the order K V K V ... -----------------------------
+      if (lane == 0) prefetch_tmap(&mapQ);
+      int item = 0, unit = 0;
+      do {
+        if (lane == 0) {
+          if (unit > 0) mbar_wait(q_free, (unit - 1) & 1, p.status, 601);
+          mbar_expect_tx(q_full, 2 * SUB * p.tm * p.hq * 128);
+          const int row = w.r.row0 + w.i * 2 * p.tm;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int sub = 0; sub < SUB; ++sub)
+              tma_load_3d(smem + t * SM::Q_TILE + sub * (CQ_BM * 128), &mapQ, q_full, sub * 64, w.g * p.hq, row + t * p.tm);
+        }
+        const int slim = w.r.pos0 + w.r.nrows;
+        for (int k = w.k0; k < w.k1; ++k) {
+          // Lane j < 8: the page of keys [128 k + 16 j, + 16). Beyond the table: page 0; behind the last
+          // key, or outside the cache: zeros.
+          const int col = k * 8 + (lane & 7);
+          int page = -1;
+          if (col * 16 < slim) page = col < p.MP ? p.table[(size_t)w.r.row0 * p.MP + col] : 0;
+          const bool in = page >= 0 && page < p.NP;
+          const size_t off = ((size_t)(in ? page : 0) * p.G + w.g) * SM::REC;
+#pragma unroll
+          for (int v = 0; v < 2; ++v, ++item) {
+            const int s = item % NRAW;
+            if (lane == 0) {
+              if (item >= NRAW) mbar_wait(&raw_empty[s], (item / NRAW - 1) & 1, p.status, 602);
+              mbar_expect_tx(&raw_full[s], SM::RAW);
+            }
+            __syncwarp();
+            if (lane < 8)
+              bulk_load(smem + SM::OFF_RAW + s * SM::RAW + lane * SM::REC, in ? (v ? p.Vc : p.Kc) + off : g_zero_record, SM::REC,
+                        &raw_full[s]);
+          }
+        }
+        ++unit;
+      } while (w.next(p));
+    } else if (warp == 1 && elect_one()) {
+      // ---- MMA issue -------------------------------------------------------------------------------
+      constexpr uint32_t idesc_s = umma_idesc_f16(CQ_BM, CQ_SN, 0, 0);
+      constexpr uint32_t idesc_o = umma_idesc_f16(CQ_BM, D, 0, 1);
+      int base = 0;             // K and V tiles of earlier units
+      int done[2] = {0, 0};     // sub-blocks of earlier units, per tile: buffers and phases follow from the running count
+      int ready = 0, unit = 0;  // tiles [0, ready) have been unpacked
+      auto slot_addr = [&](int item) { return smem_u32(smem + SM::OFF_KV + (item % NSLOT) * SM::KV_BYTES); };
+      auto need = [&](int item) {
+        while (ready <= item) {
+          mbar_wait(&kv_full[ready % NSLOT], (ready / NSLOT) & 1, p.status, 603);
+          ++ready;
+        }
+        tc_fence_after();
+      };
+      do {
+        const int nsub[2] = {subs_of(p, w, 0), subs_of(p, w, 1)};
+        const int nmax = max(nsub[0], nsub[1]), nitems = 2 * (w.k1 - w.k0);
+        auto issue_s = [&](int t, int n) {
+          const int b = (done[t] + n) & 1;
+          const uint32_t qa = smem_u32(smem + t * SM::Q_TILE);
+          const uint32_t ka = slot_addr(base + 2 * (n >> 1)) + (n & 1) * (CQ_SN * 128);
+#pragma unroll
+          for (int kd = 0; kd < D / 16; ++kd) {
+            const uint32_t off = (kd >> 2) * (CQ_BM * 128) + (kd & 3) * 32;
+            umma_f16(tmem + t * 128 + b * CQ_SN, umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024),
+                     idesc_s, kd > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[t * 2 + b]);
+        };
+        auto issue_pv = [&](int t, int n) {
+          const int b = (done[t] + n) & 1;
+          const uint32_t va = slot_addr(base + 2 * (n >> 1) + 1);
+#pragma unroll
+          for (int kk = 0; kk < CQ_SN / 16; ++kk)
+            umma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + b * CQ_SN + kk * 8,
+                        umma_desc_sw128(va + ((n & 1) * (CQ_SN / 16) + kk) * 2048, CQ_BN * 128, 1024), idesc_o,
+                        (n > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&o_done[t * 2 + b]);
+        };
+        mbar_wait(q_full, unit & 1, p.status, 604);
+        need(base);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (n < nsub[t]) issue_s(t, n);
+        umma_commit(&kv_empty[base % NSLOT]);  // K tile 0 is free once these are done
+        for (int n = 0; n < nmax; ++n) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (n < nsub[t]) {
+              const int b = done[t] + n;
+              mbar_wait(&p_ready[t * 2 + (b & 1)], (b >> 1) & 1, p.status, 605);
+              tc_fence_after();
+              need(base + 2 * (n >> 1) + 1);
+              issue_pv(t, n);
+            }
+            if (n + 2 < nsub[t]) {
+              need(base + 2 * ((n + 2) >> 1));
+              issue_s(t, n + 2);
+            }
+          }
+          if (n & 1) {
+            // Both halves of V tile n >> 1 and of K tile (n >> 1) + 1 have been issued for both tiles.
+            umma_commit(&kv_empty[(base + n) % NSLOT]);
+            if (n + 1 < nitems) umma_commit(&kv_empty[(base + n + 1) % NSLOT]);
+          }
+        }
+        umma_commit(q_free);
+        // Tiles that the loop did not give back: the last V tile where the sub-blocks are odd, and (a part
+        // without a row that sees it) whole tiles. They are unpacked all the same.
+        need(base + nitems - 1);
+        for (int n = nmax < 1 ? 1 : (nmax & 1) ? nmax : nmax + 1; n < nitems; ++n) umma_commit(&kv_empty[(base + n) % NSLOT]);
+        base += nitems;
+        done[0] += nsub[0], done[1] += nsub[1];
+        ++unit;
+      } while (w.next(p));
+    }
+  } else if (warp < 8) {
+    // ---- unpack: a thread takes 32 neighbouring elements of a key at a time ---------------------------
+    constexpr int PARTS = D / 32;  // 16-byte pieces of a row of codes
+    const int tid = threadIdx.x - 128, part = tid % PARTS;
+    int item = 0, unit = 0;
+    do {
+      const int slim = w.r.pos0 + w.r.nrows;
+      for (int k = w.k0; k < w.k1; ++k) {
+#pragma unroll 1
+        for (int v = 0; v < 2; ++v, ++item) {
+          const int rs = item % NRAW, s = item % NSLOT;
+          mbar_wait(&raw_full[rs], (item / NRAW) & 1, p.status, 606);
+          if (item >= NSLOT) mbar_wait(&kv_empty[s], (item / NSLOT - 1) & 1, p.status, 607);
+          const unsigned char* raw = smem + SM::OFF_RAW + rs * SM::RAW;
+          unsigned char* dst = smem + SM::OFF_KV + s * SM::KV_BYTES;
+#pragma unroll 4
+          for (int key = tid / PARTS; key < CQ_BN; key += 128 / PARTS) {
+            const unsigned char* rec = raw + (key >> 4) * SM::REC;
+            uint4 u = *reinterpret_cast<const uint4*>(rec + (key & 15) * (D / 2) + part * 16);
+            uint32_t head = *reinterpret_cast<const unsigned short*>(rec + 8 * D + 2 * ((key & 15) * SUB + (part >> 1)));
+            if (k * CQ_BN + key >= slim) head = 0;  // stale behind the last key
+            if (v && (head & 0x7c00u) == 0x7c00u) {
+              atomicMin(&nan_at[(unit & 3) * 2 + (part >> 1)], k * CQ_BN + key);
+              head = 0;
+            }
+            const uint32_t z = head & 15u;
+            uint32_t sc = head & 0xfff0u, c0 = 0xe400u | z, c1 = 0xd400u | (z << 4);  // scale, -(1024 + z), -(64 + z)
+            sc |= sc << 16, c0 |= c0 << 16, c1 |= c1 << 16;
+            const __half2 S = *reinterpret_cast<__half2*>(&sc), A = *reinterpret_cast<__half2*>(&c0), B = *reinterpret_cast<__half2*>(&c1);
+            const __half2 R = __float2half2_rn(0.0625f);
+            // Pieces 2 and 3 lie in the other 64-column block, at the same banks: they go in another order.
+            if (part & 2) {
+              uint32_t x = u.x;
+              u.x = u.z, u.z = x, x = u.y, u.y = u.w, u.w = x;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t word = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w, up = word >> 8;
+              uint32_t e[4] = {(word & 0x000f000fu) | 0x64006400u, (word & 0x00f000f0u) | 0x64006400u,
+                               (up & 0x000f000fu) | 0x64006400u, (up & 0x00f000f0u) | 0x64006400u};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                __half2 x = *reinterpret_cast<__half2*>(&e[j]);
+                x = (j & 1) ? __hfma2(x, R, B) : __hadd2(x, A);  // code - zero point, exactly
+                x = __hmul2(x, S);
+                e[j] = *reinterpret_cast<uint32_t*>(&x);
+              }
+              const int ch = ((part & 1) * 4 + (i ^ (part & 2))) ^ (key & 7);
+              *reinterpret_cast<uint4*>(dst + (part >> 1) * (CQ_BN * 128) + key * 128 + ch * 16) = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+          }
+          fence_proxy_async();
+          mbar_arrive(&kv_full[s]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&raw_empty[rs]);
+        }
+      }
+      ++unit;
+    } while (w.next(p));
+  } else {
+    // ---- softmax: one warpgroup per tile, one row (TMEM lane) per thread -------------------------------
+    const int t = (warp - 8) >> 2;
+    const int q = warp & 3;  // TMEM lane quadrant this warp may touch
+    const int rit = q * 32 + lane;
+    const int tok = rit / p.hq, head = rit % p.hq;
+    const float sc2 = p.scale * LOG2E;
+    const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+    const uint32_t tmem_s = tmem + lane_base + t * 128;
+    const uint32_t tmem_o = tmem + lane_base + 256 + t * D;
+    int base = 0, unit = 0;
+    do {
+      const int nt = subs_of(p, w, t);
+      const int local = w.i * 2 * p.tm + t * p.tm + tok;  // the row within its piece
+      const bool live = tok < p.tm && local < w.r.nrows;
+      const int row = w.r.pos0 + local;
+      float m_ref = -1e30f, l = 0.f;
+      for (int n = 0; n < nt; ++n) {
+        const int cnt = base + n, b = cnt & 1;
+        const int key0 = w.k0 * CQ_BN + n * CQ_SN;
+        mbar_wait(&s_full[t * 2 + b], (cnt >> 1) & 1, p.status, 608);
+        tc_fence_after();
+        uint32_t sv[CQ_SN];
+#pragma unroll
+        for (int c = 0; c < CQ_SN / 32; ++c) tmem_ld32(tmem_s + b * CQ_SN + c * 32, sv + c * 32);
+        tmem_ld_wait();
+        float mx;
+        if (key0 + CQ_SN - 1 <= row) {
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < CQ_SN; i += 4)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], __uint_as_float(sv[i + u]));
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        } else {
+          mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < CQ_SN; ++i) {
+            const float x = key0 + i <= row ? __uint_as_float(sv[i]) : -INFINITY;
+            sv[i] = __float_as_uint(x);
+            mx = fmaxf(mx, x);
+          }
+        }
+        mx *= sc2;  // log2 domain (the scale is positive)
+        const float m_new = fmaxf(m_ref, mx);
+        const bool grow = m_new > m_ref + RESCALE_STEP;
+        if (n == 0) {
+          m_ref = m_new;
+        } else if (__any_sync(0xffffffffu, grow)) {
+          // O must be quiescent: S(n) was issued behind P V(n - 2), so only P V(n - 1) can still run.
+          mbar_wait(&o_done[t * 2 + ((cnt - 1) & 1)], ((cnt - 1) >> 1) & 1, p.status, 609);
+          tc_fence_after();
+          const float f = grow ? exp2f(m_ref - m_new) : 1.0f;
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 8) {
+            uint32_t ov[8];
+            tmem_ld8(tmem_o + c0, ov);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+            tmem_st8(tmem_o + c0, ov);
+          }
+          l *= f;
+          if (grow) m_ref = m_new;
+        }
+        float sum = 0.f;
+        // Eight columns at a time, so that scores and weights are not all live at once. (All scores are in
+        // registers: overwriting the buffer's first columns loses nothing.)
+#pragma unroll
+        for (int c = 0; c < CQ_SN / 16; ++c) {
+          uint32_t pk[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float a = ex2(fmaf(__uint_as_float(sv[16 * c + 2 * i]), sc2, -m_ref));
+            const float b2 = ex2(fmaf(__uint_as_float(sv[16 * c + 2 * i + 1]), sc2, -m_ref));
+            sum += a + b2;
+            pk[i] = pack_h2(a, b2);
+          }
+          tmem_st8(tmem_s + b * CQ_SN + 8 * c, pk);
+        }
+        tmem_st_wait();
+        l += sum;
+        tc_fence_before();
+        mbar_arrive(&p_ready[t * 2 + b]);
+      }
+      if (nt > 0) {
+        // The last two products may still be running.
+        const int cnt = base + nt;
+        if (nt > 1) mbar_wait(&o_done[t * 2 + ((cnt - 2) & 1)], ((cnt - 2) >> 1) & 1, p.status, 610);
+        mbar_wait(&o_done[t * 2 + ((cnt - 1) & 1)], ((cnt - 1) >> 1) & 1, p.status, 611);
+        tc_fence_after();
+      }
+      const bool whole = w.k0 == 0 && w.k1 == w.tiles;
+      if (whole) {
+        // (Every live row of a whole unit sees a key, so its tile has sub-blocks.)
+        const float inv = 1.0f / l;
+        __half* o = p.O + ((size_t)(w.r.row0 + local) * p.H + w.g * p.hq + head) * D;
+#pragma unroll 1
+        for (int c0 = 0; nt > 0 && c0 < D; c0 += 32) {
+          uint32_t ov[32];
+          tmem_ld32(tmem_o + c0, ov);
+          tmem_ld_wait();
+          if (live) {
+            const float f = nan_at[(unit & 3) * 2 + (c0 >> 6)] <= row ? __int_as_float(0x7fc00000) : inv;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 y;
+              y.x = pack_h2(__uint_as_float(ov[i]) * f, __uint_as_float(ov[i + 1]) * f);
+              y.y = pack_h2(__uint_as_float(ov[i + 2]) * f, __uint_as_float(ov[i + 3]) * f);
+              y.z = pack_h2(__uint_as_float(ov[i + 4]) * f, __uint_as_float(ov[i + 5]) * f);
+              y.w = pack_h2(__uint_as_float(ov[i + 6]) * f, __uint_as_float(ov[i + 7]) * f);
+              *reinterpret_cast<uint4*>(o + c0 + i) = y;
+            }
+          }
+        }
+      } else {
+        float* part = p.part + (((size_t)blockIdx.x * 2 + (w.k0 == 0 ? 1 : 0)) * 256 + t * 128 + rit) * (D + 2);
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t ov[32];
+          if (nt > 0) {
+            tmem_ld32(tmem_o + c0, ov);
+            tmem_ld_wait();
+          }
+          if (live) {
+            const float f = nt == 0 ? 0.f : nan_at[(unit & 3) * 2 + (c0 >> 6)] <= row ? __int_as_float(0x7fc00000) : 1.0f;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              *reinterpret_cast<float2*>(part + c0 + i) = nt == 0 ? make_float2(0.f, 0.f) : make_float2(__uint_as_float(ov[i]) * f, __uint_as_float(ov[i + 1]) * f);
+          }
+        }
+        if (live) part[D] = m_ref, part[D + 1] = l;
+        if (t == 0 && rit == 0 && w.k0 == 0) {
+          // Cut at this CTA's end: the next CTAs go on with it.
+          int* d = p.desc + 4 * blockIdx.x;
+          d[0] = w.c, d[1] = w.g, d[2] = w.i;
+          d[3] = 1 + (int)((w.tiles - w.k1 + w.share - 1) / w.share);
+        }
+      }
+      base += nt;
+      // This unit's marks are free again once all softmax threads are through with them. The unpacking
+      // warps are at most two units (four tiles) ahead of the products, so four sets are enough.
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (threadIdx.x == 256) nan_at[(unit & 3) * 2] = nan_at[(unit & 3) * 2 + 1] = 0x7fffffff;
+      ++unit;
+    } while (w.next(p));
+  }
+  tc_fence_before();
+  __syncthreads();
+  pdl_launch();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, SM::TMEM_COLS);
+  }
+}
+
+// Joins the partials of the unit that is cut at the end of CTA blockIdx.x, if there is one: that
+// CTA's second slot and the first slots of the CTAs that follow. A warp per row, 8 rows per block of y.
+template <int D>
+__global__ void __launch_bounds__(256) chunk_q4_join_kernel(const CqParams p) {
+  pdl_wait();
+  pdl_launch();
+  const int* d = p.desc + 4 * blockIdx.x;
+  const int pieces = d[3];
+  if (pieces < 2) return;
+  const Piece r = piece_of(p, d[0]);
+  const int g = d[1], i = d[2], lane = threadIdx.x & 31;
+  for (int rr = blockIdx.y * 8 + (threadIdx.x >> 5); rr < 256; rr += gridDim.y * 8) {
+    const int t = rr >> 7, tok = (rr & 127) / p.hq, head = (rr & 127) % p.hq;
+    const int local = i * 2 * p.tm + t * p.tm + tok;
+    if (tok >= p.tm || local >= r.nrows) continue;
+    auto slot = [&](int k) { return p.part + (((size_t)(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * 256 + rr) * (D + 2); };
+    float m = -INFINITY;
+    for (int k = lane; k < pieces; k += 32) m = fmaxf(m, slot(k)[D]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f, a[D / 32];
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) a[k] = 0.f;
+    for (int k = 0; k < pieces; ++k) {
+      const float* s = slot(k);
+      const float f = ex2(s[D] - m);
+      l = fmaf(s[D + 1], f, l);
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) a[e] = fmaf(s[lane + 32 * e], f, a[e]);
+    }
+    __half* o = p.O + ((size_t)(r.row0 + local) * p.H + g * p.hq + head) * D;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) o[lane + 32 * e] = __float2half_rn(a[e] / l);
+  }
+}
+
+}  // namespace
+
+bool chunk_q4_takes(const Q4Shape& q, int T, int H, int C, int MP) {
+  return q.P == 16 && (q.D == 64 || q.D == 128) && q.NP > 0 && MP > 0 && T > 0 && C > 0 && H / q.G <= CQ_BM;
+}
+
+int make_chunk_q4(Ctx* c, Op& op, const Q4Shape& q) {
+  op.p1 = c->sm_count;
+  op.scratch_bytes = (size_t)op.p1 * (2 * 256 * (q.D + 2) * sizeof(float) + 16);
+  TB_CUDA(c, cudaMalloc(&op.scratch, op.scratch_bytes));
+  if (q.D == 128)
+    TB_CUDA(c, cudaFuncSetAttribute(chunk_q4_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, CqSmem<128>::TOTAL));
+  else
+    TB_CUDA(c, cudaFuncSetAttribute(chunk_q4_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, CqSmem<64>::TOTAL));
+  return 0;
+}
+
+int launch_chunk_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
+  const auto& s = op.shapes;
+  CqParams p;
+  p.T = (int)s[0][0], p.H = (int)s[0][1], p.G = q.G, p.hq = p.H / p.G, p.tm = CQ_BM / p.hq;
+  p.C = (int)s[4][0], p.NP = q.NP, p.MP = (int)s[3][1];
+  const uint64_t key[4] = {a[0], 0, 0, 0};
+  const MapEntry* hit = op.find_maps(key);
+  if (!hit) {
+    // Q [T, H, D]: one box = the group's heads of tm tokens, 64 columns.
+    const uint64_t dims[3] = {(uint64_t)q.D, (uint64_t)p.H, (uint64_t)p.T};
+    const uint64_t strides[2] = {(uint64_t)q.D * 2, (uint64_t)p.H * q.D * 2};
+    const uint32_t box[3] = {64, (uint32_t)p.hq, (uint32_t)p.tm};
+    CUtensorMap m;
+    if (make_tensor_map(c, &m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (const void*)a[0], dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return 1;
+    MapEntry* e = op.fresh_maps(key);
+    e->m[0] = m;
+    hit = e;
+  }
+  p.Kc = (const unsigned char*)a[1];
+  p.Vc = (const unsigned char*)a[2];
+  p.table = (const int*)a[3];
+  p.meta = (const int*)a[4];
+  p.O = (__half*)a[5];
+  p.scale = bits_f32(a[6]);
+  p.least = CQ_LEAST;
+  p.status = c->status;
+  p.part = (float*)op.scratch;
+  p.desc = (int*)(p.part + (size_t)op.p1 * 2 * 256 * (q.D + 2));
+  const dim3 grid(op.p1), join(op.p1, 8);
+  if (q.D == 128) {
+    TB_CUDA(c, launch_k(c, chunk_q4_kernel<128>, grid, dim3(CQ_THREADS), CqSmem<128>::TOTAL, 1, hit->m[0], p));
+    TB_CUDA(c, launch_k(c, chunk_q4_join_kernel<128>, join, dim3(256), 0, 1, p));
+  } else {
+    TB_CUDA(c, launch_k(c, chunk_q4_kernel<64>, grid, dim3(CQ_THREADS), CqSmem<64>::TOTAL, 1, hit->m[0], p));
+    TB_CUDA(c, launch_k(c, chunk_q4_join_kernel<64>, join, dim3(256), 0, 1, p));
+  }
+  c->launches += 2;
+  return 0;
+}
+
+}  // namespace tb

@@ -303,8 +303,9 @@ int make_kv_q4(Ctx* c, Op& op) {
       if ((why = q4_shape(op, 1, s[0][2], &q))) return bad(why);
       if (s[0][1] < 1 || s[0][1] % q.G) return bad("heads must be a multiple of kv heads");
       if (chunk && s[4][0] > 65535) return bad("at most 65535 chunks");
-      op.p0 = !chunk && decode_q4_takes(q, (int)s[0][0], (int)s[3][1]);
-      return op.p0 ? make_decode_q4(c, op, q) : 0;
+      const int T = (int)s[0][0], H = (int)s[0][1], MP = (int)s[3][1];
+      op.p0 = chunk ? chunk_q4_takes(q, T, H, (int)s[4][0], MP) : decode_q4_takes(q, T, MP);
+      return !op.p0 ? 0 : chunk ? make_chunk_q4(c, op, q) : make_decode_q4(c, op, q);
     }
     case K_PAGE_COPY:
       if (s[0].size() != 1 || s[1].size() != 2 || s[1][1] != 2) return bad("shapes are caches i64[A], pairs[N,2]");
@@ -351,7 +352,9 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
         if (!aligned_to(a[i], 16)) return bad("Q, O and the caches must be 16-byte aligned");
       const unsigned blocks = (unsigned)(((long long)T * H + 3) / 4);
       if (T == 0) return 0;
-      if (op.p0) return launch_decode_q4(c, op, a, q);
+      if (op.p0 && op.kind == K_DECODE_ATTENTION_Q4) return launch_decode_q4(c, op, a, q);
+      // (The tensor-core kernel masks before it scales, and takes the maximum of the unscaled scores.)
+      if (op.p0 && bits_f32(a[6]) > 0.f && bits_f32(a[6]) < INFINITY) return launch_chunk_q4(c, op, a, q);
       if (op.kind == K_DECODE_ATTENTION_Q4) {
         TB_CUDA(c, launch_k(c, decode_q4_generic_kernel, dim3(blocks), dim3(128), 0, 1, (const __half*)a[0],
                             (const unsigned char*)a[1], (const unsigned char*)a[2], (const int*)a[3], (const int*)a[4],

@@ -54,6 +54,10 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a);
 bool decode_q4_takes(const Q4Shape& q, int B, int MP);
 int make_decode_q4(Ctx* c, Op& op, const Q4Shape& q);
 int launch_decode_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q);
+// And behind chunk_attention_q4 (chunk_attention_q4.cu).
+bool chunk_q4_takes(const Q4Shape& q, int T, int H, int C, int MP);
+int make_chunk_q4(Ctx* c, Op& op, const Q4Shape& q);
+int launch_chunk_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q);
 
 #ifdef __CUDACC__
 
