@@ -5,9 +5,11 @@
 // query q: q.k = sum over groups of s (q.u - z sum(q)); so the tensor cores multiply q by the raw
 // codes and the scale and zero point come in afterwards, once per (token, head, group). For the
 // values, o = sum_t p_t s_t (u_t - z_t) = sum_t P_t (u_t - 8) + sum_t P_t (8 - z_t) with P = p s:
-// the scale rides on the weight, the second sum is one number per (head, group). Codes are centred
-// by 8 because all-positive products would make the accumulator hundreds of times larger than the
-// result of a long context, and the tensor cores' sums are not rounded to nearest.
+// the scale rides on the weight, the second sum is one number per (head, group). The -8 comes in as a
+// second product with a constant operand right behind the codes' own: without it the all-positive
+// products would make the accumulator hundreds of times larger than the result of a long context,
+// and the tensor cores' sums are not rounded to nearest. (A product costs less than centring the
+// operands: one instruction instead of four.)
 //
 // A code becomes an f16 operand by one AND: the nibble in the low bits of an f16 is the subnormal
 // u 2^-24, the next nibble 16 u 2^-24, and the tensor cores take subnormals as they are. For the
@@ -23,23 +25,23 @@
 //
 // Bound: HBM bytes, 2 (D/2 + 2 D/64) per token and KV head, with the issue slots close behind.
 //
-// Work split. A CTA takes an equal share of the step's (sequence, KV head, page) list, whatever the
-// lengths are: it finds its place from the lengths, walks through as many (sequence, head) units as
-// its share covers, and writes O itself for units that lie wholly inside. A unit that is cut leaves
-// one partial in each CTA; a second, tiny kernel joins them.
+// Work split. Every warp works on its own: it takes an equal share of the step's (sequence, KV head,
+// page) list, whatever the lengths are, finds its place from the lengths, brings its pages through a
+// ring of its own (bulk copies it issues itself, a few pairs of pages ahead, across units), and
+// writes O for units that lie wholly inside its share. A unit that is cut leaves one partial with
+// each warp; a second, tiny kernel joins them.
 #include "kv_q4.cuh"
 
 namespace tb {
 
 namespace {
 
-constexpr int DQ_WARPS = 4;                       // consumer warps
-constexpr int DQ_THREADS = (DQ_WARPS + 1) * 32;   // + one producer warp
-constexpr int DQ_STAGES = 8;                      // pairs of pages in flight per CTA
-constexpr int DQ_CTAS = 3;                        // per SM
-constexpr int DQ_LEAST = 8;                       // pages a CTA takes at least: two per warp
-constexpr int DQ_SLOT = 8;                        // heads of a partial
-static_assert(DQ_STAGES % DQ_WARPS == 0, "a slot is always read by the same warp");
+constexpr int DQ_WARPS = 4;
+constexpr int DQ_THREADS = DQ_WARPS * 32;
+constexpr int DQ_STAGES = 3;  // pairs of pages in a warp's ring
+constexpr int DQ_CTAS = 4;    // per SM
+constexpr int DQ_LEAST = 8;   // pages a warp takes at least
+constexpr int DQ_SLOT = 8;    // heads of a partial
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float TWO24 = 16777216.0f;
 constexpr float GROW = 8.0f;        // the running maximum is renewed when a score passes it by this (log2): p <= 2^8
@@ -55,8 +57,8 @@ struct DqParams {
   const int* table;
   const int* lens;
   __half* O;
-  float* part;  // [CTA][2][8][D + 2]: accumulators, then maximum and sum, per head
-  int* desc;    // [CTA][4]: sequence, head group, CTAs that hold a piece of the unit cut at this CTA's end (0: none)
+  float* part;  // [warp][2][8][D + 2]: accumulators [8][D], then maxima [8] and sums [8]
+  int* desc;    // [warp][4]: sequence, head group, warps that hold a piece of the unit cut at this warp's end (0: none)
   float scale;
   int B, H, G, NP, MP, hgroups, least;
   unsigned int* status;
@@ -65,14 +67,12 @@ struct DqParams {
 template <int D>
 struct DqSmem {
   static constexpr int REC = 16 * (D / 2 + 2 * (D / 64));
-  static constexpr int KV = (REC + 127) / 128 * 128;
-  static constexpr int PAGE = 2 * KV;    // K and V of a page
+  static constexpr int PAGE = 2 * REC;  // K and V of a page
   static constexpr int STAGE = 2 * PAGE;
-  static constexpr int RING = DQ_STAGES * STAGE;
-  static constexpr int WARP = 8 * D + 16;  // floats a warp leaves for the merge: acc[head][d], m[8], l[8]
-  static constexpr int BARS = RING + DQ_WARPS * WARP * 4;
-  static constexpr int SCAN = BARS + 2 * DQ_STAGES * 8;  // long long [DQ_THREADS + 1], then the CTA's start
-  static constexpr int TOTAL = SCAN + (DQ_THREADS + 4) * 8 + 128;
+  static constexpr int RING = DQ_STAGES * STAGE;                // of one warp
+  static constexpr int BARS = DQ_WARPS * RING;
+  static constexpr int SCAN = BARS + DQ_WARPS * DQ_STAGES * 8;  // long long [DQ_THREADS + 1], then the warps' places
+  static constexpr int TOTAL = SCAN + (DQ_THREADS + 1 + 2 * DQ_WARPS) * 8 + 128;
 };
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -82,12 +82,12 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 __device__ __forceinline__ uint32_t movm_t(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -112,11 +112,6 @@ __device__ __forceinline__ uint32_t lds16(uint32_t a) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
   return v;
 }
-__device__ __forceinline__ uint32_t add_h2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
 __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -134,62 +129,78 @@ struct Place {
 
 __device__ __forceinline__ long long pages_of(int n) { return n > 0 ? ((long long)n + 15) / 16 : 0; }
 
-// The number of (unit, page) items, the share of a CTA, and where CTA `cta` begins. All threads call it.
-__device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, long long cta, long long* total,
-                                            long long* share) {
-  const int units = p.G * p.hgroups;
+// The number of (unit, page) items, the share of a warp, and where this one begins. All threads call it.
+__device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, long long* total, long long* share) {
+  const int units = p.G * p.hgroups, lane = threadIdx.x & 31;
   const int per = (p.B + DQ_THREADS - 1) / DQ_THREADS;
   const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
   long long sum = 0;
   for (int b = b0; b < b1; ++b) sum += pages_of(p.lens[b]);
-  scan[threadIdx.x] = sum;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    // Exclusive prefix of the threads' sums: a lane owns DQ_WARPS + 1 neighbours.
-    constexpr int OWN = DQ_THREADS / 32;
-    long long own = 0;
-    for (int i = 0; i < OWN; ++i) own += scan[threadIdx.x * OWN + i];
-    long long inc = own;
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-      if ((int)threadIdx.x >= o) inc += up;
-    }
-    long long at = inc - own;
-    for (int i = 0; i < OWN; ++i) {
-      const long long v = scan[threadIdx.x * OWN + i];
-      scan[threadIdx.x * OWN + i] = at;
-      at += v;
-    }
-    if (threadIdx.x == 31) scan[DQ_THREADS] = at;
+  // Exclusive prefix of the threads' sums.
+  long long inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += up;
   }
+  if (lane == 31) scan[threadIdx.x >> 5] = inc;
   __syncthreads();
-  const long long all = scan[DQ_THREADS] * units;
-  const long long w = max((all + gridDim.x - 1) / gridDim.x, (long long)p.least);
-  const long long start = cta * w;
+  long long before = inc - sum, pages = 0;
+#pragma unroll
+  for (int w = 0; w < DQ_WARPS; ++w) {
+    if (w < (int)(threadIdx.x >> 5)) before += scan[w];
+    pages += scan[w];
+  }
+  const long long all = pages * units, workers = (long long)gridDim.x * DQ_WARPS;
+  const long long s = max((all + workers - 1) / workers, (long long)p.least);
   *total = all;
-  *share = w;
-  // The thread whose sequences hold `start` says which one.
-  if (start < all) {
-    long long at = scan[threadIdx.x] * units;
-    for (int b = b0; b < b1; ++b) {
-      const long long np = pages_of(p.lens[b]);
-      if (start >= at && start < at + np * units) {
-        scan[DQ_THREADS + 1] = b;
-        scan[DQ_THREADS + 2] = start - at;
+  *share = s;
+  // The thread whose sequences hold a warp's start says which one.
+  long long at = before * units;
+  for (int b = b0; b < b1; ++b) {
+    const long long end = at + pages_of(p.lens[b]) * units;
+#pragma unroll
+    for (int w = 0; w < DQ_WARPS; ++w) {
+      const long long start = ((long long)blockIdx.x * DQ_WARPS + w) * s;
+      if (start >= at && start < end) {
+        scan[DQ_WARPS + 2 * w] = b;
+        scan[DQ_WARPS + 2 * w + 1] = start - at;
       }
-      at += np * units;
     }
+    at = end;
   }
   __syncthreads();
   Place r = {0, 0, 0};
-  if (start < all) {
-    r.b = (int)scan[DQ_THREADS + 1];
-    const long long np = pages_of(p.lens[r.b]), in = scan[DQ_THREADS + 2];
+  if (((long long)blockIdx.x * DQ_WARPS + (threadIdx.x >> 5)) * s < all) {
+    r.b = (int)scan[DQ_WARPS + 2 * (threadIdx.x >> 5)];
+    const long long np = pages_of(p.lens[r.b]), in = scan[DQ_WARPS + 2 * (threadIdx.x >> 5) + 1];
     r.hg = (int)(in / np);
     r.page = in % np;
   }
   return r;
 }
+
+// A walk along a warp's share: the current unit's pages [at.page, at.page + count) are its own.
+struct Walk {
+  Place at;
+  long long left, np;
+  int n, count;
+  __device__ __forceinline__ void set(const DqParams& p) {
+    n = p.lens[at.b];
+    while (n <= 0) n = p.lens[++at.b];  // (only at the start of a sequence; `left` says that one follows)
+    np = pages_of(n);
+    count = (int)min(np - at.page, left);
+    left -= count;
+  }
+  // To the next unit; false at the end of the share.
+  __device__ __forceinline__ bool next(const DqParams& p, int units) {
+    if (left <= 0) return false;
+    at.page = 0;
+    if (++at.hg == units) at.hg = 0, ++at.b;
+    set(p);
+    return true;
+  }
+};
 
 template <int D, bool SIDE>
 __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const DqParams p) {
@@ -198,77 +209,80 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
   constexpr int NG = D / 64;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 127) & ~(uintptr_t)127);
-  uint64_t* full = (uint64_t*)(smem + SM::BARS);
-  uint64_t* empty = full + DQ_STAGES;
-  long long* scan = (long long*)(smem + SM::SCAN);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < DQ_STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
+  const int worker = blockIdx.x * DQ_WARPS + warp;
+  unsigned char* ring = smem + warp * SM::RING;
+  uint64_t* full = (uint64_t*)(smem + SM::BARS) + warp * DQ_STAGES;
+  if (lane == 0) {
+    for (int s = 0; s < DQ_STAGES; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
-    p.desc[4 * blockIdx.x + 2] = 0;
+    p.desc[4 * worker + 2] = 0;
   }
   long long total, share;
-  Place at = find_place(p, scan, blockIdx.x, &total, &share);
-  const long long first = blockIdx.x * share;
-  long long left = first < total ? min(share, total - first) : 0;
+  Walk w;
+  w.at = find_place(p, (long long*)(smem + SM::SCAN), &total, &share);
+  const long long first = worker * share;
+  w.left = first < total ? min(share, total - first) : 0;
   const int units = p.G * p.hgroups, hq = p.H / p.G;
+  bool busy = w.left > 0;
+  if (busy) w.set(p);
 
-  if (warp == DQ_WARPS) {
-    // ---- producer: walks the block tables and brings one record of K and of V per page ------------
-    const size_t rec_page = (size_t)p.G * SM::REC;
-    int j = 0;  // pairs issued; a slot's phase follows from it
-    for (; left > 0; at.page = 0, ++at.hg) {
-      if (at.hg == units) at.hg = 0, ++at.b;
-      long long np = pages_of(p.lens[at.b]);
-      while (np == 0) np = pages_of(p.lens[++at.b]);  // (only at the start of a sequence; `left` says that one follows)
-      const long long count = min(np - at.page, left);
-      const size_t head = (size_t)(at.hg / p.hgroups) * SM::REC;
-      for (long long j0 = 0; j0 < count; j0 += 32) {
-        const long long col = at.page + j0 + lane;  // beyond the table: page 0
-        const int mine = (j0 + lane < count && col < p.MP) ? p.table[(size_t)at.b * p.MP + col] : 0;
-        const int lim = (int)min(32LL, count - j0);
-        for (int i = 0; i < lim; i += 2, ++j) {
-          const int pa = __shfl_sync(0xffffffffu, mine, i), pb = __shfl_sync(0xffffffffu, mine, i + 1);
-          if (lane == 0) {
-            const int s = j % DQ_STAGES, n = min(2, lim - i);
-            mbar_wait(&empty[s], ((j / DQ_STAGES) & 1) ^ 1, p.status, 501);
-            mbar_expect_tx(&full[s], n * 2 * SM::REC);
-            unsigned char* dst = smem + s * SM::STAGE;
-            for (int e = 0; e < n; ++e, dst += SM::PAGE) {
-              const int page = e ? pb : pa;
-              const bool in = page >= 0 && page < p.NP;
-              const size_t off = (size_t)page * rec_page + head;
-              bulk_load(dst, in ? p.Kc + off : g_zero_record, SM::REC, &full[s]);
-              bulk_load(dst + SM::KV, in ? p.Vc + off : g_zero_record, SM::REC, &full[s]);
-            }
-          }
-        }
-      }
-      left -= count;
+  // ---- loads: `lw` walks the same units ahead of `w` -------------------------------------------------
+  Walk lw = w;
+  bool more = busy;
+  int lpair = 0, ls = 0;      // the pair of its unit that comes next, and its slot
+  int tab = 0, tab_next = 0;          // the block table's entries of 16 pairs, a page per lane, and of the next 16
+  const int rec_page = p.G * SM::REC;
+  size_t aim = 0;  // lw's KV head within a page
+  auto entries = [&](int pair) {
+    const long long i = 2LL * pair + lane, col = lw.at.page + i;  // beyond the table: page 0
+    return i < lw.count && col < p.MP ? p.table[(size_t)lw.at.b * p.MP + col] : 0;
+  };
+  auto load = [&]() {
+    if (!more) return;
+    if ((lpair & 15) == 0) {
+      tab = lpair == 0 ? entries(0) : tab_next;
+      if (2 * (lpair + 16) < lw.count) tab_next = entries(lpair + 16);
     }
-    return;
-  }
+    const int pages = min(2, lw.count - 2 * lpair);
+    const int pa = __shfl_sync(0xffffffffu, tab, 2 * (lpair & 15)), pb = __shfl_sync(0xffffffffu, tab, 2 * (lpair & 15) + 1);
+    if (elect_one()) {
+      unsigned char* dst = ring + ls * SM::STAGE;
+      mbar_expect_tx(&full[ls], pages * SM::PAGE);
+      const bool in_a = (unsigned)pa < (unsigned)p.NP, in_b = (unsigned)pb < (unsigned)p.NP;
+      const size_t off_a = aim + (long long)pa * rec_page, off_b = aim + (long long)pb * rec_page;
+      bulk_load(dst, in_a ? p.Kc + off_a : g_zero_record, SM::REC, &full[ls]);
+      bulk_load(dst + SM::REC, in_a ? p.Vc + off_a : g_zero_record, SM::REC, &full[ls]);
+      if (pages == 2) {
+        bulk_load(dst + 2 * SM::REC, in_b ? p.Kc + off_b : g_zero_record, SM::REC, &full[ls]);
+        bulk_load(dst + 3 * SM::REC, in_b ? p.Vc + off_b : g_zero_record, SM::REC, &full[ls]);
+      }
+    }
+    __syncwarp();
+    if (++ls == DQ_STAGES) ls = 0;
+    if (2 * ++lpair >= lw.count) {
+      lpair = 0;
+      more = lw.next(p, units);
+      aim = (size_t)(lw.at.hg / p.hgroups) * SM::REC;
+    }
+  };
+  aim = (size_t)(lw.at.hg / p.hgroups) * SM::REC;
+  for (int i = 0; i < DQ_STAGES - 1; ++i) load();
 
-  // ---- consumers -----------------------------------------------------------------------------------
   const int gq = lane >> 2, t = lane & 3;
   // Rows of the K tile (and columns of the V tile) are the page's tokens in the order that lets a
   // lane's four V tokens be t, 4 + t, 8 + t, 12 + t: row r is token (r & 7) / 2 + 4 (r & 1) + (r & 8).
   const int tok_a = (gq >> 1) + 4 * (gq & 1), tok_b = tok_a + 8;
   const float sc2 = p.scale * LOG2E * TWO24;
-  const uint32_t ring = smem_u32(smem);
+  const uint32_t ring_u = smem_u32(ring);
   const int side = SIDE ? t >> 1 : 0;  // the page of a pair whose scores this lane holds
-  int base = 0;  // pairs of the CTA before this segment
-  for (; left > 0; at.page = 0, ++at.hg) {
-    if (at.hg == units) at.hg = 0, ++at.b;
-    int n = p.lens[at.b];
-    while (n <= 0) n = p.lens[++at.b];
-    const long long np = pages_of(n);
-    const int count = (int)min(np - at.page, left), pairs = (count + 1) / 2;
+  int cs = 0, phase = 0;               // the slot that is read next, and its phase
+  for (; busy; busy = w.next(p, units)) {
+    const Place& at = w.at;
+    const int n = w.n, count = w.count, pairs = (count + 1) / 2;
     // Tokens of this segment: those behind it are another CTA's, or do not exist.
-    const int tokens = (int)min((long long)count * 16, (long long)n - at.page * 16);
+    const long long here = (long long)n - at.page * 16;
+    const int tokens = (int)min((long long)count * 16, here);
     const int g = at.hg / p.hgroups, h0 = g * hq + (at.hg % p.hgroups) * 8, nh = min(8, hq - (at.hg % p.hgroups) * 8);
 
     // Q as the B operand: column gq is head gq (SIDE: head gq & 3, for page gq >> 2 of the pair), the
@@ -323,10 +337,10 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       uint32_t hka, hkb, hva, hvb;  // headers of its two tokens: a pair of f16 (or one)
       if (NG == 2) {
         hka = lds32(own + 8 * D + 4 * tok_a), hkb = lds32(own + 8 * D + 4 * tok_b);
-        hva = lds32(own + SM::KV + 8 * D + 4 * tok_a), hvb = lds32(own + SM::KV + 8 * D + 4 * tok_b);
+        hva = lds32(own + SM::REC + 8 * D + 4 * tok_a), hvb = lds32(own + SM::REC + 8 * D + 4 * tok_b);
       } else {
         hka = lds16(own + 8 * D + 2 * tok_a), hkb = lds16(own + 8 * D + 2 * tok_b);
-        hva = lds16(own + SM::KV + 8 * D + 2 * tok_a), hvb = lds16(own + SM::KV + 8 * D + 2 * tok_b);
+        hva = lds16(own + SM::REC + 8 * D + 2 * tok_a), hvb = lds16(own + SM::REC + 8 * D + 2 * tok_b);
       }
       // Tokens behind the last one: stale headers may be NaN, and the scores are masked below.
       const bool tail = limit < (SIDE ? 32 : 16);
@@ -429,102 +443,90 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
           const bool hi = !SIDE || (gq < 4) == (s == 0);
           const uint32_t b_0 = hi ? bh0 : ol0, b_1 = hi ? bh1 : ol1;
           // V^T: a lane's word gq of the group, for its four tokens; two tokens' halves side by side.
-          const uint32_t v = pg + s * SM::PAGE + SM::KV + 32 * x + 4 * gq + t * (D / 2);
+          const uint32_t v = pg + s * SM::PAGE + SM::REC + 32 * x + 4 * gq + t * (D / 2);
           const uint32_t w0 = lds32(v), w1 = lds32(v + 2 * D), w2 = lds32(v + 4 * D), w3 = lds32(v + 6 * D);
           const uint32_t lo01 = __byte_perm(w0, w1, 0x5410), hi01 = __byte_perm(w0, w1, 0x7632);
           const uint32_t lo23 = __byte_perm(w2, w3, 0x5410), hi23 = __byte_perm(w2, w3, 0x7632);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {  // elements 2k, 2k + 1 of the word: rows gq, gq + 8
-            const int sh = (k >> 1) * 8;
-            const uint32_t mask = (k & 1) ? 0x00f000f0u : 0x000f000fu, centre = (k & 1) ? 0x80808080u : 0x80088008u;
-            const uint32_t a_0 = add_h2((lo01 >> sh) & mask, centre), a_1 = add_h2((hi01 >> sh) & mask, centre);
-            const uint32_t a_2 = add_h2((lo23 >> sh) & mask, centre), a_3 = add_h2((hi23 >> sh) & mask, centre);
+          for (int k = 0; k < 4; ++k) {
+            // Of the word's nibbles e0 e2 e4 e6 e1 e3 e5 e7: k = 0: e0, e2 are rows gq, gq + 8; 1: e4, e6; 2: e1,
+            // e3; 3: e5, e7. Rows 8..15 always weigh 16, so one constant operand serves all.
+            const uint32_t v01 = (k & 2 ? hi01 : lo01) >> (8 * (k & 1)), v23 = (k & 2 ? hi23 : lo23) >> (8 * (k & 1));
+            const uint32_t a_0 = v01 & 0x000f000fu, a_1 = v01 & 0x00f000f0u, a_2 = v23 & 0x000f000fu, a_3 = v23 & 0x00f000f0u;
             mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, b_0, b_1);
-            if (!SIDE) mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bl0, bl1);
+            mma16816(acc[4 * x + k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b_0, b_1);  // -8 of each
+            if (!SIDE) {
+              mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bl0, bl1);
+              mma16816(acc[4 * x + k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, bl0, bl1);
+            }
           }
         }
       }
     };
 
-    for (int j = base + ((warp - base) & (DQ_WARPS - 1)); j < base + pairs; j += DQ_WARPS) {
-      const int s = j % DQ_STAGES, limit = tokens - 32 * (j - base);
-      mbar_wait(&full[s], (j / DQ_STAGES) & 1, p.status, 502);
-      tile(ring + s * SM::STAGE, min(limit, 32));
-      if (!SIDE && limit > 16) tile(ring + s * SM::STAGE + SM::PAGE, min(limit - 16, 16));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
+    for (int j = 0; j < pairs; ++j) {
+      load();
+      const int limit = tokens - 32 * j;
+      mbar_wait(&full[cs], phase, p.status, 502);
+      const uint32_t pg = ring_u + cs * SM::STAGE;
+      tile(pg, min(limit, 32));
+      if (!SIDE && limit > 16) tile(pg + SM::PAGE, min(limit - 16, 16));
+      if (++cs == DQ_STAGES) cs = 0, phase ^= 1;
+      __syncwarp();  // the slot may be filled again
     }
 
-    // ---- the four warps' sums of this segment, merged ---------------------------------------------
+    // ---- the segment's result ---------------------------------------------------------------------------
     float z[NG][2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int d = 4; d <= 16; d <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], d);
+      for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) l[c] += __shfl_xor_sync(0xffffffffu, l[c], d);
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
         z[x][c] = zacc[x][c];
 #pragma unroll
-        for (int d = 4; d <= 16; d <<= 1) z[x][c] += __shfl_xor_sync(0xffffffffu, z[x][c], d);
+        for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) z[x][c] += __shfl_xor_sync(0xffffffffu, z[x][c], d);
       }
     }
-    float* mine = (float*)(smem + SM::RING) + warp * SM::WARP;
     const float unit = TWO24 / F;
+    const bool whole = at.page == 0 && count == w.np;
+    float* part = p.part + ((size_t)worker * 2 + (at.page == 0 ? 1 : 0)) * DQ_SLOT * (D + 2);
 #pragma unroll
-    for (int i = 0; i < 4 * NG; i += 2) {
-      const int d = 64 * (i >> 2) + 8 * gq + 2 * (i & 3);
+    for (int c = 0; c < 2; ++c) {
+      const int hh = (SIDE ? 2 * (t & 1) : 2 * t) + c;  // the head of this column
+      const float inv = 1.0f / l[c];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float zz = z[i >> 2][c] * unit;
-        float4 v;
-        v.x = fmaf(acc[i][c], unit, zz);
-        v.y = fmaf(acc[i][2 + c], unit, zz);
-        v.z = fmaf(acc[i + 1][c], 0.0625f * unit, zz);
-        v.w = fmaf(acc[i + 1][2 + c], 0.0625f * unit, zz);
-        *reinterpret_cast<float4*>(mine + (2 * t + c) * D + d) = v;
+      for (int x = 0; x < NG; ++x) {
+        float v[8];  // elements 64 x + 8 gq ...
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int upper = (i >> 1) & 1;  // the nibble's weight; its product: see above
+          float a = acc[4 * x + 2 * (i & 1) + (i >> 2)][2 * upper + c];
+          if (SIDE) a += __shfl_xor_sync(0xffffffffu, a, 2);  // columns h and h + 4 are the same head
+          v[i] = fmaf(a, upper ? 0.0625f * unit : unit, z[x][c] * unit);
+        }
+        // SIDE: both lanes of a pair hold the sums; they take a group each.
+        if (hh < nh && (!SIDE || (t >> 1) == x)) {
+          const int d = 64 * x + 8 * gq;
+          if (whole) {
+            uint4 y;
+            y.x = pack_h2(v[0] * inv, v[1] * inv), y.y = pack_h2(v[2] * inv, v[3] * inv);
+            y.z = pack_h2(v[4] * inv, v[5] * inv), y.w = pack_h2(v[6] * inv, v[7] * inv);
+            *reinterpret_cast<uint4*>(p.O + ((size_t)at.b * p.H + h0 + hh) * D + d) = y;
+          } else {
+            *reinterpret_cast<float4*>(part + hh * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(part + hh * D + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
+          }
+        }
       }
+      if (!whole && gq == 0 && hh < nh && (!SIDE || t < 2)) part[DQ_SLOT * D + hh] = m[c], part[DQ_SLOT * (D + 1) + hh] = l[c];
     }
-    if (gq == 0) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) mine[8 * D + 2 * t + c] = m[c], mine[8 * D + 8 + 2 * t + c] = l[c];
-    }
-    asm volatile("bar.sync 1, %0;" ::"r"(DQ_WARPS * 32) : "memory");
-    const float* all = (const float*)(smem + SM::RING);
-    const bool whole = at.page == 0 && count == np;
-    float* part = p.part + ((size_t)blockIdx.x * 2 + (at.page == 0 ? 1 : 0)) * DQ_SLOT * (D + 2);
-    for (int i = threadIdx.x; i < nh * D; i += DQ_WARPS * 32) {
-      const int hh = i / D, d = i % D;
-      float mt = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < DQ_WARPS; ++w) mt = fmaxf(mt, all[w * SM::WARP + 8 * D + hh]);
-      float lt = 0.f, o = 0.f;
-#pragma unroll
-      for (int w = 0; w < DQ_WARPS; ++w) {
-        const float* a = all + w * SM::WARP;
-        const float mw = a[8 * D + hh], lw = SIDE ? a[8 * D + 8 + hh] + a[8 * D + 12 + hh] : a[8 * D + 8 + hh];
-        // A warp without a page has nothing; one whose scores were all NaN has a NaN sum.
-        const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2(mw - mt);
-        float v = a[hh * D + d];
-        if (SIDE) v += a[(hh + 4) * D + d];
-        if (f != 0.f || v != v) o = fmaf(v, f, o);
-        lt = fmaf(lw, f, lt);
-      }
-      if (whole) {
-        p.O[((size_t)at.b * p.H + h0 + hh) * D + d] = __float2half_rn(o / lt);
-      } else {
-        part[hh * D + d] = o;
-        if (d == 0) part[DQ_SLOT * D + hh] = mt, part[DQ_SLOT * (D + 1) + hh] = lt;
-      }
-    }
-    if (threadIdx.x == 0 && !whole && at.page == 0) {
-      // The unit is cut at this CTA's end: the next CTAs go on with it.
-      int* d = p.desc + 4 * blockIdx.x;
+    if (lane == 0 && !whole && at.page == 0) {
+      // The unit is cut at this warp's end: the next ones go on with it.
+      int* d = p.desc + 4 * worker;
       d[0] = at.b, d[1] = at.hg;
-      d[2] = 1 + (int)((np - count + share - 1) / share);
+      d[2] = 1 + (int)((w.np - count + share - 1) / share);
     }
-    asm volatile("bar.sync 1, %0;" ::"r"(DQ_WARPS * 32) : "memory");
-    base += pairs;
-    left -= count;
   }
 
   // Only now: the next kernel's CTAs, let in earlier, would take the places of this one's and make the
@@ -533,23 +535,25 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
   // Rows without a cached token: 0/0, as decode_attention gives.
   for (int b = blockIdx.x; b < p.B; b += gridDim.x)
     if (p.lens[b] <= 0)
-      for (int i = threadIdx.x; i < p.H * D; i += DQ_WARPS * 32)
+      for (int i = threadIdx.x; i < p.H * D; i += DQ_THREADS)
         p.O[(size_t)b * p.H * D + i] = __float2half_rn(__int_as_float(0x7fc00000));
 }
 
-// Joins the partials of the unit that is cut at the end of CTA blockIdx.x, if there is one: that
-// CTA's second slot and the first slots of the CTAs that follow. One warp per head.
+// Joins the partials of the unit that is cut at the end of a warp's share, if there is one: that
+// warp's second slot and the first slots of the warps that follow. One warp per (worker, head).
 template <int D>
-__global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p) {
+__global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p, int heads, int workers) {
   pdl_wait();
   pdl_launch();
-  const int* d = p.desc + 4 * blockIdx.x;
+  const int i0 = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int worker = i0 / heads, hh = i0 % heads;
+  if (worker >= workers) return;
+  const int* d = p.desc + 4 * worker;
   const int b = d[0], hg = d[1], pieces = d[2];
   if (pieces < 2) return;
   const int hq = p.H / p.G, h0 = (hg / p.hgroups) * hq + (hg % p.hgroups) * 8, nh = min(8, hq - (hg % p.hgroups) * 8);
-  const int hh = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (hh >= nh) return;
-  auto slot = [&](int i) { return p.part + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * DQ_SLOT * (D + 2); };
+  auto slot = [&](int i) { return p.part + ((size_t)(worker + i) * 2 + (i == 0 ? 1 : 0)) * DQ_SLOT * (D + 2); };
   float m = -INFINITY;
   for (int i = lane; i < pieces; i += 32) m = fmaxf(m, slot(i)[DQ_SLOT * D + hh]);
 #pragma unroll
@@ -571,11 +575,11 @@ __global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p) {
 }
 
 template <int D, bool SIDE>
-int run(Ctx* c, Op& op, DqParams p, const Q4Shape& q) {
-  const int grid = op.p1;
+int run(Ctx* c, Op& op, DqParams p) {
+  const int grid = op.p1, workers = grid * DQ_WARPS, heads = min(8, p.H / p.G);
   TB_CUDA(c, launch_k(c, decode_q4_kernel<D, SIDE>, dim3(grid), dim3(DQ_THREADS), DqSmem<D>::TOTAL, 1, p));
   c->launches += 1;
-  TB_CUDA(c, launch_k(c, decode_q4_join_kernel<D>, dim3(grid), dim3(256), 0, 1, p));
+  TB_CUDA(c, launch_k(c, decode_q4_join_kernel<D>, dim3((workers * heads + 7) / 8), dim3(256), 0, 1, p, heads, workers));
   c->launches += 1;
   return 0;
 }
@@ -591,10 +595,10 @@ int make_decode_q4(Ctx* c, Op& op, const Q4Shape& q) {
   const int units = q.G * ((H / q.G + 7) / 8);
   // As many CTAs as stay resident, and no more than have DQ_LEAST pages to work on. (Lengths beyond
   // the table only make the shares larger.)
-  const long long most = ((long long)B * units * op.shapes[3][1] + DQ_LEAST - 1) / DQ_LEAST;
+  const long long most = ((long long)B * units * op.shapes[3][1] + DQ_LEAST * DQ_WARPS - 1) / (DQ_LEAST * DQ_WARPS);
   const long long fit = (long long)c->sm_count * DQ_CTAS;
   op.p1 = (int)(most < fit ? most : fit);
-  op.scratch_bytes = (size_t)op.p1 * (2 * DQ_SLOT * (q.D + 2) * sizeof(float) + 16);
+  op.scratch_bytes = (size_t)op.p1 * DQ_WARPS * (2 * DQ_SLOT * (q.D + 2) * sizeof(float) + 16);
   TB_CUDA(c, cudaMalloc(&op.scratch, op.scratch_bytes));
   auto attr = [&](auto kern, int bytes) { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); };
   TB_CUDA(c, attr(decode_q4_kernel<128, true>, DqSmem<128>::TOTAL));
@@ -618,13 +622,13 @@ int launch_decode_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
   p.least = DQ_LEAST;
   p.status = c->status;
   p.part = (float*)op.scratch;
-  p.desc = (int*)(p.part + (size_t)op.p1 * 2 * DQ_SLOT * (q.D + 2));
+  p.desc = (int*)(p.part + (size_t)op.p1 * DQ_WARPS * 2 * DQ_SLOT * (q.D + 2));
   const bool side = p.H / p.G <= 4;
   int r;
   if (q.D == 128)
-    r = side ? run<128, true>(c, op, p, q) : run<128, false>(c, op, p, q);
+    r = side ? run<128, true>(c, op, p) : run<128, false>(c, op, p);
   else
-    r = side ? run<64, true>(c, op, p, q) : run<64, false>(c, op, p, q);
+    r = side ? run<64, true>(c, op, p) : run<64, false>(c, op, p);
   return r;
 }
 
