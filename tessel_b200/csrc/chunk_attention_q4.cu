@@ -49,7 +49,7 @@ struct CqParams {
   const int* table;
   const int* meta;
   __half* O;
-  float* part;  // [CTA][2][256][D + 2]: numerator, maximum, sum of a row
+  float* part;  // [CTA][2][D + 2][256]: a row's numerator, maximum and sum, rows side by side
   int* desc;    // [CTA][4]: piece, KV head, block, CTAs that hold a part of the unit cut at this CTA's end (0: none)
   float scale;
   int T, H, G, hq, tm, C, NP, MP, least;  // tm: tokens of a tile
@@ -545,7 +545,8 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
           }
         }
       } else {
-        float* part = p.part + (((size_t)blockIdx.x * 2 + (w.k0 == 0 ? 1 : 0)) * 256 + t * 128 + rit) * (D + 2);
+        // A column at a time, a warp's rows side by side: full lines.
+        float* part = p.part + ((size_t)blockIdx.x * 2 + (w.k0 == 0 ? 1 : 0)) * 256 * (D + 2) + t * 128 + rit;
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t ov[32];
@@ -554,13 +555,13 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
             tmem_ld_wait();
           }
           if (live) {
-            const float f = nt == 0 ? 0.f : nan_at[(unit & 3) * 2 + (c0 >> 6)] <= row ? __int_as_float(0x7fc00000) : 1.0f;
+            const bool spoilt = nan_at[(unit & 3) * 2 + (c0 >> 6)] <= row;
 #pragma unroll
-            for (int i = 0; i < 32; i += 2)
-              *reinterpret_cast<float2*>(part + c0 + i) = nt == 0 ? make_float2(0.f, 0.f) : make_float2(__uint_as_float(ov[i]) * f, __uint_as_float(ov[i + 1]) * f);
+            for (int i = 0; i < 32; ++i)
+              part[(size_t)(c0 + i) * 256] = nt == 0 ? 0.f : spoilt ? __int_as_float(0x7fc00000) : __uint_as_float(ov[i]);
           }
         }
-        if (live) part[D] = m_ref, part[D + 1] = l;
+        if (live) part[D * 256] = m_ref, part[(D + 1) * 256] = l;
         if (t == 0 && rit == 0 && w.k0 == 0) {
           // Cut at this CTA's end: the next CTAs go on with it.
           int* d = p.desc + 4 * blockIdx.x;
@@ -586,39 +587,39 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
 }
 
 // Joins the partials of the unit that is cut at the end of CTA blockIdx.x, if there is one: that
-// CTA's second slot and the first slots of the CTAs that follow. A warp per row, 8 rows per block of y.
+// CTA's second slot and the first slots of the CTAs that follow. A thread joins eight columns of a row;
+// the block's y says which.
 template <int D>
 __global__ void __launch_bounds__(256) chunk_q4_join_kernel(const CqParams p) {
   pdl_wait();
   pdl_launch();
   const int* d = p.desc + 4 * blockIdx.x;
-  const int pieces = d[3];
+  const int c = d[0], g = d[1], i = d[2], pieces = d[3];
   if (pieces < 2) return;
-  const Piece r = piece_of(p, d[0]);
-  const int g = d[1], i = d[2], lane = threadIdx.x & 31;
-  for (int rr = blockIdx.y * 8 + (threadIdx.x >> 5); rr < 256; rr += gridDim.y * 8) {
-    const int t = rr >> 7, tok = (rr & 127) / p.hq, head = (rr & 127) % p.hq;
-    const int local = i * 2 * p.tm + t * p.tm + tok;
-    if (tok >= p.tm || local >= r.nrows) continue;
-    auto slot = [&](int k) { return p.part + (((size_t)(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * 256 + rr) * (D + 2); };
-    float m = -INFINITY;
-    for (int k = lane; k < pieces; k += 32) m = fmaxf(m, slot(k)[D]);
+  const Piece r = piece_of(p, c);
+  const int rr = threadIdx.x, t = rr >> 7, tok = (rr & 127) / p.hq, head = (rr & 127) % p.hq;
+  const int local = i * 2 * p.tm + t * p.tm + tok;
+  if (tok >= p.tm || local >= r.nrows) return;
+  float m = -1e30f, l = 0.f, a[8];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, a[D / 32];
+  for (int e = 0; e < 8; ++e) a[e] = 0.f;
+#pragma unroll 2
+  for (int k = 0; k < pieces; ++k) {
+    const float* s = p.part + ((size_t)(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * 256 * (D + 2) + rr;
+    float v[8];
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) a[k] = 0.f;
-    for (int k = 0; k < pieces; ++k) {
-      const float* s = slot(k);
-      const float f = ex2(s[D] - m);
-      l = fmaf(s[D + 1], f, l);
+    for (int e = 0; e < 8; ++e) v[e] = s[(size_t)(blockIdx.y * 8 + e) * 256];
+    const float mk = s[D * 256], lk = s[(D + 1) * 256];
+    const float m2 = fmaxf(m, mk), f = ex2(m - m2), fk = ex2(mk - m2);
+    l = fmaf(l, f, lk * fk);
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) a[e] = fmaf(s[lane + 32 * e], f, a[e]);
-    }
-    __half* o = p.O + ((size_t)(r.row0 + local) * p.H + g * p.hq + head) * D;
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) o[lane + 32 * e] = __float2half_rn(a[e] / l);
+    for (int e = 0; e < 8; ++e) a[e] = fmaf(a[e], f, v[e] * fk);
+    m = m2;
   }
+  uint4 y;
+  y.x = pack_h2(a[0] / l, a[1] / l), y.y = pack_h2(a[2] / l, a[3] / l);
+  y.z = pack_h2(a[4] / l, a[5] / l), y.w = pack_h2(a[6] / l, a[7] / l);
+  *reinterpret_cast<uint4*>(p.O + ((size_t)(r.row0 + local) * p.H + g * p.hq + head) * D + blockIdx.y * 8) = y;
 }
 
 }  // namespace
@@ -667,7 +668,7 @@ int launch_chunk_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
   p.status = c->status;
   p.part = (float*)op.scratch;
   p.desc = (int*)(p.part + (size_t)op.p1 * 2 * 256 * (q.D + 2));
-  const dim3 grid(op.p1), join(op.p1, 8);
+  const dim3 grid(op.p1), join(op.p1, q.D / 8);
   if (q.D == 128) {
     TB_CUDA(c, launch_k(c, chunk_q4_kernel<128>, grid, dim3(CQ_THREADS), CqSmem<128>::TOTAL, 1, hit->m[0], p));
     TB_CUDA(c, launch_k(c, chunk_q4_join_kernel<128>, join, dim3(256), 0, 1, p));

@@ -17,10 +17,10 @@
 // values out of the accumulators. P is split in two f16 (hi + lo), so the second product keeps f32
 // accuracy.
 //
-// The eight columns of a product. With four or fewer query heads per KV head (SIDE) a warp takes two
-// pages at a time: the first page's scores come out in columns 0..3, the second's in 4..7 (the
-// operand q has zeros in the other page's columns), so no lane of the softmax idles; and the hi and
-// lo parts of P share a product, side by side. With five to eight heads a page fills the columns,
+// The eight columns of a product. With four or fewer query heads per KV head (SIDE) q stands in them
+// twice and a warp takes two pages at a time: columns 0..3 of the first page's scores and 4..7 of the
+// second's go on, so no lane of the softmax does another's work; and the hi and lo parts of P share a
+// product, side by side. With five to eight heads a page fills the columns,
 // and lo is a second product.
 //
 // Bound: HBM bytes, 2 (D/2 + 2 D/64) per token and KV head, with the issue slots close behind.
@@ -29,7 +29,9 @@
 // page) list, whatever the lengths are, finds its place from the lengths, brings its pages through a
 // ring of its own (bulk copies it issues itself, a few pairs of pages ahead, across units), and
 // writes O for units that lie wholly inside its share. A unit that is cut leaves one partial with
-// each warp; a second, tiny kernel joins them.
+// each warp; a second, tiny kernel joins them. Where the KV heads are even in number, two or four
+// neighbouring warps take neighbouring heads of the same pages: their records lie side by side, and
+// DRAM delivers neighbours that are asked for together faster than records picked one by one.
 #include "kv_q4.cuh"
 
 namespace tb {
@@ -38,17 +40,19 @@ namespace {
 
 constexpr int DQ_WARPS = 4;
 constexpr int DQ_THREADS = DQ_WARPS * 32;
-constexpr int DQ_STAGES = 3;  // pairs of pages in a warp's ring
-constexpr int DQ_CTAS = 4;    // per SM
+static_assert(DQ_WARPS % 4 == 0, "sets of one, two or four head groups divide a CTA's warps");
+constexpr int DQ_STAGES = 4;  // pairs of pages in a ring
+constexpr int DQ_CTAS = 3;    // per SM
 constexpr int DQ_LEAST = 8;   // pages a warp takes at least
 constexpr int DQ_SLOT = 8;    // heads of a partial
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float TWO24 = 16777216.0f;
+constexpr float NO_MAX = -1e30f;    // the running maximum before the first page
 constexpr float GROW = 8.0f;        // the running maximum is renewed when a score passes it by this (log2): p <= 2^8
 constexpr float SCALE_MOST = 128.f; // and the values' running scale when s F passes this: P = p s F < 2^15 fits an f16
 
 // What a table entry outside the cache reads as.
-__device__ __align__(128) unsigned char g_zero_record[2048];
+__device__ __align__(128) unsigned char g_zero_record[4608];
 
 struct DqParams {
   const __half* Q;
@@ -61,6 +65,7 @@ struct DqParams {
   int* desc;    // [warp][4]: sequence, head group, warps that hold a piece of the unit cut at this warp's end (0: none)
   float scale;
   int B, H, G, NP, MP, hgroups, least;
+  int units;  // sets of WH head groups, which neighbouring warps take side by side, in a sequence
   unsigned int* status;
 };
 
@@ -69,9 +74,9 @@ struct DqSmem {
   static constexpr int REC = 16 * (D / 2 + 2 * (D / 64));
   static constexpr int PAGE = 2 * REC;  // K and V of a page
   static constexpr int STAGE = 2 * PAGE;
-  static constexpr int RING = DQ_STAGES * STAGE;                // of one warp
+  static constexpr int RING = DQ_STAGES * STAGE;  // a warp's part of its set's ring
   static constexpr int BARS = DQ_WARPS * RING;
-  static constexpr int SCAN = BARS + DQ_WARPS * DQ_STAGES * 8;  // long long [DQ_THREADS + 1], then the warps' places
+  static constexpr int SCAN = BARS + 2 * DQ_WARPS * DQ_STAGES * 8;  // long long [DQ_THREADS + 1], then the sets' places
   static constexpr int TOTAL = SCAN + (DQ_THREADS + 1 + 2 * DQ_WARPS) * 8 + 128;
 };
 
@@ -120,18 +125,20 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float lo_f32(uint32_t h2) { return __low2float(*reinterpret_cast<__half2*>(&h2)); }
 __device__ __forceinline__ float hi_f32(uint32_t h2) { return __high2float(*reinterpret_cast<__half2*>(&h2)); }
 
-// A place in the list of (sequence, head group, page): sequences in order, the head groups of one
+// A place in the list of (sequence, set of head groups, page): sequences in order, the sets of one
 // after another, its pages within.
 struct Place {
-  int b, hg;
-  long long page;
+  int b, hg, page;
 };
 
 __device__ __forceinline__ long long pages_of(int n) { return n > 0 ? ((long long)n + 15) / 16 : 0; }
 
-// The number of (unit, page) items, the share of a warp, and where this one begins. All threads call it.
+// The number of (unit, page) items, the share of a set of WH warps, and where this one begins. All
+// threads call it.
+template <int WH>
 __device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, long long* total, long long* share) {
-  const int units = p.G * p.hgroups, lane = threadIdx.x & 31;
+  constexpr int owners = DQ_WARPS / WH;
+  const int units = p.units, lane = threadIdx.x & 31;
   const int per = (p.B + DQ_THREADS - 1) / DQ_THREADS;
   const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
   long long sum = 0;
@@ -151,7 +158,7 @@ __device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, 
     if (w < (int)(threadIdx.x >> 5)) before += scan[w];
     pages += scan[w];
   }
-  const long long all = pages * units, workers = (long long)gridDim.x * DQ_WARPS;
+  const long long all = pages * units, workers = (long long)gridDim.x * owners;
   const long long s = max((all + workers - 1) / workers, (long long)p.least);
   *total = all;
   *share = s;
@@ -160,8 +167,8 @@ __device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, 
   for (int b = b0; b < b1; ++b) {
     const long long end = at + pages_of(p.lens[b]) * units;
 #pragma unroll
-    for (int w = 0; w < DQ_WARPS; ++w) {
-      const long long start = ((long long)blockIdx.x * DQ_WARPS + w) * s;
+    for (int w = 0; w < owners; ++w) {
+      const long long start = ((long long)blockIdx.x * owners + w) * s;
       if (start >= at && start < end) {
         scan[DQ_WARPS + 2 * w] = b;
         scan[DQ_WARPS + 2 * w + 1] = start - at;
@@ -171,11 +178,12 @@ __device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, 
   }
   __syncthreads();
   Place r = {0, 0, 0};
-  if (((long long)blockIdx.x * DQ_WARPS + (threadIdx.x >> 5)) * s < all) {
-    r.b = (int)scan[DQ_WARPS + 2 * (threadIdx.x >> 5)];
-    const long long np = pages_of(p.lens[r.b]), in = scan[DQ_WARPS + 2 * (threadIdx.x >> 5) + 1];
+  const int own = (threadIdx.x >> 5) / WH;
+  if (((long long)blockIdx.x * owners + own) * s < all) {
+    r.b = (int)scan[DQ_WARPS + 2 * own];
+    const long long np = pages_of(p.lens[r.b]), in = scan[DQ_WARPS + 2 * own + 1];
     r.hg = (int)(in / np);
-    r.page = in % np;
+    r.page = (int)(in % np);
   }
   return r;
 }
@@ -183,13 +191,12 @@ __device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, 
 // A walk along a warp's share: the current unit's pages [at.page, at.page + count) are its own.
 struct Walk {
   Place at;
-  long long left, np;
-  int n, count;
+  int left, np, n, count;
   __device__ __forceinline__ void set(const DqParams& p) {
     n = p.lens[at.b];
     while (n <= 0) n = p.lens[++at.b];  // (only at the start of a sequence; `left` says that one follows)
-    np = pages_of(n);
-    count = (int)min(np - at.page, left);
+    np = (int)pages_of(n);
+    count = min(np - at.page, left);
     left -= count;
   }
   // To the next unit; false at the end of the share.
@@ -202,7 +209,7 @@ struct Walk {
   }
 };
 
-template <int D, bool SIDE>
+template <int D, bool SIDE, int WH>
 __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const DqParams p) {
   pdl_wait();
   using SM = DqSmem<D>;
@@ -211,31 +218,45 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 127) & ~(uintptr_t)127);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int worker = blockIdx.x * DQ_WARPS + warp;
-  unsigned char* ring = smem + warp * SM::RING;
-  uint64_t* full = (uint64_t*)(smem + SM::BARS) + warp * DQ_STAGES;
+  const int own = warp / WH, wh = warp % WH;  // this warp's set, and its head group in it
+  unsigned char* ring = smem + own * (WH * SM::RING);
+  uint64_t* full = (uint64_t*)(smem + SM::BARS) + own * DQ_STAGES;
+  uint64_t* empty = (uint64_t*)(smem + SM::BARS) + (DQ_WARPS + own) * DQ_STAGES;
   if (lane == 0) {
-    for (int s = 0; s < DQ_STAGES; ++s) mbar_init(&full[s], 1);
-    fence_barrier_init();
+    if (wh == 0) {
+      for (int s = 0; s < DQ_STAGES; ++s) {
+        mbar_init(&full[s], 1);
+        mbar_init(&empty[s], WH);
+      }
+      fence_barrier_init();
+    }
     p.desc[4 * worker + 2] = 0;
   }
   long long total, share;
   Walk w;
-  w.at = find_place(p, (long long*)(smem + SM::SCAN), &total, &share);
-  const long long first = worker * share;
-  w.left = first < total ? min(share, total - first) : 0;
-  const int units = p.G * p.hgroups, hq = p.H / p.G;
+  w.at = find_place<WH>(p, (long long*)(smem + SM::SCAN), &total, &share);
+  const long long first = (long long)(worker / WH) * share;
+  w.left = first < total ? (int)min(share, total - first) : 0;  // (2^31 pages for one warp would be hours of work)
+  const int units = p.units, hq = p.H / p.G;
   bool busy = w.left > 0;
   if (busy) w.set(p);
 
-  // ---- loads: `lw` walks the same units ahead of `w` -------------------------------------------------
+  // ---- loads: `lw` walks the same units ahead of `w`. The set's warps take turns: one of them brings a
+  // pair of pages for all, the records of the set's KV heads in one copy per page and cache. ------------
   Walk lw = w;
   bool more = busy;
-  int lpair = 0, ls = 0;      // the pair of its unit that comes next, and its slot
-  int tab = 0, tab_next = 0;          // the block table's entries of 16 pairs, a page per lane, and of the next 16
+  int lpair = 0, ls = 0, lphase = 1, turn = 0;  // the pair of its unit that comes next, its slot, and whose turn it is
+  int tab = 0, tab_next = 0;                    // the block table's entries of 16 pairs, a page per lane, and of the next 16
   const int rec_page = p.G * SM::REC;
-  size_t aim = 0;  // lw's KV head within a page
+  size_t aim = 0;   // the set's first KV head within a page
+  int heads_b = 0;  // and the bytes of its KV heads (head groups of one KV head share them)
+  auto take_aim = [&]() {
+    const int k0 = lw.at.hg * WH / p.hgroups, k1 = (lw.at.hg * WH + WH - 1) / p.hgroups;
+    aim = (size_t)k0 * SM::REC;
+    heads_b = (k1 - k0 + 1) * SM::REC;
+  };
   auto entries = [&](int pair) {
-    const long long i = 2LL * pair + lane, col = lw.at.page + i;  // beyond the table: page 0
+    const int i = 2 * pair + lane, col = lw.at.page + i;  // beyond the table: page 0
     return i < lw.count && col < p.MP ? p.table[(size_t)lw.at.b * p.MP + col] : 0;
   };
   auto load = [&]() {
@@ -245,29 +266,35 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       if (2 * (lpair + 16) < lw.count) tab_next = entries(lpair + 16);
     }
     const int pages = min(2, lw.count - 2 * lpair);
-    const int pa = __shfl_sync(0xffffffffu, tab, 2 * (lpair & 15)), pb = __shfl_sync(0xffffffffu, tab, 2 * (lpair & 15) + 1);
-    if (elect_one()) {
-      unsigned char* dst = ring + ls * SM::STAGE;
-      mbar_expect_tx(&full[ls], pages * SM::PAGE);
-      const bool in_a = (unsigned)pa < (unsigned)p.NP, in_b = (unsigned)pb < (unsigned)p.NP;
-      const size_t off_a = aim + (long long)pa * rec_page, off_b = aim + (long long)pb * rec_page;
-      bulk_load(dst, in_a ? p.Kc + off_a : g_zero_record, SM::REC, &full[ls]);
-      bulk_load(dst + SM::REC, in_a ? p.Vc + off_a : g_zero_record, SM::REC, &full[ls]);
-      if (pages == 2) {
-        bulk_load(dst + 2 * SM::REC, in_b ? p.Kc + off_b : g_zero_record, SM::REC, &full[ls]);
-        bulk_load(dst + 3 * SM::REC, in_b ? p.Vc + off_b : g_zero_record, SM::REC, &full[ls]);
+    if (WH == 1 || turn == wh) {
+      const int pa = __shfl_sync(0xffffffffu, tab, 2 * (lpair & 15)), pb = __shfl_sync(0xffffffffu, tab, 2 * (lpair & 15) + 1);
+      if (elect_one()) {
+        unsigned char* dst = ring + ls * (WH * SM::STAGE);
+        mbar_wait(&empty[ls], lphase, p.status, 501);
+        mbar_expect_tx(&full[ls], pages * 2 * heads_b);
+        const bool in_a = (unsigned)pa < (unsigned)p.NP, in_b = (unsigned)pb < (unsigned)p.NP;
+        const size_t off_a = aim + (long long)pa * rec_page, off_b = aim + (long long)pb * rec_page;
+        bulk_load(dst, in_a ? p.Kc + off_a : g_zero_record, heads_b, &full[ls]);
+        bulk_load(dst + WH * SM::REC, in_a ? p.Vc + off_a : g_zero_record, heads_b, &full[ls]);
+        if (pages == 2) {
+          bulk_load(dst + WH * SM::PAGE, in_b ? p.Kc + off_b : g_zero_record, heads_b, &full[ls]);
+          bulk_load(dst + WH * (SM::PAGE + SM::REC), in_b ? p.Vc + off_b : g_zero_record, heads_b, &full[ls]);
+        }
       }
+      __syncwarp();
     }
-    __syncwarp();
-    if (++ls == DQ_STAGES) ls = 0;
+    if (WH > 1) turn = (turn + 1) % WH;
+    if (++ls == DQ_STAGES) ls = 0, lphase ^= 1;
     if (2 * ++lpair >= lw.count) {
       lpair = 0;
       more = lw.next(p, units);
-      aim = (size_t)(lw.at.hg / p.hgroups) * SM::REC;
+      take_aim();
     }
   };
-  aim = (size_t)(lw.at.hg / p.hgroups) * SM::REC;
-  for (int i = 0; i < DQ_STAGES - 1; ++i) load();
+  take_aim();
+  // Two pairs ahead: the slot that is filled next was read a pair ago, so that the set's warps need not
+  // keep pace exactly.
+  for (int i = 0; i < DQ_STAGES - 2; ++i) load();
 
   const int gq = lane >> 2, t = lane & 3;
   // Rows of the K tile (and columns of the V tile) are the page's tokens in the order that lets a
@@ -281,14 +308,14 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
     const Place& at = w.at;
     const int n = w.n, count = w.count, pairs = (count + 1) / 2;
     // Tokens of this segment: those behind it are another CTA's, or do not exist.
-    const long long here = (long long)n - at.page * 16;
-    const int tokens = (int)min((long long)count * 16, here);
-    const int g = at.hg / p.hgroups, h0 = g * hq + (at.hg % p.hgroups) * 8, nh = min(8, hq - (at.hg % p.hgroups) * 8);
+    const int tokens = (int)min(16LL * count, n - 16LL * at.page);
+    const int hg = at.hg * WH + wh;
+    const uint32_t mine = (hg / p.hgroups - at.hg * WH / p.hgroups) * SM::REC;  // this head's record in a slot
+    const int h0 = hg / p.hgroups * hq + (hg % p.hgroups) * 8, nh = min(8, hq - (hg % p.hgroups) * 8);
 
-    // Q as the B operand: column gq is head gq (SIDE: head gq & 3, for page gq >> 2 of the pair), the
-    // rows of step k of group x are elements 64 x + 16 t + 2 k, + 1 and the same + 8, as the words of
+    // Q as the B operand: column gq is head gq (SIDE: head gq & 3), the rows of step k of group x are elements 64 x + 16 t + 2 k, + 1 and the same + 8, as the words of
     // codes hold them; odd steps' nibbles weigh 16.
-    uint32_t qf[SIDE ? 2 : 1][NG][4][2];
+    uint32_t qf[NG][4][2];
     float qsum[NG][2];
     {
       const int hc = SIDE ? gq & 3 : gq;
@@ -307,15 +334,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
         for (int k = 0; k < 4; ++k) {
           s += lo_f32(w[k][0]) + hi_f32(w[k][0]) + lo_f32(w[k][1]) + hi_f32(w[k][1]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t v = (k & 1) ? mul_h2(w[k][e], 0x2c002c00u) : w[k][e];  // 1/16
-            if (SIDE) {
-              qf[0][x][k][e] = gq < 4 ? v : 0u;
-              qf[SIDE][x][k][e] = gq < 4 ? 0u : v;
-            } else {
-              qf[0][x][k][e] = v;
-            }
-          }
+          for (int e = 0; e < 2; ++e) qf[x][k][e] = (k & 1) ? mul_h2(w[k][e], 0x2c002c00u) : w[k][e];  // 1/16
         }
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
@@ -323,7 +342,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
         qsum[x][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);  // of column 2t + 1
       }
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float m[2] = {NO_MAX, NO_MAX}, l[2] = {0.f, 0.f};
     float F = 67108864.0f;  // fits the smallest scale, 2^-20: the first page sets it
     float acc[4 * NG][4], zacc[NG][2];
 #pragma unroll
@@ -333,14 +352,14 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 
     // One product's worth of tokens: a page, or (SIDE) a pair of pages at `pg`, `limit` tokens of them.
     auto tile = [&](uint32_t pg, int limit) {
-      const uint32_t own = pg + side * SM::PAGE;  // the page of this lane's scores
+      const uint32_t page = pg + side * (WH * SM::PAGE);  // the page of this lane's scores
       uint32_t hka, hkb, hva, hvb;  // headers of its two tokens: a pair of f16 (or one)
       if (NG == 2) {
-        hka = lds32(own + 8 * D + 4 * tok_a), hkb = lds32(own + 8 * D + 4 * tok_b);
-        hva = lds32(own + SM::REC + 8 * D + 4 * tok_a), hvb = lds32(own + SM::REC + 8 * D + 4 * tok_b);
+        hka = lds32(page + 8 * D + 4 * tok_a), hkb = lds32(page + 8 * D + 4 * tok_b);
+        hva = lds32(page + WH * SM::REC + 8 * D + 4 * tok_a), hvb = lds32(page + WH * SM::REC + 8 * D + 4 * tok_b);
       } else {
-        hka = lds16(own + 8 * D + 2 * tok_a), hkb = lds16(own + 8 * D + 2 * tok_b);
-        hva = lds16(own + SM::REC + 8 * D + 2 * tok_a), hvb = lds16(own + SM::REC + 8 * D + 2 * tok_b);
+        hka = lds16(page + 8 * D + 2 * tok_a), hkb = lds16(page + 8 * D + 2 * tok_b);
+        hva = lds16(page + WH * SM::REC + 8 * D + 2 * tok_a), hvb = lds16(page + WH * SM::REC + 8 * D + 2 * tok_b);
       }
       // Tokens behind the last one: stale headers may be NaN, and the scores are masked below.
       const bool tail = limit < (SIDE ? 32 : 16);
@@ -349,47 +368,61 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
         if (!ok_a) hka = hva = 0;
         if (!ok_b) hkb = hvb = 0;
       }
+      constexpr int NS = SIDE ? 2 : 1;
       float e[NG][4];
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
-        e[x][0] = e[x][1] = e[x][2] = e[x][3] = 0.f;
+        float ep[NS][4];
+        uint2 ua[NS], ub[NS];
 #pragma unroll
-        for (int s = 0; s < (SIDE ? 2 : 1); ++s) {
-          const uint32_t kb = pg + s * SM::PAGE + 32 * x + 8 * t;
-          const uint2 wa = lds64(kb + tok_a * (D / 2)), wb = lds64(kb + tok_b * (D / 2));
-          mma16816(e[x], wa.x & 0x000f000fu, wb.x & 0x000f000fu, wa.y & 0x000f000fu, wb.y & 0x000f000fu, qf[s][x][0][0], qf[s][x][0][1]);
-          mma16816(e[x], wa.x & 0x00f000f0u, wb.x & 0x00f000f0u, wa.y & 0x00f000f0u, wb.y & 0x00f000f0u, qf[s][x][1][0], qf[s][x][1][1]);
-          const uint32_t ax = wa.x >> 8, bx = wb.x >> 8, ay = wa.y >> 8, by = wb.y >> 8;
-          mma16816(e[x], ax & 0x000f000fu, bx & 0x000f000fu, ay & 0x000f000fu, by & 0x000f000fu, qf[s][x][2][0], qf[s][x][2][1]);
-          mma16816(e[x], ax & 0x00f000f0u, bx & 0x00f000f0u, ay & 0x00f000f0u, by & 0x00f000f0u, qf[s][x][3][0], qf[s][x][3][1]);
+        for (int s = 0; s < NS; ++s) {
+          const uint32_t k0 = pg + s * (WH * SM::PAGE) + 32 * x + 8 * t;
+          ua[s] = lds64(k0 + tok_a * (D / 2)), ub[s] = lds64(k0 + tok_b * (D / 2));
+          ep[s][0] = ep[s][1] = ep[s][2] = ep[s][3] = 0.f;
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {
+            const uint32_t mask = (k & 1) ? 0x00f000f0u : 0x000f000fu;
+            const int sh = 8 * (k >> 1);
+            mma16816(ep[s], (ua[s].x >> sh) & mask, (ub[s].x >> sh) & mask, (ua[s].y >> sh) & mask, (ub[s].y >> sh) & mask,
+                     qf[x][k][0], qf[x][k][1]);
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[x][i] = SIDE && side ? ep[NS - 1][i] : ep[0][i];
       }
-      float xa[2], xb[2];  // scores of columns 2t, 2t + 1 in the log2 domain
+      // Scores of columns 2t, 2t + 1 in the log2 domain, less `from`.
+      float xa[2], xb[2];
+      auto scores = [&](float from0, float from1) {
+        xa[0] = xb[0] = -from0, xa[1] = xb[1] = -from1;
 #pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        const uint32_t sa = hka & 0xfff0fff0u, za = hka & 0x000f000fu, sb = hkb & 0xfff0fff0u, zb = hkb & 0x000f000fu;
-        const float ka = (x ? hi_f32(sa) : lo_f32(sa)) * sc2, kza = x ? hi_f32(za) : lo_f32(za);
-        const float kbs = (x ? hi_f32(sb) : lo_f32(sb)) * sc2, kzb = x ? hi_f32(zb) : lo_f32(zb);
+        for (int x = 0; x < NG; ++x) {
+          const uint32_t sa = hka & 0xfff0fff0u, za = hka & 0x000f000fu, sb = hkb & 0xfff0fff0u, zb = hkb & 0x000f000fu;
+          const float ka = (x ? hi_f32(sa) : lo_f32(sa)) * sc2, kza = x ? hi_f32(za) : lo_f32(za);
+          const float kb = (x ? hi_f32(sb) : lo_f32(sb)) * sc2, kzb = x ? hi_f32(zb) : lo_f32(zb);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float ya = fmaf(-kza, qsum[x][c], e[x][c]), yb = fmaf(-kzb, qsum[x][c], e[x][2 + c]);
-          xa[c] = x ? fmaf(ka, ya, xa[c]) : ka * ya;
-          xb[c] = x ? fmaf(kbs, yb, xb[c]) : kbs * yb;
+          for (int c = 0; c < 2; ++c) {
+            xa[c] = fmaf(ka, fmaf(-kza, qsum[x][c], e[x][c]), xa[c]);
+            xb[c] = fmaf(kb, fmaf(-kzb, qsum[x][c], e[x][2 + c]), xb[c]);
+          }
         }
-      }
-      if (tail) {
-        if (!ok_a) xa[0] = xa[1] = -INFINITY;
-        if (!ok_b) xb[0] = xb[1] = -INFINITY;
-      }
+        if (tail) {
+          if (!ok_a) xa[0] = xa[1] = -INFINITY;
+          if (!ok_b) xb[0] = xb[1] = -INFINITY;
+        }
+      };
+      scores(m[0], m[1]);
       // The running maximum is lazy: renewed (and the sums rescaled) only when a score outgrew it by 2^8.
-      if (__any_sync(0xffffffffu, fmaxf(xa[0], xb[0]) > m[0] + GROW || fmaxf(xa[1], xb[1]) > m[1] + GROW)) {
+      if (__any_sync(0xffffffffu, fmaxf(fmaxf(xa[0], xb[0]), fmaxf(xa[1], xb[1])) > GROW)) {
+        scores(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float mx = fmaxf(xa[c], xb[c]);
 #pragma unroll
           for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           mx = fmaxf(m[c], mx);
-          const float f = m[c] == -INFINITY ? 0.f : ex2(m[c] - mx);  // (nothing to rescale before the first page)
+          const float f = ex2(m[c] - mx);
           m[c] = mx;
           l[c] *= f;
 #pragma unroll
@@ -397,8 +430,9 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 #pragma unroll
           for (int x = 0; x < NG; ++x) zacc[x][c] *= f;
         }
+        scores(m[0], m[1]);
       }
-      const float pa[2] = {ex2(xa[0] - m[0]), ex2(xa[1] - m[1])}, pb[2] = {ex2(xb[0] - m[0]), ex2(xb[1] - m[1])};
+      const float pa[2] = {ex2(xa[0]), ex2(xa[1])}, pb[2] = {ex2(xb[0]), ex2(xb[1])};
       l[0] += pa[0] + pb[0];
       l[1] += pa[1] + pb[1];
       // P = p s F: F, a power of two, keeps it in f16's range whatever the values' size. It follows the
@@ -422,6 +456,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
           for (int x = 0; x < NG; ++x) zacc[x][0] *= f, zacc[x][1] *= f;
         }
       }
+      uint32_t bf[NG][2][2];  // P as the B operand: SIDE: of either page; else its hi and its lo
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
         const uint32_t za = hva & 0x000f000fu, zb = hvb & 0x000f000fu;
@@ -434,16 +469,22 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
         const uint32_t bh0 = movm_t(pha), bh1 = movm_t(phb);
         const uint32_t bl0 = movm_t(pack_h2(a0 - lo_f32(pha), a1 - hi_f32(pha)));
         const uint32_t bl1 = movm_t(pack_h2(b0 - lo_f32(phb), b1 - hi_f32(phb)));
-        // SIDE: columns 0..3 of (bh, bl) are the first page's, 4..7 the second's. The first page's
-        // product takes its hi in columns 0..3 and its lo in 4..7, the second's the other way round.
-        uint32_t ol0 = 0, ol1 = 0;
-        if (SIDE) ol0 = __shfl_xor_sync(0xffffffffu, bl0, 16), ol1 = __shfl_xor_sync(0xffffffffu, bl1, 16);
+        if (SIDE) {
+          // Columns 0..3 of (bh, bl) are the first page's, 4..7 the second's. The first page's product takes
+          // its hi in columns 0..3 and its lo in 4..7, the second's the other way round.
+          const uint32_t ol0 = __shfl_xor_sync(0xffffffffu, bl0, 16), ol1 = __shfl_xor_sync(0xffffffffu, bl1, 16);
+          bf[x][0][0] = gq < 4 ? bh0 : ol0, bf[x][0][1] = gq < 4 ? bh1 : ol1;
+          bf[x][1][0] = gq < 4 ? ol0 : bh0, bf[x][1][1] = gq < 4 ? ol1 : bh1;
+        } else {
+          bf[x][0][0] = bh0, bf[x][0][1] = bh1, bf[x][1][0] = bl0, bf[x][1][1] = bl1;
+        }
+      }
 #pragma unroll
-        for (int s = 0; s < (SIDE ? 2 : 1); ++s) {
-          const bool hi = !SIDE || (gq < 4) == (s == 0);
-          const uint32_t b_0 = hi ? bh0 : ol0, b_1 = hi ? bh1 : ol1;
+      for (int x = 0; x < NG; ++x) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
           // V^T: a lane's word gq of the group, for its four tokens; two tokens' halves side by side.
-          const uint32_t v = pg + s * SM::PAGE + SM::REC + 32 * x + 4 * gq + t * (D / 2);
+          const uint32_t v = pg + s * (WH * SM::PAGE) + WH * SM::REC + 32 * x + 4 * gq + t * (D / 2);
           const uint32_t w0 = lds32(v), w1 = lds32(v + 2 * D), w2 = lds32(v + 4 * D), w3 = lds32(v + 6 * D);
           const uint32_t lo01 = __byte_perm(w0, w1, 0x5410), hi01 = __byte_perm(w0, w1, 0x7632);
           const uint32_t lo23 = __byte_perm(w2, w3, 0x5410), hi23 = __byte_perm(w2, w3, 0x7632);
@@ -453,14 +494,15 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
             // e3; 3: e5, e7. Rows 8..15 always weigh 16, so one constant operand serves all.
             const uint32_t v01 = (k & 2 ? hi01 : lo01) >> (8 * (k & 1)), v23 = (k & 2 ? hi23 : lo23) >> (8 * (k & 1));
             const uint32_t a_0 = v01 & 0x000f000fu, a_1 = v01 & 0x00f000f0u, a_2 = v23 & 0x000f000fu, a_3 = v23 & 0x00f000f0u;
-            mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, b_0, b_1);
-            mma16816(acc[4 * x + k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b_0, b_1);  // -8 of each
-            if (!SIDE) {
-              mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bl0, bl1);
-              mma16816(acc[4 * x + k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, bl0, bl1);
-            }
+            mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bf[x][s][0], bf[x][s][1]);
+            if (!SIDE) mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bf[x][1][0], bf[x][1][1]);
           }
         }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // -8 of each code
+            mma16816(acc[4 * x + k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, bf[x][s][0], bf[x][s][1]);
       }
     };
 
@@ -468,11 +510,12 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       load();
       const int limit = tokens - 32 * j;
       mbar_wait(&full[cs], phase, p.status, 502);
-      const uint32_t pg = ring_u + cs * SM::STAGE;
+      const uint32_t pg = ring_u + cs * (WH * SM::STAGE) + mine;
       tile(pg, min(limit, 32));
-      if (!SIDE && limit > 16) tile(pg + SM::PAGE, min(limit - 16, 16));
+      if (!SIDE && limit > 16) tile(pg + WH * SM::PAGE, min(limit - 16, 16));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[cs]);
       if (++cs == DQ_STAGES) cs = 0, phase ^= 1;
-      __syncwarp();  // the slot may be filled again
     }
 
     // ---- the segment's result ---------------------------------------------------------------------------
@@ -524,7 +567,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
     if (lane == 0 && !whole && at.page == 0) {
       // The unit is cut at this warp's end: the next ones go on with it.
       int* d = p.desc + 4 * worker;
-      d[0] = at.b, d[1] = at.hg;
+      d[0] = at.b, d[1] = hg;
       d[2] = 1 + (int)((w.np - count + share - 1) / share);
     }
   }
@@ -540,49 +583,79 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 }
 
 // Joins the partials of the unit that is cut at the end of a warp's share, if there is one: that
-// warp's second slot and the first slots of the warps that follow. One warp per (worker, head).
-template <int D>
-__global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p, int heads, int workers) {
+// warp's second slot and the first slots of the warps that follow (`wh` apart). One block per share:
+// HP heads, 8 / HP warps each, four partials in flight per warp (a long context has dozens).
+template <int D, int HP>
+__global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p, int wh) {
   pdl_wait();
   pdl_launch();
-  const int i0 = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int worker = i0 / heads, hh = i0 % heads;
-  if (worker >= workers) return;
-  const int* d = p.desc + 4 * worker;
+  constexpr int NSP = 8 / HP, V = D / 32;
+  __shared__ float other[8][D + 2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hh = warp % HP, sp = warp / HP;
+  const int* d = p.desc + 4 * blockIdx.x;
   const int b = d[0], hg = d[1], pieces = d[2];
   if (pieces < 2) return;
   const int hq = p.H / p.G, h0 = (hg / p.hgroups) * hq + (hg % p.hgroups) * 8, nh = min(8, hq - (hg % p.hgroups) * 8);
-  if (hh >= nh) return;
-  auto slot = [&](int i) { return p.part + ((size_t)(worker + i) * 2 + (i == 0 ? 1 : 0)) * DQ_SLOT * (D + 2); };
-  float m = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) m = fmaxf(m, slot(i)[DQ_SLOT * D + hh]);
+  float m = NO_MAX, l = 0.f, a[V];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float l = 0.f, a[D / 32];
+  for (int k = 0; k < V; ++k) a[k] = 0.f;
+  for (int i0 = sp; i0 < pieces && hh < nh; i0 += 4 * NSP) {
+    float mi[4], li[4], ai[4][V];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) a[i] = 0.f;
-  for (int i = 0; i < pieces; ++i) {
-    const float* s = slot(i);
-    const float mi = s[DQ_SLOT * D + hh];
-    const float f = mi == -INFINITY ? 1.f : ex2(mi - m);  // (only where its scores were all NaN, and so are its sums)
-    l = fmaf(s[DQ_SLOT * (D + 1) + hh], f, l);
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * NSP;
+      const bool in = i < pieces;
+      const float* s = p.part + ((size_t)(blockIdx.x + (in ? i : 0) * wh) * 2 + (in && i > 0 ? 0 : 1)) * DQ_SLOT * (D + 2);
+      mi[u] = in ? s[DQ_SLOT * D + hh] : NO_MAX;
+      li[u] = in ? s[DQ_SLOT * (D + 1) + hh] : 0.f;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) a[k] = fmaf(s[hh * D + lane + 32 * k], f, a[k]);
+      for (int k = 0; k < V; ++k) ai[u][k] = in ? s[hh * D + lane + 32 * k] : 0.f;
+    }
+    const float m2 = fmaxf(fmaxf(m, fmaxf(mi[0], mi[1])), fmaxf(mi[2], mi[3])), f = ex2(m - m2);
+    l *= f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) a[k] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float fu = ex2(mi[u] - m2);
+      l = fmaf(li[u], fu, l);
+#pragma unroll
+      for (int k = 0; k < V; ++k) a[k] = fmaf(ai[u][k], fu, a[k]);
+    }
+    m = m2;
   }
+  if (NSP > 1) {
 #pragma unroll
-  for (int k = 0; k < D / 32; ++k)
+    for (int k = 0; k < V; ++k) other[warp][lane + 32 * k] = a[k];
+    if (lane == 0) other[warp][D] = m, other[warp][D + 1] = l;
+    __syncthreads();
+    if (sp > 0) return;
+#pragma unroll
+    for (int o = 1; o < NSP; ++o) {
+      const float* s = other[warp + o * HP];
+      const float m2 = fmaxf(m, s[D]), f = ex2(m - m2), fo = ex2(s[D] - m2);
+      l = fmaf(l, f, s[D + 1] * fo);
+#pragma unroll
+      for (int k = 0; k < V; ++k) a[k] = fmaf(a[k], f, s[lane + 32 * k] * fo);
+      m = m2;
+    }
+  }
+  if (hh >= nh) return;
+#pragma unroll
+  for (int k = 0; k < V; ++k)
     p.O[((size_t)b * p.H + h0 + hh) * D + lane + 32 * k] = __float2half_rn(a[k] / l);
 }
 
-template <int D, bool SIDE>
-int run(Ctx* c, Op& op, DqParams p) {
-  const int grid = op.p1, workers = grid * DQ_WARPS, heads = min(8, p.H / p.G);
-  TB_CUDA(c, launch_k(c, decode_q4_kernel<D, SIDE>, dim3(grid), dim3(DQ_THREADS), DqSmem<D>::TOTAL, 1, p));
-  c->launches += 1;
-  TB_CUDA(c, launch_k(c, decode_q4_join_kernel<D>, dim3((workers * heads + 7) / 8), dim3(256), 0, 1, p, heads, workers));
-  c->launches += 1;
-  return 0;
+int set_of(int sets) { return sets % 4 == 0 ? 4 : sets % 2 == 0 ? 2 : 1; }
+
+// The kernel for a head_dim, at most four heads per KV head or more, and sets of one, two or four.
+typedef void (*DqKernel)(DqParams);
+template <int D>
+DqKernel kernel_of(bool side, int wh) {
+  if (side) return wh == 4 ? decode_q4_kernel<D, true, 4> : wh == 2 ? decode_q4_kernel<D, true, 2> : decode_q4_kernel<D, true, 1>;
+  return wh == 4 ? decode_q4_kernel<D, false, 4> : wh == 2 ? decode_q4_kernel<D, false, 2> : decode_q4_kernel<D, false, 1>;
 }
+DqKernel kernel_of(int D, int hq, int wh) { return D == 128 ? kernel_of<128>(hq <= 4, wh) : kernel_of<64>(hq <= 4, wh); }
 
 }  // namespace
 
@@ -600,11 +673,8 @@ int make_decode_q4(Ctx* c, Op& op, const Q4Shape& q) {
   op.p1 = (int)(most < fit ? most : fit);
   op.scratch_bytes = (size_t)op.p1 * DQ_WARPS * (2 * DQ_SLOT * (q.D + 2) * sizeof(float) + 16);
   TB_CUDA(c, cudaMalloc(&op.scratch, op.scratch_bytes));
-  auto attr = [&](auto kern, int bytes) { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); };
-  TB_CUDA(c, attr(decode_q4_kernel<128, true>, DqSmem<128>::TOTAL));
-  TB_CUDA(c, attr(decode_q4_kernel<128, false>, DqSmem<128>::TOTAL));
-  TB_CUDA(c, attr(decode_q4_kernel<64, true>, DqSmem<64>::TOTAL));
-  TB_CUDA(c, attr(decode_q4_kernel<64, false>, DqSmem<64>::TOTAL));
+  TB_CUDA(c, cudaFuncSetAttribute(kernel_of(q.D, H / q.G, set_of(units)), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  q.D == 128 ? DqSmem<128>::TOTAL : DqSmem<64>::TOTAL));
   return 0;
 }
 
@@ -619,17 +689,20 @@ int launch_decode_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
   p.scale = bits_f32(a[6]);
   p.B = (int)op.shapes[0][0], p.H = (int)op.shapes[0][1], p.G = q.G, p.NP = q.NP, p.MP = (int)op.shapes[3][1];
   p.hgroups = (p.H / p.G + 7) / 8;
+  const int wh = set_of(p.G * p.hgroups);
+  p.units = p.G * p.hgroups / wh;
   p.least = DQ_LEAST;
   p.status = c->status;
   p.part = (float*)op.scratch;
   p.desc = (int*)(p.part + (size_t)op.p1 * DQ_WARPS * 2 * DQ_SLOT * (q.D + 2));
-  const bool side = p.H / p.G <= 4;
-  int r;
-  if (q.D == 128)
-    r = side ? run<128, true>(c, op, p) : run<128, false>(c, op, p);
-  else
-    r = side ? run<64, true>(c, op, p) : run<64, false>(c, op, p);
-  return r;
+  const bool few = p.H / p.G <= 4;
+  TB_CUDA(c, launch_k(c, kernel_of(q.D, p.H / p.G, wh), dim3(op.p1), dim3(DQ_THREADS),
+                      q.D == 128 ? DqSmem<128>::TOTAL : DqSmem<64>::TOTAL, 1, p));
+  TB_CUDA(c, launch_k(c, q.D == 128 ? (few ? decode_q4_join_kernel<128, 4> : decode_q4_join_kernel<128, 8>)
+                                    : (few ? decode_q4_join_kernel<64, 4> : decode_q4_join_kernel<64, 8>),
+                      dim3(op.p1 * DQ_WARPS), dim3(256), 0, 1, p, wh));
+  c->launches += 2;
+  return 0;
 }
 
 }  // namespace tb
