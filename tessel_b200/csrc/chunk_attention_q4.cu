@@ -371,54 +371,80 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
       } while (w.next(p));
     }
   } else if (warp < 8) {
-    // ---- unpack: a thread takes 32 neighbouring elements of a key at a time ---------------------------
-    constexpr int PARTS = D / 32;  // 16-byte pieces of a row of codes
-    const int tid = threadIdx.x - 128, part = tid % PARTS;
+    // ---- unpack: a thread takes 32 neighbouring elements of a key, of ITER keys a fixed distance apart ----
+    // (straight-line code: the loads of all its keys are in flight before the first is used)
+    constexpr int PARTS = D / 32;           // 16-byte pieces of a row of codes
+    constexpr int STEP = 128 / PARTS;       // keys between a thread's keys
+    constexpr int ITER = CQ_BN / STEP;
+    static_assert(STEP % 16 == 0, "a thread's keys have one place in their pages");
+    const int tid = threadIdx.x - 128, part = tid % PARTS, key0 = tid / PARTS;
+    const int from = (key0 >> 4) * SM::REC + (key0 & 15) * (D / 2) + part * 16;
+    const int head_from = (key0 >> 4) * SM::REC + 8 * D + 2 * ((key0 & 15) * SUB + (part >> 1));
+    // The four 16-byte chunks this thread's words become, in the swizzled tile. Pieces 2 and 3 lie in the
+    // other 64-column block, at the same banks: they go in another order.
+    uint32_t to[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      to[i] = (part >> 1) * (CQ_BN * 128) + key0 * 128 + (((((part & 1) * 4 + (i ^ (part & 2))) ^ (key0 & 7))) << 4);
+    const __half2 R = __float2half2_rn(0.0625f);
     int item = 0, unit = 0;
     do {
       const int slim = w.r.pos0 + w.r.nrows;
       for (int k = w.k0; k < w.k1; ++k) {
+        const bool tail = (k + 1) * CQ_BN > slim;
 #pragma unroll 1
         for (int v = 0; v < 2; ++v, ++item) {
           const int rs = item % NRAW, s = item % NSLOT;
           mbar_wait(&raw_full[rs], (item / NRAW) & 1, p.status, 606);
-          if (item >= NSLOT) mbar_wait(&kv_empty[s], (item / NSLOT - 1) & 1, p.status, 607);
           const unsigned char* raw = smem + SM::OFF_RAW + rs * SM::RAW;
+          uint4 u[ITER];
+          uint32_t head[ITER];
+#pragma unroll
+          for (int j = 0; j < ITER; ++j) {
+            u[j] = *reinterpret_cast<const uint4*>(raw + from + j * (STEP / 16) * SM::REC);
+            head[j] = *reinterpret_cast<const unsigned short*>(raw + head_from + j * (STEP / 16) * SM::REC);
+          }
+          if (tail) {
+#pragma unroll
+            for (int j = 0; j < ITER; ++j)
+              if (k * CQ_BN + key0 + j * STEP >= slim) head[j] = 0;  // stale behind the last key
+          }
+          if (v) {
+            bool spoilt = false;
+#pragma unroll
+            for (int j = 0; j < ITER; ++j) spoilt |= (head[j] & 0x7c00u) == 0x7c00u;
+            if (spoilt) {
+#pragma unroll
+              for (int j = 0; j < ITER; ++j)
+                if ((head[j] & 0x7c00u) == 0x7c00u) {
+                  atomicMin(&nan_at[(unit & 3) * 2 + (part >> 1)], k * CQ_BN + key0 + j * STEP);
+                  head[j] = 0;
+                }
+            }
+          }
+          if (item >= NSLOT) mbar_wait(&kv_empty[s], (item / NSLOT - 1) & 1, p.status, 607);
           unsigned char* dst = smem + SM::OFF_KV + s * SM::KV_BYTES;
-#pragma unroll 4
-          for (int key = tid / PARTS; key < CQ_BN; key += 128 / PARTS) {
-            const unsigned char* rec = raw + (key >> 4) * SM::REC;
-            uint4 u = *reinterpret_cast<const uint4*>(rec + (key & 15) * (D / 2) + part * 16);
-            uint32_t head = *reinterpret_cast<const unsigned short*>(rec + 8 * D + 2 * ((key & 15) * SUB + (part >> 1)));
-            if (k * CQ_BN + key >= slim) head = 0;  // stale behind the last key
-            if (v && (head & 0x7c00u) == 0x7c00u) {
-              atomicMin(&nan_at[(unit & 3) * 2 + (part >> 1)], k * CQ_BN + key);
-              head = 0;
-            }
-            const uint32_t z = head & 15u;
-            uint32_t sc = head & 0xfff0u, c0 = 0xe400u | z, c1 = 0xd400u | (z << 4);  // scale, -(1024 + z), -(64 + z)
-            sc |= sc << 16, c0 |= c0 << 16, c1 |= c1 << 16;
-            const __half2 S = *reinterpret_cast<__half2*>(&sc), A = *reinterpret_cast<__half2*>(&c0), B = *reinterpret_cast<__half2*>(&c1);
-            const __half2 R = __float2half2_rn(0.0625f);
-            // Pieces 2 and 3 lie in the other 64-column block, at the same banks: they go in another order.
-            if (part & 2) {
-              uint32_t x = u.x;
-              u.x = u.z, u.z = x, x = u.y, u.y = u.w, u.w = x;
-            }
+#pragma unroll
+          for (int j = 0; j < ITER; ++j) {
+            const uint32_t z = head[j] & 15u;
+            // Scale, -(1024 + z) and -(64 + z), twice each.
+            const uint32_t sc = __byte_perm(head[j] & 0xfff0u, 0, 0x1010), c0 = (z | z << 16) | 0xe400e400u,
+                           c1 = (z << 4 | z << 20) | 0xd400d400u;
+            const __half2 S = *reinterpret_cast<const __half2*>(&sc), A = *reinterpret_cast<const __half2*>(&c0), B = *reinterpret_cast<const __half2*>(&c1);
+            const uint32_t word[4] = {part & 2 ? u[j].z : u[j].x, part & 2 ? u[j].w : u[j].y, part & 2 ? u[j].x : u[j].z, part & 2 ? u[j].y : u[j].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t word = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w, up = word >> 8;
-              uint32_t e[4] = {(word & 0x000f000fu) | 0x64006400u, (word & 0x00f000f0u) | 0x64006400u,
+              const uint32_t up = word[i] >> 8;
+              uint32_t e[4] = {(word[i] & 0x000f000fu) | 0x64006400u, (word[i] & 0x00f000f0u) | 0x64006400u,
                                (up & 0x000f000fu) | 0x64006400u, (up & 0x00f000f0u) | 0x64006400u};
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                __half2 x = *reinterpret_cast<__half2*>(&e[j]);
-                x = (j & 1) ? __hfma2(x, R, B) : __hadd2(x, A);  // code - zero point, exactly
+              for (int q = 0; q < 4; ++q) {
+                __half2 x = *reinterpret_cast<__half2*>(&e[q]);
+                x = (q & 1) ? __hfma2(x, R, B) : __hadd2(x, A);  // code - zero point, exactly
                 x = __hmul2(x, S);
-                e[j] = *reinterpret_cast<uint32_t*>(&x);
+                e[q] = *reinterpret_cast<uint32_t*>(&x);
               }
-              const int ch = ((part & 1) * 4 + (i ^ (part & 2))) ^ (key & 7);
-              *reinterpret_cast<uint4*>(dst + (part >> 1) * (CQ_BN * 128) + key * 128 + ch * 16) = make_uint4(e[0], e[1], e[2], e[3]);
+              *reinterpret_cast<uint4*>(dst + to[i] + j * STEP * 128) = make_uint4(e[0], e[1], e[2], e[3]);
             }
           }
           fence_proxy_async();
