@@ -11,7 +11,7 @@
 // rounds nothing.
 //
 // Roles of a CTA's sixteen warps: warp 0 brings Q (TMA) and the pages' 4-bit records (bulk copies);
-// warp 1 issues the MMAs; warps 4-7 unpack a 128-key tile of K or V into the 128-byte-swizzled layout
+// warps 1 and 2 issue the MMAs, one for each tile; warps 4-7 unpack a 128-key tile of K or V into the 128-byte-swizzled layout
 // the tensor cores read; warps 8-15 are two softmax warpgroups, one query row per thread.
 //
 // Rows. The M = 128 rows of a tile are (token, query head) pairs of ONE KV head: 128 / hq tokens times
@@ -21,7 +21,10 @@
 // Work split. A unit is (piece, KV head, block of two tiles); its work is the 128-key tiles its last
 // row sees. The units' tiles form one list, a CTA takes an equal, contiguous share of it (one CTA per
 // SM), whatever the pieces' lengths are. A unit that is cut leaves one partial in each CTA (f32
-// numerator, maximum and sum), which a second kernel joins.
+// numerator, maximum and sum), which a second kernel joins. A block that fits one tile (a piece of a
+// few rows) is worked on by both: they hold the same rows, one takes the first 64 keys of every 128,
+// the other the second, and their results are joined at the end. (One softmax warpgroup alone waits
+// for its own latencies: 1.9 us per 128 keys against 1.25 us for two of them.)
 //
 // NaN. A weight of zero times a NaN is a NaN, so a spoilt V row would reach rows that do not see it.
 // The unpacking warps store zeros for it instead and note the least such position of each 64-column
@@ -35,7 +38,7 @@ namespace {
 constexpr int CQ_BM = 128;       // rows of a tile
 constexpr int CQ_BN = 128;       // keys of a K / V tile
 constexpr int CQ_SN = 64;        // keys of a sub-block: the unit of S, softmax and P V
-constexpr int CQ_THREADS = 512;  // 0 TMA, 1 MMA, (2, 3 idle), 4-7 unpack, 8-15 softmax
+constexpr int CQ_THREADS = 512;  // warps 0 TMA, 1-2 MMA, (3 idle), 4-7 unpack, 8-15 softmax
 constexpr int CQ_LEAST = 2;      // tiles a CTA takes at least
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.0f;
@@ -68,7 +71,8 @@ struct CqSmem {
   static constexpr int OFF_KV = 2 * Q_TILE;
   static constexpr int OFF_RAW = OFF_KV + NSLOT * KV_BYTES;
   static constexpr int OFF_BAR = OFF_RAW + NRAW * RAW;
-  static constexpr int TOTAL = OFF_BAR + 40 * 8 + 1024;
+  static constexpr int OFF_EX = OFF_BAR + 40 * 8;  // a narrow unit's maxima [2][128] and sums [128]
+  static constexpr int TOTAL = OFF_EX + 3 * 128 * 4 + 1024;
   static constexpr int TMEM_COLS = 512;
   static_assert(TOTAL <= 227 * 1024, "shared memory");
   static_assert(RAW % 128 == 0 && OFF_BAR % 8 == 0, "alignment");
@@ -91,8 +95,8 @@ struct Piece {
   int row0, nrows, pos0, blocks;
 };
 __device__ __forceinline__ Piece piece_of(const CqParams& p, int c) {
-  const int* m = p.meta + 4 * c;
-  Piece r = {m[0], m[1], m[2], 0};
+  const int4 m = *reinterpret_cast<const int4*>(p.meta + 4 * c);
+  Piece r = {m.x, m.y, m.z, 0};
   if (r.row0 < 0 || r.nrows <= 0 || r.pos0 < 0 || r.nrows > p.T - r.row0 || r.nrows > 0x7fffffff - 256 - r.pos0)
     r.nrows = 0;
   r.blocks = (r.nrows + 2 * p.tm - 1) / (2 * p.tm);
@@ -108,9 +112,11 @@ struct Walk {
   int c, g, i, left, share;
   Piece r;
   int tiles, k0, k1;
+  bool narrow;  // the block's rows fit one tile
 
   __device__ __forceinline__ void set(const CqParams& p, int from) {
     tiles = tiles_of(p, r, i);
+    narrow = r.nrows - i * 2 * p.tm <= p.tm;
     k0 = from;
     k1 = left < tiles - from ? from + left : tiles;
     left -= k1 - k0;
@@ -188,17 +194,18 @@ __device__ __forceinline__ bool find_walk(const CqParams& p, long long* scan, Wa
   return true;
 }
 
-// Sub-blocks of keys that tile `t` of the current unit visits in this CTA's part, and its last key + 1.
+// Sub-blocks of keys that tile `t` of the current unit visits in this CTA's part. In a narrow unit
+// sub-block n of tile t is half t of K / V tile n, else half n & 1 of tile n >> 1.
 __device__ __forceinline__ int subs_of(const CqParams& p, const Walk& w, int t) {
-  const int first = w.i * 2 * p.tm + t * p.tm;
+  const int first = w.i * 2 * p.tm + (w.narrow ? 0 : t * p.tm);
   if (first >= w.r.nrows) return 0;
   const int end = min(CQ_BN * w.k1, w.r.pos0 + min(first + p.tm, w.r.nrows));
-  return max(0, (end - CQ_BN * w.k0 + CQ_SN - 1) / CQ_SN);
+  const int subs = max(0, (end - CQ_BN * w.k0 + CQ_SN - 1) / CQ_SN);
+  return w.narrow ? (subs + 1 - t) / 2 : subs;
 }
 
 template <int D>
 __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_constant__ CUtensorMap mapQ, const CqParams p) {
-  pdl_wait();
   using SM = CqSmem<D>;
   constexpr int SUB = SM::SUB, NSLOT = SM::NSLOT, NRAW = SM::NRAW;
   extern __shared__ unsigned char smem_raw[];
@@ -217,22 +224,16 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
   int* nan_at = (int*)(bars + 31);      // [unit & 3][group]: least position of a spoilt V row
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) p.desc[4 * blockIdx.x + 3] = 0;
-  Walk w;
-  if (!find_walk(p, (long long*)(smem + SM::OFF_KV), &w)) {
-    pdl_launch();
-    return;
-  }
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_free, 1);
+    mbar_init(q_free, 2);
     for (int i = 0; i < NRAW; ++i) {
       mbar_init(&raw_full[i], 1);
       mbar_init(&raw_empty[i], 4);
     }
     for (int i = 0; i < NSLOT; ++i) {
       mbar_init(&kv_full[i], 128);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
@@ -247,11 +248,17 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  pdl_wait();
+  if (threadIdx.x == 0) p.desc[4 * blockIdx.x + 3] = 0;
+  Walk w;
+  const bool busy = find_walk(p, (long long*)(smem + SM::OFF_KV), &w);
+  __syncthreads();  // the prefix sums lie where the first tile will
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp < 4) {
+  if (!busy) {
+    // Nothing to do but to give the tensor memory back.
+  } else if (warp < 4) {
     if (warp == 0) {
       // ---- Q and the records of K and V tiles, in the order K V K V ... -----------------------------
       if (lane == 0) prefetch_tmap(&mapQ);
@@ -265,15 +272,19 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int sub = 0; sub < SUB; ++sub)
-              tma_load_3d(smem + t * SM::Q_TILE + sub * (CQ_BM * 128), &mapQ, q_full, sub * 64, w.g * p.hq, row + t * p.tm);
+              tma_load_3d(smem + t * SM::Q_TILE + sub * (CQ_BM * 128), &mapQ, q_full, sub * 64, w.g * p.hq, row + (w.narrow ? 0 : t * p.tm));
         }
         const int slim = w.r.pos0 + w.r.nrows;
-        for (int k = w.k0; k < w.k1; ++k) {
-          // Lane j < 8: the page of keys [128 k + 16 j, + 16). Beyond the table: page 0; behind the last
-          // key, or outside the cache: zeros.
+        // Lane j < 8: the page of keys [128 k + 16 j, + 16). Beyond the table: page 0; behind the last key,
+        // or outside the cache: zeros. Looked up a tile ahead.
+        auto page_of = [&](int k) {
           const int col = k * 8 + (lane & 7);
-          int page = -1;
-          if (col * 16 < slim) page = col < p.MP ? p.table[(size_t)w.r.row0 * p.MP + col] : 0;
+          return k >= w.k1 || (long long)col * 16 >= slim ? -1 : col < p.MP ? p.table[(size_t)w.r.row0 * p.MP + col] : 0;
+        };
+        int next = page_of(w.k0);
+        for (int k = w.k0; k < w.k1; ++k) {
+          const int page = next;
+          next = page_of(k + 1);
           const bool in = page >= 0 && page < p.NP;
           const size_t off = ((size_t)(in ? page : 0) * p.G + w.g) * SM::REC;
 #pragma unroll
@@ -291,15 +302,20 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
         }
         ++unit;
       } while (w.next(p));
-    } else if (warp == 1 && elect_one()) {
-      // ---- MMA issue -------------------------------------------------------------------------------
+    } else if (warp < 3 && elect_one()) {
+      // ---- MMA issue: a warp per tile -----------------------------------------------------------------
+      // (One thread issuing for both was the kernel's clock: with its waits and fences it took 2240 cycles
+      // for a sub-block of both tiles, whose products take 1024.)
       constexpr uint32_t idesc_s = umma_idesc_f16(CQ_BM, CQ_SN, 0, 0);
       constexpr uint32_t idesc_o = umma_idesc_f16(CQ_BM, D, 0, 1);
-      int base = 0;             // K and V tiles of earlier units
-      int done[2] = {0, 0};     // sub-blocks of earlier units, per tile: buffers and phases follow from the running count
+      const int t = warp - 1;
+      const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * D;
+      const uint64_t qd = umma_desc_sw128(smem_u32(smem + t * SM::Q_TILE), 16, 1024);
+      int base = 0, done = 0;   // K and V tiles, and this tile's sub-blocks, of earlier units: buffers and phases follow
       int ready = 0, unit = 0;  // tiles [0, ready) have been unpacked
       auto slot_addr = [&](int item) { return smem_u32(smem + SM::OFF_KV + (item % NSLOT) * SM::KV_BYTES); };
       auto need = [&](int item) {
+        if (ready > item) return;
         while (ready <= item) {
           mbar_wait(&kv_full[ready % NSLOT], (ready / NSLOT) & 1, p.status, 603);
           ++ready;
@@ -307,66 +323,63 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
         tc_fence_after();
       };
       do {
-        const int nsub[2] = {subs_of(p, w, 0), subs_of(p, w, 1)};
-        const int nmax = max(nsub[0], nsub[1]), nitems = 2 * (w.k1 - w.k0);
-        auto issue_s = [&](int t, int n) {
-          const int b = (done[t] + n) & 1;
-          const uint32_t qa = smem_u32(smem + t * SM::Q_TILE);
-          const uint32_t ka = slot_addr(base + 2 * (n >> 1)) + (n & 1) * (CQ_SN * 128);
+        const int nt = subs_of(p, w, t), nitems = 2 * (w.k1 - w.k0);
+        // Sub-block n's K (V) tile, its half of it, and whether it is the tile's last sub-block.
+        auto tile_of = [&](int n) { return w.narrow ? n : n >> 1; };
+        auto half_of = [&](int n) { return w.narrow ? t : n & 1; };
+        auto last_of = [&](int n) { return w.narrow || (n & 1); };
+        // (Descriptors hold addresses in units of 16 bytes.)
+        auto issue_s = [&](int n) {
+          const int b = (done + n) & 1;
+          const uint64_t kd0 = umma_desc_sw128(slot_addr(base + 2 * tile_of(n)) + half_of(n) * (CQ_SN * 128), 16, 1024);
 #pragma unroll
           for (int kd = 0; kd < D / 16; ++kd) {
-            const uint32_t off = (kd >> 2) * (CQ_BM * 128) + (kd & 3) * 32;
-            umma_f16(tmem + t * 128 + b * CQ_SN, umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024),
-                     idesc_s, kd > 0 ? 1u : 0u);
+            const uint32_t off = ((kd >> 2) * (CQ_BM * 128) + (kd & 3) * 32) >> 4;
+            umma_f16(ts + b * CQ_SN, qd + off, kd0 + off, idesc_s, kd > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[t * 2 + b]);
         };
-        auto issue_pv = [&](int t, int n) {
-          const int b = (done[t] + n) & 1;
-          const uint32_t va = slot_addr(base + 2 * (n >> 1) + 1);
+        auto issue_pv = [&](int n) {
+          const int b = (done + n) & 1;
+          const uint64_t vd = umma_desc_sw128(slot_addr(base + 2 * tile_of(n) + 1) + half_of(n) * (CQ_SN * 128), CQ_BN * 128, 1024);
 #pragma unroll
           for (int kk = 0; kk < CQ_SN / 16; ++kk)
-            umma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + b * CQ_SN + kk * 8,
-                        umma_desc_sw128(va + ((n & 1) * (CQ_SN / 16) + kk) * 2048, CQ_BN * 128, 1024), idesc_o,
-                        (n > 0 || kk > 0) ? 1u : 0u);
+            umma_f16_ts(to, ts + b * CQ_SN + kk * 8, vd + kk * (2048 >> 4), idesc_o, (n > 0 || kk > 0) ? 1u : 0u);
           umma_commit(&o_done[t * 2 + b]);
         };
         mbar_wait(q_full, unit & 1, p.status, 604);
-        need(base);
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (n < nsub[t]) issue_s(t, n);
-        umma_commit(&kv_empty[base % NSLOT]);  // K tile 0 is free once these are done
-        for (int n = 0; n < nmax; ++n) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (n < nsub[t]) {
-              const int b = done[t] + n;
-              mbar_wait(&p_ready[t * 2 + (b & 1)], (b >> 1) & 1, p.status, 605);
-              tc_fence_after();
-              need(base + 2 * (n >> 1) + 1);
-              issue_pv(t, n);
-            }
-            if (n + 2 < nsub[t]) {
-              need(base + 2 * ((n + 2) >> 1));
-              issue_s(t, n + 2);
-            }
-          }
-          if (n & 1) {
-            // Both halves of V tile n >> 1 and of K tile (n >> 1) + 1 have been issued for both tiles.
-            umma_commit(&kv_empty[(base + n) % NSLOT]);
-            if (n + 1 < nitems) umma_commit(&kv_empty[(base + n + 1) % NSLOT]);
+        tc_fence_after();
+        // A K or V tile is given back once its products are issued; those that no sub-block of this tile
+        // reads (a last one's second half, keys behind its rows) at the end.
+        int freed_k = 0, freed_v = 0;
+        for (int n = 0; n < 2 && n < nt; ++n) {
+          need(base + 2 * tile_of(n));
+          issue_s(n);
+          if (last_of(n)) umma_commit(&kv_empty[(base + 2 * freed_k++) % NSLOT]);
+        }
+        for (int n = 0; n < nt; ++n) {
+          const int b = done + n;
+          need(base + 2 * tile_of(n) + 1);
+          mbar_wait(&p_ready[t * 2 + (b & 1)], (b >> 1) & 1, p.status, 605);
+          tc_fence_after();
+          issue_pv(n);
+          if (last_of(n)) umma_commit(&kv_empty[(base + 2 * freed_v++ + 1) % NSLOT]);
+          if (n + 2 < nt) {
+            need(base + 2 * tile_of(n + 2));
+            issue_s(n + 2);
+            if (last_of(n + 2)) umma_commit(&kv_empty[(base + 2 * freed_k++) % NSLOT]);
           }
         }
         umma_commit(q_free);
-        // Tiles that the loop did not give back: the last V tile where the sub-blocks are odd, and (a part
-        // without a row that sees it) whole tiles. They are unpacked all the same.
-        need(base + nitems - 1);
-        for (int n = nmax < 1 ? 1 : (nmax & 1) ? nmax : nmax + 1; n < nitems; ++n) umma_commit(&kv_empty[(base + n) % NSLOT]);
+        for (; 2 * freed_k < nitems || 2 * freed_v < nitems;) {
+          // In the order of the items: a tile can only be given back once it is there.
+          const bool k = freed_k <= freed_v && 2 * freed_k < nitems;
+          const int item = k ? 2 * freed_k++ : 2 * freed_v++ + 1;
+          need(base + item);
+          umma_commit(&kv_empty[(base + item) % NSLOT]);
+        }
         base += nitems;
-        done[0] += nsub[0], done[1] += nsub[1];
+        done += nt;
         ++unit;
       } while (w.next(p));
     }
@@ -404,6 +417,8 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
             u[j] = *reinterpret_cast<const uint4*>(raw + from + j * (STEP / 16) * SM::REC);
             head[j] = *reinterpret_cast<const unsigned short*>(raw + head_from + j * (STEP / 16) * SM::REC);
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&raw_empty[rs]);  // all of it is in registers: the next tile may come
           if (tail) {
 #pragma unroll
             for (int j = 0; j < ITER; ++j)
@@ -449,8 +464,6 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
           }
           fence_proxy_async();
           mbar_arrive(&kv_full[s]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&raw_empty[rs]);
         }
       }
       ++unit;
@@ -468,13 +481,13 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
     int base = 0, unit = 0;
     do {
       const int nt = subs_of(p, w, t);
-      const int local = w.i * 2 * p.tm + t * p.tm + tok;  // the row within its piece
+      const int local = w.i * 2 * p.tm + (w.narrow ? 0 : t * p.tm) + tok;  // the row within its piece
       const bool live = tok < p.tm && local < w.r.nrows;
       const int row = w.r.pos0 + local;
       float m_ref = -1e30f, l = 0.f;
       for (int n = 0; n < nt; ++n) {
         const int cnt = base + n, b = cnt & 1;
-        const int key0 = w.k0 * CQ_BN + n * CQ_SN;
+        const int key0 = w.k0 * CQ_BN + (w.narrow ? 2 * n + t : n) * CQ_SN;
         mbar_wait(&s_full[t * 2 + b], (cnt >> 1) & 1, p.status, 608);
         tc_fence_after();
         uint32_t sv[CQ_SN];
@@ -548,46 +561,60 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
         tc_fence_after();
       }
       const bool whole = w.k0 == 0 && w.k1 == w.tiles;
-      if (whole) {
-        // (Every live row of a whole unit sees a key, so its tile has sub-blocks.)
-        const float inv = 1.0f / l;
-        __half* o = p.O + ((size_t)(w.r.row0 + local) * p.H + w.g * p.hq + head) * D;
+      // A narrow unit's tiles agree on a maximum; the first takes the second's rows, which lie in the same
+      // lanes of tensor memory, with its own.
+      float mine = 1.0f, others = 0.f;
+      if (w.narrow) {
+        float* ex = (float*)(smem + SM::OFF_EX);
+        ex[t * 128 + rit] = m_ref;
+        if (t == 1) ex[256 + rit] = l;
+        tc_fence_before();
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        tc_fence_after();
+        if (t == 0) {
+          const float mo = ex[128 + rit], m2 = fmaxf(m_ref, mo);
+          mine = exp2f(m_ref - m2);
+          if (subs_of(p, w, 1) > 0) others = exp2f(mo - m2), l = l * mine + ex[256 + rit] * others;
+          m_ref = m2;
+        }
+      }
+      const bool joins = others != 0.f || l != l;  // (a NaN sum comes with NaN rows)
+      const bool stores = live && !(w.narrow && t == 1);
+      const float inv = 1.0f / l;
+      __half* o = p.O + ((size_t)(w.r.row0 + local) * p.H + w.g * p.hq + head) * D;
+      // A partial: a column at a time, a warp's rows side by side: full lines.
+      float* part = p.part + ((size_t)blockIdx.x * 2 + (w.k0 == 0 ? 1 : 0)) * 256 * (D + 2) + (w.narrow ? 0 : t * 128) + rit;
+      const bool second = w.narrow && t == 0 && subs_of(p, w, 1) > 0;
 #pragma unroll 1
-        for (int c0 = 0; nt > 0 && c0 < D; c0 += 32) {
-          uint32_t ov[32];
-          tmem_ld32(tmem_o + c0, ov);
-          tmem_ld_wait();
-          if (live) {
-            const float f = nan_at[(unit & 3) * 2 + (c0 >> 6)] <= row ? __int_as_float(0x7fc00000) : inv;
+      for (int c0 = 0; c0 < D && !(w.narrow && t == 1); c0 += 8) {
+        uint32_t ov[8], ow[8];
+        if (nt > 0) tmem_ld8(tmem_o + c0, ov);
+        if (second) tmem_ld8(tmem_o + D + c0, ow);
+        tmem_ld_wait();
+        float y[8];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 y;
-              y.x = pack_h2(__uint_as_float(ov[i]) * f, __uint_as_float(ov[i + 1]) * f);
-              y.y = pack_h2(__uint_as_float(ov[i + 2]) * f, __uint_as_float(ov[i + 3]) * f);
-              y.z = pack_h2(__uint_as_float(ov[i + 4]) * f, __uint_as_float(ov[i + 5]) * f);
-              y.w = pack_h2(__uint_as_float(ov[i + 6]) * f, __uint_as_float(ov[i + 7]) * f);
-              *reinterpret_cast<uint4*>(o + c0 + i) = y;
-            }
+        for (int i = 0; i < 8; ++i) {
+          y[i] = nt > 0 ? __uint_as_float(ov[i]) * mine : 0.f;
+          if (second && joins) y[i] = fmaf(__uint_as_float(ow[i]), others, y[i]);
+        }
+        if (stores) {
+          if (nan_at[(unit & 3) * 2 + (c0 >> 6)] <= row) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = __int_as_float(0x7fc00000);
+          }
+          if (whole) {
+            uint4 h;
+            h.x = pack_h2(y[0] * inv, y[1] * inv), h.y = pack_h2(y[2] * inv, y[3] * inv);
+            h.z = pack_h2(y[4] * inv, y[5] * inv), h.w = pack_h2(y[6] * inv, y[7] * inv);
+            *reinterpret_cast<uint4*>(o + c0) = h;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part[(size_t)(c0 + i) * 256] = y[i];
           }
         }
-      } else {
-        // A column at a time, a warp's rows side by side: full lines.
-        float* part = p.part + ((size_t)blockIdx.x * 2 + (w.k0 == 0 ? 1 : 0)) * 256 * (D + 2) + t * 128 + rit;
-#pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t ov[32];
-          if (nt > 0) {
-            tmem_ld32(tmem_o + c0, ov);
-            tmem_ld_wait();
-          }
-          if (live) {
-            const bool spoilt = nan_at[(unit & 3) * 2 + (c0 >> 6)] <= row;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              part[(size_t)(c0 + i) * 256] = nt == 0 ? 0.f : spoilt ? __int_as_float(0x7fc00000) : __uint_as_float(ov[i]);
-          }
-        }
-        if (live) part[D * 256] = m_ref, part[(D + 1) * 256] = l;
+      }
+      if (!whole) {
+        if (stores) part[D * 256] = m_ref, part[(D + 1) * 256] = l;
         if (t == 0 && rit == 0 && w.k0 == 0) {
           // Cut at this CTA's end: the next CTAs go on with it.
           int* d = p.desc + 4 * blockIdx.x;
@@ -605,7 +632,7 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
   }
   tc_fence_before();
   __syncthreads();
-  pdl_launch();
+  pdl_launch();  // only now: a dependent's CTA let in earlier would wait for this one's shared memory
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, SM::TMEM_COLS);
