@@ -90,6 +90,24 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two f32 at a time: one instruction where the softmax warps are short of issue slots.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void split2(uint64_t d, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // A piece of the step, empty if its descriptor does not lie inside it.
 struct Piece {
   int row0, nrows, pos0, blocks;
@@ -533,7 +551,8 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
           l *= f;
           if (grow) m_ref = m_new;
         }
-        float sum = 0.f;
+        uint64_t sum[2] = {0, 0};  // two pairs of partial sums
+        const uint64_t by = pair2(sc2, sc2), less = pair2(-m_ref, -m_ref);
         // Eight columns at a time, so that scores and weights are not all live at once. (All scores are in
         // registers: overwriting the buffer's first columns loses nothing.)
 #pragma unroll
@@ -541,15 +560,18 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
           uint32_t pk[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float a = ex2(fmaf(__uint_as_float(sv[16 * c + 2 * i]), sc2, -m_ref));
-            const float b2 = ex2(fmaf(__uint_as_float(sv[16 * c + 2 * i + 1]), sc2, -m_ref));
-            sum += a + b2;
+            float a, b2;
+            split2(fma2(pair2(__uint_as_float(sv[16 * c + 2 * i]), __uint_as_float(sv[16 * c + 2 * i + 1])), by, less), a, b2);
+            a = ex2(a), b2 = ex2(b2);
+            sum[i & 1] = add2(sum[i & 1], pair2(a, b2));
             pk[i] = pack_h2(a, b2);
           }
           tmem_st8(tmem_s + b * CQ_SN + 8 * c, pk);
         }
+        float s0, s1;
+        split2(add2(sum[0], sum[1]), s0, s1);
         tmem_st_wait();
-        l += sum;
+        l += s0 + s1;
         tc_fence_before();
         mbar_arrive(&p_ready[t * 2 + b]);
       }
