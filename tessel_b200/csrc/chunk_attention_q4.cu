@@ -84,6 +84,19 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                "l"((uint64_t)src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  unsigned short v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -230,7 +243,7 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = (uint64_t*)(smem + SM::OFF_BAR);
   uint64_t* q_full = bars;              // a unit's Q has landed
-  uint64_t* q_free = bars + 1;          // and its last S has been computed
+  uint64_t* q_free = bars + 1;          // and each tile's last S has been computed
   uint64_t* raw_full = bars + 2;        // [NRAW]
   uint64_t* raw_empty = bars + 6;       // [NRAW]
   uint64_t* kv_full = bars + 10;        // [NSLOT]
@@ -239,7 +252,7 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
   uint64_t* p_ready = bars + 22;        // [tile][buffer]
   uint64_t* o_done = bars + 26;         // [tile][parity]
   uint32_t* tmem_slot = (uint32_t*)(bars + 30);
-  int* nan_at = (int*)(bars + 31);      // [unit & 3][group]: least position of a spoilt V row
+  int* nan_at = (int*)(bars + 31);      // [unit & 7][group]: least position of a spoilt V row
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -257,8 +270,8 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], CQ_BM);
       mbar_init(&o_done[i], 1);
-      nan_at[i] = nan_at[4 + i] = 0x7fffffff;
     }
+    for (int i = 0; i < 16; ++i) nan_at[i] = 0x7fffffff;
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -282,16 +295,6 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
       if (lane == 0) prefetch_tmap(&mapQ);
       int item = 0, unit = 0;
       do {
-        if (lane == 0) {
-          if (unit > 0) mbar_wait(q_free, (unit - 1) & 1, p.status, 601);
-          mbar_expect_tx(q_full, 2 * SUB * p.tm * p.hq * 128);
-          const int row = w.r.row0 + w.i * 2 * p.tm;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int sub = 0; sub < SUB; ++sub)
-              tma_load_3d(smem + t * SM::Q_TILE + sub * (CQ_BM * 128), &mapQ, q_full, sub * 64, w.g * p.hq, row + (w.narrow ? 0 : t * p.tm));
-        }
         const int slim = w.r.pos0 + w.r.nrows;
         // Lane j < 8: the page of keys [128 k + 16 j, + 16). Beyond the table: page 0; behind the last key,
         // or outside the cache: zeros. Looked up a tile ahead.
@@ -299,7 +302,20 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
           const int col = k * 8 + (lane & 7);
           return k >= w.k1 || (long long)col * 16 >= slim ? -1 : col < p.MP ? p.table[(size_t)w.r.row0 * p.MP + col] : 0;
         };
+        auto load_q = [&]() {
+          if (lane == 0) {
+            mbar_expect_tx(q_full, 2 * SUB * p.tm * p.hq * 128);
+            const int row = w.r.row0 + w.i * 2 * p.tm;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int sub = 0; sub < SUB; ++sub)
+                tma_load_3d(smem + t * SM::Q_TILE + sub * (CQ_BM * 128), &mapQ, q_full, sub * 64, w.g * p.hq, row + (w.narrow ? 0 : t * p.tm));
+          }
+          __syncwarp();
+        };
         int next = page_of(w.k0);
+        if (unit == 0) load_q();
         for (int k = w.k0; k < w.k1; ++k) {
           const int page = next;
           next = page_of(k + 1);
@@ -316,6 +332,12 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
             if (lane < 8)
               bulk_load(smem + SM::OFF_RAW + s * SM::RAW + lane * SM::REC, in ? (v ? p.Vc : p.Kc) + off : g_zero_record, SM::REC,
                         &raw_full[s]);
+          }
+          // Behind the first tile's records: the unpacking warps fetch a unit's first tile before they convert
+          // the last one of the unit before, whose products free Q's place.
+          if (k == w.k0 && unit > 0) {
+            if (lane == 0) mbar_wait(q_free, (unit - 1) & 1, p.status, 601);
+            load_q();
           }
         }
         ++unit;
@@ -370,9 +392,11 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
         // A K or V tile is given back once its products are issued; those that no sub-block of this tile
         // reads (a last one's second half, keys behind its rows) at the end.
         int freed_k = 0, freed_v = 0;
+        if (nt == 0) umma_commit(q_free);
         for (int n = 0; n < 2 && n < nt; ++n) {
           need(base + 2 * tile_of(n));
           issue_s(n);
+          if (n + 1 == nt) umma_commit(q_free);
           if (last_of(n)) umma_commit(&kv_empty[(base + 2 * freed_k++) % NSLOT]);
         }
         for (int n = 0; n < nt; ++n) {
@@ -385,10 +409,10 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
           if (n + 2 < nt) {
             need(base + 2 * tile_of(n + 2));
             issue_s(n + 2);
+            if (n + 3 == nt) umma_commit(q_free);
             if (last_of(n + 2)) umma_commit(&kv_empty[(base + 2 * freed_k++) % NSLOT]);
           }
         }
-        umma_commit(q_free);
         for (; 2 * freed_k < nitems || 2 * freed_v < nitems;) {
           // In the order of the items: a tile can only be given back once it is there.
           const bool k = freed_k <= freed_v && 2 * freed_k < nitems;
@@ -418,74 +442,92 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
     for (int i = 0; i < 4; ++i)
       to[i] = (part >> 1) * (CQ_BN * 128) + key0 * 128 + (((((part & 1) * 4 + (i ^ (part & 2))) ^ (key0 & 7))) << 4);
     const __half2 R = __float2half2_rn(0.0625f);
-    int item = 0, unit = 0;
-    do {
-      const int slim = w.r.pos0 + w.r.nrows;
-      for (int k = w.k0; k < w.k1; ++k) {
-        const bool tail = (k + 1) * CQ_BN > slim;
-#pragma unroll 1
-        for (int v = 0; v < 2; ++v, ++item) {
-          const int rs = item % NRAW, s = item % NSLOT;
-          mbar_wait(&raw_full[rs], (item / NRAW) & 1, p.status, 606);
-          const unsigned char* raw = smem + SM::OFF_RAW + rs * SM::RAW;
-          uint4 u[ITER];
-          uint32_t head[ITER];
+    const uint32_t smem_at = smem_u32(smem);
+    // `fetch` takes the next item's codes and headers into registers, a step ahead of their conversion, and
+    // gives the raw slot back at once. Headers behind the last key are stale and count as zero; spoilt
+    // headers of V are noted and count as zero.
+    uint4 u[ITER], un[ITER];
+    uint32_t head[ITER], headn[ITER];
+    int fetched = 0, unit = 0, k = w.k0, v = 0;  // the item that is fetched next, its unit, tile and cache
+    bool more = true;
+    auto fetch = [&]() {
+      const int rs = fetched % NRAW;
+      mbar_wait(&raw_full[rs], (fetched / NRAW) & 1, p.status, 606);
+      const uint32_t raw = smem_at + SM::OFF_RAW + rs * SM::RAW;
 #pragma unroll
-          for (int j = 0; j < ITER; ++j) {
-            u[j] = *reinterpret_cast<const uint4*>(raw + from + j * (STEP / 16) * SM::REC);
-            head[j] = *reinterpret_cast<const unsigned short*>(raw + head_from + j * (STEP / 16) * SM::REC);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&raw_empty[rs]);  // all of it is in registers: the next tile may come
-          if (tail) {
+      for (int j = 0; j < ITER; ++j) {
+        // (Pieces 2 and 3 swap their halves here: see `to`.)
+        const uint32_t c = raw + from + j * (STEP / 16) * SM::REC;
+        const uint2 lo = lds64(c + (part & 2) * 4), hi = lds64(c + 8 - (part & 2) * 4);
+        un[j] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        headn[j] = lds16(raw + head_from + j * (STEP / 16) * SM::REC);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[rs]);
+      const int slim = w.r.pos0 + w.r.nrows, at = k * CQ_BN + key0;
+      if ((k + 1) * CQ_BN > slim) {
 #pragma unroll
-            for (int j = 0; j < ITER; ++j)
-              if (k * CQ_BN + key0 + j * STEP >= slim) head[j] = 0;  // stale behind the last key
-          }
-          if (v) {
-            bool spoilt = false;
+        for (int j = 0; j < ITER; ++j)
+          if (at + j * STEP >= slim) headn[j] = 0;
+      }
+      if (v) {
+        bool spoilt = false;
 #pragma unroll
-            for (int j = 0; j < ITER; ++j) spoilt |= (head[j] & 0x7c00u) == 0x7c00u;
-            if (spoilt) {
+        for (int j = 0; j < ITER; ++j) spoilt |= (headn[j] & 0x7c00u) == 0x7c00u;
+        if (spoilt) {
 #pragma unroll
-              for (int j = 0; j < ITER; ++j)
-                if ((head[j] & 0x7c00u) == 0x7c00u) {
-                  atomicMin(&nan_at[(unit & 3) * 2 + (part >> 1)], k * CQ_BN + key0 + j * STEP);
-                  head[j] = 0;
-                }
+          for (int j = 0; j < ITER; ++j)
+            if ((headn[j] & 0x7c00u) == 0x7c00u) {
+              atomicMin(&nan_at[(unit & 7) * 2 + (part >> 1)], at + j * STEP);
+              headn[j] = 0;
             }
-          }
-          if (item >= NSLOT) mbar_wait(&kv_empty[s], (item / NSLOT - 1) & 1, p.status, 607);
-          unsigned char* dst = smem + SM::OFF_KV + s * SM::KV_BYTES;
-#pragma unroll
-          for (int j = 0; j < ITER; ++j) {
-            const uint32_t z = head[j] & 15u;
-            // Scale, -(1024 + z) and -(64 + z), twice each.
-            const uint32_t sc = __byte_perm(head[j] & 0xfff0u, 0, 0x1010), c0 = (z | z << 16) | 0xe400e400u,
-                           c1 = (z << 4 | z << 20) | 0xd400d400u;
-            const __half2 S = *reinterpret_cast<const __half2*>(&sc), A = *reinterpret_cast<const __half2*>(&c0), B = *reinterpret_cast<const __half2*>(&c1);
-            const uint32_t word[4] = {part & 2 ? u[j].z : u[j].x, part & 2 ? u[j].w : u[j].y, part & 2 ? u[j].x : u[j].z, part & 2 ? u[j].y : u[j].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t up = word[i] >> 8;
-              uint32_t e[4] = {(word[i] & 0x000f000fu) | 0x64006400u, (word[i] & 0x00f000f0u) | 0x64006400u,
-                               (up & 0x000f000fu) | 0x64006400u, (up & 0x00f000f0u) | 0x64006400u};
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                __half2 x = *reinterpret_cast<__half2*>(&e[q]);
-                x = (q & 1) ? __hfma2(x, R, B) : __hadd2(x, A);  // code - zero point, exactly
-                x = __hmul2(x, S);
-                e[q] = *reinterpret_cast<uint32_t*>(&x);
-              }
-              *reinterpret_cast<uint4*>(dst + to[i] + j * STEP * 128) = make_uint4(e[0], e[1], e[2], e[3]);
-            }
-          }
-          fence_proxy_async();
-          mbar_arrive(&kv_full[s]);
         }
       }
-      ++unit;
-    } while (w.next(p));
+      ++fetched;
+      v ^= 1;
+      if (v == 0 && ++k == w.k1) {
+        more = w.next(p);
+        k = w.k0;
+        ++unit;
+      }
+    };
+    fetch();
+    bool have = true;
+#pragma unroll 1
+    for (int item = 0; have; ++item) {
+#pragma unroll
+      for (int j = 0; j < ITER; ++j) u[j] = un[j], head[j] = headn[j];
+      have = more;
+      if (more) fetch();
+      const int s = item % NSLOT;
+      if (item >= NSLOT) mbar_wait(&kv_empty[s], (item / NSLOT - 1) & 1, p.status, 607);
+      const uint32_t dst = smem_at + SM::OFF_KV + s * SM::KV_BYTES;
+#pragma unroll
+      for (int j = 0; j < ITER; ++j) {
+        const uint32_t z = head[j] & 15u;
+        // Scale, -(1024 + z) and -(64 + z), twice each.
+        const uint32_t sc = __byte_perm(head[j] & 0xfff0u, 0, 0x1010), c0 = (z | z << 16) | 0xe400e400u,
+                       c1 = (z << 4 | z << 20) | 0xd400d400u;
+        const __half2 S = *reinterpret_cast<const __half2*>(&sc), A = *reinterpret_cast<const __half2*>(&c0), B = *reinterpret_cast<const __half2*>(&c1);
+        const uint32_t word[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t up = word[i] >> 8;
+          uint32_t e[4] = {(word[i] & 0x000f000fu) | 0x64006400u, (word[i] & 0x00f000f0u) | 0x64006400u,
+                           (up & 0x000f000fu) | 0x64006400u, (up & 0x00f000f0u) | 0x64006400u};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            __half2 x = *reinterpret_cast<__half2*>(&e[q]);
+            x = (q & 1) ? __hfma2(x, R, B) : __hadd2(x, A);  // code - zero point, exactly
+            x = __hmul2(x, S);
+            e[q] = *reinterpret_cast<uint32_t*>(&x);
+          }
+          sts128(dst + to[i] + j * STEP * 128, e[0], e[1], e[2], e[3]);
+        }
+      }
+      fence_proxy_async();
+      mbar_arrive(&kv_full[s]);
+    }
   } else {
     // ---- softmax: one warpgroup per tile, one row (TMEM lane) per thread -------------------------------
     const int t = (warp - 8) >> 2;
@@ -620,7 +662,7 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
           if (second && joins) y[i] = fmaf(__uint_as_float(ow[i]), others, y[i]);
         }
         if (stores) {
-          if (nan_at[(unit & 3) * 2 + (c0 >> 6)] <= row) {
+          if (nan_at[(unit & 7) * 2 + (c0 >> 6)] <= row) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = __int_as_float(0x7fc00000);
           }
@@ -646,9 +688,9 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
       }
       base += nt;
       // This unit's marks are free again once all softmax threads are through with them. The unpacking
-      // warps are at most two units (four tiles) ahead of the products, so four sets are enough.
+      // warps are at most three units (six tiles) ahead of the products: eight sets are enough.
       asm volatile("bar.sync 2, 256;" ::: "memory");
-      if (threadIdx.x == 256) nan_at[(unit & 3) * 2] = nan_at[(unit & 3) * 2 + 1] = 0x7fffffff;
+      if (threadIdx.x == 256) nan_at[(unit & 7) * 2] = nan_at[(unit & 7) * 2 + 1] = 0x7fffffff;
       ++unit;
     } while (w.next(p));
   }
