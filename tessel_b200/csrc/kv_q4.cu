@@ -18,110 +18,142 @@ union H8 {
 // that kernel's bit for bit.
 //
 // HBM-bound (at decode sizes: launch latency): the QKV row is read and the Q, K, V rows are written
-// once, plus 4.25 bits per cached element. Eight lanes own the 64 elements of a group, eight
-// elements each, so the bounds are three shuffles, and a lane's codes are one 32-bit store. A lane's
-// rotation partner lies D/2 away in the same row: both halves are loaded by both lanes (from L1).
-__global__ void rope_kv_q4_kernel(const __half* __restrict__ QKV, const int* __restrict__ pos,
-                                  const int* __restrict__ slot, const float* __restrict__ Ct,
-                                  const float* __restrict__ St, __half* __restrict__ Q, unsigned char* __restrict__ Kc,
-                                  unsigned char* __restrict__ Vc, __half* __restrict__ Kd, __half* __restrict__ Vd,
-                                  int T, int H, int NPOS, Q4Shape s) {
+// once, plus 4.25 bits per cached element. A row's work is a list of items: first the groups of its KV
+// heads, eight lanes to a group's 64 elements (the bounds are three shuffles, a lane's codes one 32-bit
+// store; the rotation partner lies D/2 away in the same row, both lanes load both halves), then the
+// pairs of its query heads, eight to a thread. A thread keeps its place in the row and goes from row to
+// row, so an item is taken apart once (64-bit divisions per item took a third of the time). x / scale
+// is x times the reciprocal, corrected once by its exact remainder (Markstein): the quotient a division
+// would give, for three instructions.
+
+// Eight numbers of a group as codes and (in lane 0 of eight) the group's header.
+__device__ __forceinline__ void quantise8(const H8& x, uint32_t& word, uint32_t& head) {
+  float y[8], lo = 0.f, hi = 0.f;
+  bool odd = false;  // an infinity or a NaN
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    y[j] = __half2float(x.h[j]);
+    odd |= !(fabsf(y[j]) <= 65504.0f);
+    lo = fminf(lo, y[j]);
+    hi = fmaxf(hi, y[j]);
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    odd |= __shfl_xor_sync(0xffffffffu, (int)odd, o) != 0;
+  }
+  head = odd ? 0x7e00u : q4_scale_bits(lo, hi);
+  const float scale = q4_scale(head);
+  word = 0;
+  if (odd || scale == 0.f) return;
+  const float r = __frcp_rn(scale);
+  auto over = [&](float v) {
+    const float q = v * r;
+    return fmaf(fmaf(-q, scale, v), r, q);
+  };
+  const float zp = fminf(rintf(over(-lo)), 15.f), most = floorf(over(65504.f));
+  // rint(x / scale) kept to +-most and its sum with zp to 0..15: the bounds are integers, so they may
+  // come before the rounding. Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the
+  // low bits.
+  const float least = fmaxf(-most, -zp), largest = fminf(most, 15.f - zp);
+  const int z = (int)zp;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float q = fminf(fmaxf(over(y[j]), least), largest) + 12582912.0f;
+    word |= ((__float_as_uint(q) + z) & 15u) << (4 * ((j >> 1) + 4 * (j & 1)));
+  }
+  head |= (uint32_t)z;
+}
+
+__device__ __forceinline__ void load8(const float* __restrict__ p, bool in, float* o) {
+  const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+  *reinterpret_cast<float4*>(o) = in ? *reinterpret_cast<const float4*>(p) : z;
+  *reinterpret_cast<float4*>(o + 4) = in ? *reinterpret_cast<const float4*>(p + 4) : z;
+}
+
+constexpr int WRITE_THREADS = 128;
+
+__global__ void __launch_bounds__(WRITE_THREADS)
+    rope_kv_q4_kernel(const __half* __restrict__ QKV, const int* __restrict__ pos, const int* __restrict__ slot,
+                      const float* __restrict__ Ct, const float* __restrict__ St, __half* __restrict__ Q,
+                      unsigned char* __restrict__ Kc, unsigned char* __restrict__ Vc, __half* __restrict__ Kd,
+                      __half* __restrict__ Vd, int T, int H, int NPOS, Q4Shape s) {
   pdl_launch();
   pdl_wait();
-  const int G = s.G, D = s.D, d2 = D >> 1, W = (H + 2 * G) * D, ng = s.ng();
-  const long long kv = ((long long)T * G * ng * 8 + 31) / 32 * 32;  // whole warps: the shuffles below are warp-wide
-  const int per = D >> 4;
-  const long long total = kv + (long long)T * H * per;
-  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-    if (i < kv) {
-      const long long unit = i >> 3;
-      const int gi = (int)(unit % ng), g = (int)((unit / ng) % G), t = (int)(unit / ((long long)ng * G));
-      const int e = gi * Q4_GROUP + (int)(i & 7) * 8;  // this lane's first element
-      const bool live = t < T && e < D;
+  const int G = s.G, D = s.D, d2 = D >> 1, ng = s.ng(), per = D >> 4;
+  const size_t W = (size_t)(H + 2 * G) * D;
+  const int kv = (G * ng * 8 + 31) / 32 * 32;  // whole warps: the shuffles are warp-wide
+  const int items = kv + H * per, i = blockIdx.y * WRITE_THREADS + threadIdx.x;
+  if (i < kv) {
+    const int unit = i >> 3, g = unit / ng, gi = unit % ng;
+    const int e = gi * Q4_GROUP + (i & 7) * 8;  // this lane's first element
+    const bool mine = g < G && e < D;
+    const bool first = e < d2;
+    const int ec = first ? e : e - d2;
+    for (int t = blockIdx.x; t < T; t += gridDim.x) {
       H8 k, v;
       k.u = v.u = make_uint4(0, 0, 0, 0);
-      if (live) {
+      if (mine) {
         const int p = pos[t];
         const bool in = p >= 0 && p < NPOS;
-        const __half* src = QKV + (size_t)t * W + (size_t)(H + g) * D;
-        const bool first = e < d2;
-        const int ec = first ? e : e - d2;
+        const __half* src = QKV + t * W + (size_t)(H + g) * D;
         H8 x1, x2;
         x1.u = *reinterpret_cast<const uint4*>(src + ec);
         x2.u = *reinterpret_cast<const uint4*>(src + ec + d2);
         v.u = *reinterpret_cast<const uint4*>(src + (size_t)G * D + e);
         const size_t to = (size_t)(in ? p : 0) * d2 + ec;
+        float c[8], sn[8];
+        load8(Ct + to, in, c);
+        load8(St + to, in, sn);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float c = in ? Ct[to + j] : 0.f, sn = in ? St[to + j] : 0.f;
           const float a = __half2float(x1.h[j]), b = __half2float(x2.h[j]);
-          const float y = first ? __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, sn)) : __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, sn));
+          const float y = first ? __fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(b, sn[j])) : __fadd_rn(__fmul_rn(b, c[j]), __fmul_rn(a, sn[j]));
           k.h[j] = __float2half_rn(y);
         }
         const size_t dd = ((size_t)t * G + g) * D + e;
         *reinterpret_cast<uint4*>(Kd + dd) = k.u;
         *reinterpret_cast<uint4*>(Vd + dd) = v.u;
       }
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const H8& x = w ? v : k;
-        float lo = 0.f, hi = 0.f;
-        bool odd = false;  // an infinity or a NaN
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float y = __half2float(x.h[j]);
-          odd |= !(fabsf(y) <= 65504.0f);
-          lo = fminf(lo, y);
-          hi = fmaxf(hi, y);
-        }
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-          odd |= __shfl_xor_sync(0xffffffffu, (int)odd, o) != 0;
-        }
-        uint32_t head = odd ? 0x7e00u : q4_scale_bits(lo, hi);
-        const float scale = q4_scale(head);
-        uint32_t word = 0;
-        if (!odd && scale > 0.f) {
-          const float zp = fminf(rintf(__fdiv_rn(-lo, scale)), 15.f);
-          const float most = floorf(__fdiv_rn(65504.f, scale));
-          head |= (uint32_t)zp;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float q = fminf(fmaxf(rintf(__fdiv_rn(__half2float(x.h[j]), scale)), -most), most) + zp;
-            word |= (uint32_t)fminf(fmaxf(q, 0.f), 15.f) << (4 * ((j >> 1) + 4 * (j & 1)));
-          }
-        }
-        if (live) {
-          const int at = slot[t];
-          if (at >= 0 && at < s.NP * s.P) {
-            unsigned char* rec = (w ? Vc : Kc) + ((size_t)(at / s.P) * G + g) * s.record();
-            const int row = at % s.P;
-            *reinterpret_cast<uint32_t*>(rec + (size_t)row * d2 + (e >> 1)) = word;
-            if ((i & 7) == 0)
-              *reinterpret_cast<unsigned short*>(rec + (size_t)s.P * d2 + 2 * (row * ng + gi)) = (unsigned short)head;
-          }
+      uint32_t kw, kh, vw, vh;
+      quantise8(k, kw, kh);
+      quantise8(v, vw, vh);
+      const int at = slot[t];
+      if (mine && at >= 0 && at < s.NP * s.P) {
+        const int page = at / s.P, row = at - page * s.P;
+        const size_t rec = ((size_t)page * G + g) * s.record(), code = rec + (size_t)row * d2 + (e >> 1);
+        *reinterpret_cast<uint32_t*>(Kc + code) = kw;
+        *reinterpret_cast<uint32_t*>(Vc + code) = vw;
+        if ((i & 7) == 0) {
+          const size_t h = rec + (size_t)s.P * d2 + 2 * (row * ng + gi);
+          *reinterpret_cast<unsigned short*>(Kc + h) = (unsigned short)kh;
+          *reinterpret_cast<unsigned short*>(Vc + h) = (unsigned short)vh;
         }
       }
-    } else {
-      const long long q = i - kv;
-      const int ch = (int)(q % per), h = (int)((q / per) % H), t = (int)(q / ((long long)per * H));
+    }
+  } else if (i < items) {
+    const int h = (i - kv) / per, ch = (i - kv) % per;
+    const size_t from = (size_t)h * D + ch * 8;
+#pragma unroll 2
+    for (int t = blockIdx.x; t < T; t += gridDim.x) {
       const int p = pos[t];
       const bool in = p >= 0 && p < NPOS;
-      const __half* src = QKV + (size_t)t * W + (size_t)h * D + ch * 8;
+      const __half* src = QKV + t * W + from;
       H8 x1, x2, y1, y2;
       x1.u = *reinterpret_cast<const uint4*>(src);
       x2.u = *reinterpret_cast<const uint4*>(src + d2);
       const size_t to = (size_t)(in ? p : 0) * d2 + ch * 8;
+      float c[8], sn[8];
+      load8(Ct + to, in, c);
+      load8(St + to, in, sn);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float c = in ? Ct[to + j] : 0.f, sn = in ? St[to + j] : 0.f;
         const float a = __half2float(x1.h[j]), b = __half2float(x2.h[j]);
-        y1.h[j] = __float2half_rn(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, sn)));
-        y2.h[j] = __float2half_rn(__fadd_rn(__fmul_rn(b, c), __fmul_rn(a, sn)));
+        y1.h[j] = __float2half_rn(__fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(b, sn[j])));
+        y2.h[j] = __float2half_rn(__fadd_rn(__fmul_rn(b, c[j]), __fmul_rn(a, sn[j])));
       }
-      __half* dst = Q + ((size_t)t * H + h) * D + ch * 8;
+      __half* dst = Q + (size_t)t * H * D + from;
       *reinterpret_cast<uint4*>(dst) = y1.u;
       *reinterpret_cast<uint4*>(dst + d2) = y2.u;
     }
@@ -129,31 +161,39 @@ __global__ void rope_kv_q4_kernel(const __half* __restrict__ QKV, const int* __r
 }
 
 // Rows of the cache as f16 (exactly what they stand for); zeros for a slot outside the cache.
-// A thread reads eight elements' codes and writes them as one 16-byte store: HBM-bound.
-__global__ void kv_unpack_q4_kernel(const unsigned char* __restrict__ Kc, const unsigned char* __restrict__ Vc,
-                                    const int* __restrict__ slot, __half* __restrict__ K, __half* __restrict__ V, int N,
-                                    Q4Shape s) {
+// A thread reads eight elements' codes and writes them as one 16-byte store; it keeps its place in the
+// row and goes from row to row, four at a time in flight. HBM-bound: the f16 rows are four fifths of it.
+__global__ void __launch_bounds__(256)
+    kv_unpack_q4_kernel(const unsigned char* __restrict__ Kc, const unsigned char* __restrict__ Vc, const int* __restrict__ slot,
+                        __half* __restrict__ K, __half* __restrict__ V, int N, Q4Shape s, int rows) {
   pdl_launch();
   pdl_wait();
-  const int per = s.D >> 3, G = s.G, ng = s.ng();
-  const long long half = (long long)N * G * per, total = 2 * half;
-  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-    const bool isv = i >= half;
-    const long long j = isv ? i - half : i;
-    const int ch = (int)(j % per), g = (int)((j / per) % G), n = (int)(j / ((long long)per * G));
+  const int per = s.D >> 3, G = s.G, ng = s.ng(), half = G * per, items = 2 * half;
+  // `rows` rows side by side in a block where a row has fewer items than threads.
+  const int r = threadIdx.x / (256 / rows), i = blockIdx.y * (256 / rows) + threadIdx.x % (256 / rows);
+  if (i >= items) return;
+  const bool isv = i >= half;
+  const int j = isv ? i - half : i, g = j / per, ch = j % per;
+  const unsigned char* cache = (isv ? Vc : Kc) + (size_t)g * s.record();
+  __half* out = (isv ? V : K) + (size_t)g * s.D + ch * 8;
+  const size_t page_bytes = (size_t)G * s.record();
+  const int code = ch * 4, head = s.P * (s.D >> 1) + 2 * (ch >> 3);
+#pragma unroll 4
+  for (int n = blockIdx.x * rows + r; n < N; n += gridDim.x * rows) {
     const int at = slot[n];
-    H8 y;
-    y.u = make_uint4(0, 0, 0, 0);
-    if (at >= 0 && at < s.NP * s.P) {
-      const unsigned char* rec = (isv ? Vc : Kc) + ((size_t)(at / s.P) * G + g) * s.record();
-      const int row = at % s.P;
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + (size_t)row * (s.D >> 1) + ch * 4);
-      const uint32_t head = *reinterpret_cast<const unsigned short*>(rec + (size_t)s.P * (s.D >> 1) + 2 * (row * ng + (ch >> 3)));
-      const float sc = q4_scale(head), zp = q4_zero(head);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y.h[e] = __float2half_rn(sc * ((float)q4_code(w, e) - zp));
+    const bool in = at >= 0 && at < s.NP * s.P;
+    const int page = in ? at / s.P : 0, row = in ? at - page * s.P : 0;
+    const unsigned char* rec = cache + page * page_bytes;
+    uint32_t w = 0, hd = 0;
+    if (in) {
+      w = *reinterpret_cast<const uint32_t*>(rec + code + (size_t)row * (s.D >> 1));
+      hd = *reinterpret_cast<const unsigned short*>(rec + head + 2 * row * ng);
     }
-    *reinterpret_cast<uint4*>((isv ? V : K) + ((size_t)n * G + g) * s.D + ch * 8) = y.u;
+    const float sc = q4_scale(hd), zp = q4_zero(hd);
+    H8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y.h[e] = __float2half_rn(sc * ((float)q4_code(w, e) - zp));
+    *reinterpret_cast<uint4*>(out + (size_t)n * G * s.D) = y.u;
   }
 }
 
@@ -258,9 +298,10 @@ __global__ void page_copy_kernel(const unsigned long long* __restrict__ caches, 
   }
 }
 
-int blocks_for(long long threads, int block, int sms) {
-  const long long g = (threads + block - 1) / block, cap = (long long)sms * 16;
-  return (int)(g < 1 ? 1 : g > cap ? cap : g);
+// Blocks along the rows, when `y` blocks share a row: one per row, at most `cap` in all.
+unsigned rows_for(int rows, unsigned y, int cap) {
+  const unsigned most = (unsigned)cap / y > 0 ? (unsigned)cap / y : 1u;
+  return (unsigned)rows < most ? (unsigned)rows : most;
 }
 
 }  // namespace
@@ -326,8 +367,11 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
       if (T == 0) return 0;
       for (int i : {0, 5, 6, 7, 8, 9})
         if (!aligned_to(a[i], 16)) return bad("QKV, Q, K, V and the caches must be 16-byte aligned");
-      const long long n = ((long long)T * q.G * q.ng() * 8 + 31) / 32 * 32 + (long long)T * H * (D / 16);
-      TB_CUDA(c, launch_k(c, rope_kv_q4_kernel, dim3(blocks_for(n, 128, c->sm_count)), dim3(128), 0, 1, (const __half*)a[0],
+      const int items = (q.G * q.ng() * 8 + 31) / 32 * 32 + H * (D / 16);
+      for (int i : {3, 4})
+        if (!aligned_to(a[i], 16)) return bad("the rotation tables must be 16-byte aligned");
+      const unsigned y = (unsigned)((items + WRITE_THREADS - 1) / WRITE_THREADS);
+      TB_CUDA(c, launch_k(c, rope_kv_q4_kernel, dim3(rows_for(T, y, c->sm_count * 16), y), dim3(WRITE_THREADS), 0, 1, (const __half*)a[0],
                           (const int*)a[1], (const int*)a[2], (const float*)a[3], (const float*)a[4], (__half*)a[5],
                           (unsigned char*)a[6], (unsigned char*)a[7], (__half*)a[8], (__half*)a[9], T, H, NPOS, q));
       break;
@@ -338,10 +382,13 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
       if (N == 0) return 0;
       for (int i : {0, 1, 3, 4})
         if (!aligned_to(a[i], 16)) return bad("K, V and the caches must be 16-byte aligned");
-      const long long n = 2LL * N * q.G * (D / 8);
-      TB_CUDA(c, launch_k(c, kv_unpack_q4_kernel, dim3(blocks_for(n, 256, c->sm_count)), dim3(256), 0, 1,
+      const int items = 2 * q.G * (D / 8);
+      int rows = 1;
+      while (rows < 16 && items * rows * 2 <= 256) rows *= 2;
+      const unsigned y = (unsigned)((items + 256 / rows - 1) / (256 / rows));
+      TB_CUDA(c, launch_k(c, kv_unpack_q4_kernel, dim3(rows_for((N + rows - 1) / rows, y, c->sm_count * 8), y), dim3(256), 0, 1,
                           (const unsigned char*)a[0], (const unsigned char*)a[1], (const int*)a[2], (__half*)a[3],
-                          (__half*)a[4], N, q));
+                          (__half*)a[4], N, q, rows));
       break;
     }
     case K_DECODE_ATTENTION_Q4:

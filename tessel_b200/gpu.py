@@ -52,6 +52,20 @@ class K:
     name: str
 
 
+# ctypes array types of launch arguments, by their number (a launch costs the host a few microseconds, of which building this
+# type anew would be one).
+_RAW: Dict[int, type] = {}
+
+
+def _raw(args: Sequence[Arg]):
+    """The launch arguments as the library takes them: one 64-bit word each."""
+    n = len(args)
+    t = _RAW.get(n)
+    if t is None:
+        t = _RAW[n] = C.c_uint64 * max(n, 1)
+    return t(*[a.ptr if type(a) is Buf else _bits(a) for a in args])
+
+
 def _bits(a: Arg) -> int:
     if isinstance(a, Buf):
         return a.ptr
@@ -174,9 +188,10 @@ class Gpu:
 
     def launch(self, k: K, args: Sequence[Arg]) -> None:
         """Launches ``k`` (asynchronously)."""
-        raw = (C.c_uint64 * max(len(args), 1))(*[_bits(a) for a in args])
         self.launches += 1
-        self._check(self._l.tb200_launch(self._h, k.id, raw, len(args)))
+        rc = self._l.tb200_launch(self._h, k.id, _raw(args), len(args))
+        if rc != 0:
+            self._check(rc)
 
     # -- the per-kernel profile (src/gpu.rs:38-42, :198-222), kept by the library ------------
     @property
@@ -207,7 +222,7 @@ class Gpu:
         """Times the candidate tiles of projection kernel ``k`` on ``args`` and keeps the fastest
         (``tb200_tune``; the reference's ``Engine::mm``, src/llm/engine.rs:233-270). Returns
         ((MT, BN, splits), microseconds); whatever ``k`` writes is clobbered."""
-        raw = (C.c_uint64 * max(len(args), 1))(*[_bits(a) for a in args])
+        raw = _raw(args)
         plan = (C.c_int32 * 3)()
         us = C.c_float()
         self._check(self._l.tb200_tune(self._h, k.id, raw, len(args), plan, C.byref(us)))
