@@ -39,7 +39,7 @@ constexpr int CQ_BM = 128;       // rows of a tile
 constexpr int CQ_BN = 128;       // keys of a K / V tile
 constexpr int CQ_SN = 64;        // keys of a sub-block: the unit of S, softmax and P V
 constexpr int CQ_THREADS = 512;  // warps 0 TMA, 1-2 MMA, (3 idle), 4-7 unpack, 8-15 softmax
-constexpr int CQ_LEAST = 2;      // tiles a CTA takes at least
+constexpr int CQ_LEAST = 1;      // tiles a CTA takes at least
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.0f;
 

@@ -43,7 +43,7 @@ constexpr int DQ_THREADS = DQ_WARPS * 32;
 static_assert(DQ_WARPS % 4 == 0, "sets of one, two or four head groups divide a CTA's warps");
 constexpr int DQ_STAGES = 4;  // pairs of pages in a ring
 constexpr int DQ_CTAS = 3;    // per SM
-constexpr int DQ_LEAST = 8;   // pages a warp takes at least
+constexpr int DQ_LEAST = 2;   // pages a warp takes at least: a pair
 constexpr int DQ_SLOT = 8;    // heads of a partial
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float TWO24 = 16777216.0f;
@@ -211,7 +211,6 @@ struct Walk {
 
 template <int D, bool SIDE, int WH>
 __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const DqParams p) {
-  pdl_wait();
   using SM = DqSmem<D>;
   constexpr int NG = D / 64;
   extern __shared__ unsigned char smem_raw[];
@@ -230,8 +229,9 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       }
       fence_barrier_init();
     }
-    p.desc[4 * worker + 2] = 0;
   }
+  pdl_wait();
+  if (lane == 0) p.desc[4 * worker + 2] = 0;
   long long total, share;
   Walk w;
   w.at = find_place<WH>(p, (long long*)(smem + SM::SCAN), &total, &share);
