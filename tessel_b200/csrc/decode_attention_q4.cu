@@ -5,11 +5,11 @@
 // query q: q.k = sum over groups of s (q.u - z sum(q)); so the tensor cores multiply q by the raw
 // codes and the scale and zero point come in afterwards, once per (token, head, group). For the
 // values, o = sum_t p_t s_t (u_t - z_t) = sum_t P_t (u_t - 8) + sum_t P_t (8 - z_t) with P = p s:
-// the scale rides on the weight, the second sum is one number per (head, group). The -8 comes in as a
-// second product with a constant operand right behind the codes' own: without it the all-positive
-// products would make the accumulator hundreds of times larger than the result of a long context,
-// and the tensor cores' sums are not rounded to nearest. (A product costs less than centring the
-// operands: one instruction instead of four.)
+// the scale rides on the weight, the second sum is one number per (head, group). Without the -8 the
+// all-positive products would make the accumulator hundreds of times larger than the result of a long
+// context, and the tensor cores' sums are not rounded to nearest. It is taken out of the accumulators
+// every CENTRE pairs of pages (8 sum P, one number per column): that costs a tenth of centring the
+// operands, and between two times the accumulator grows by the weights of 256 tokens only.
 //
 // A code becomes an f16 operand by one AND: the nibble in the low bits of an f16 is the subnormal
 // u 2^-24, the next nibble 16 u 2^-24, and the tensor cores take subnormals as they are. For the
@@ -50,6 +50,8 @@ constexpr float TWO24 = 16777216.0f;
 constexpr float NO_MAX = -1e30f;    // the running maximum before the first page
 constexpr float GROW = 8.0f;        // the running maximum is renewed when a score passes it by this (log2): p <= 2^8
 constexpr float SCALE_MOST = 128.f; // and the values' running scale when s F passes this: P = p s F < 2^15 fits an f16
+
+constexpr int CENTRE = 8;            // pairs of pages between two centrings of the accumulators
 
 // What a table entry outside the cache reads as.
 __device__ __align__(128) unsigned char g_zero_record[4608];
@@ -344,11 +346,11 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
     }
     float m[2] = {NO_MAX, NO_MAX}, l[2] = {0.f, 0.f};
     float F = 67108864.0f;  // fits the smallest scale, 2^-20: the first page sets it
-    float acc[4 * NG][4], zacc[NG][2];
+    float acc[4 * NG][4], zacc[NG][2], psum[NG][2];  // psum: P since the last centring, of this lane's tokens
 #pragma unroll
     for (int i = 0; i < 4 * NG; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
-    for (int x = 0; x < NG; ++x) zacc[x][0] = zacc[x][1] = 0.f;
+    for (int x = 0; x < NG; ++x) zacc[x][0] = zacc[x][1] = psum[x][0] = psum[x][1] = 0.f;
 
     // One product's worth of tokens: a page, or (SIDE) a pair of pages at `pg`, `limit` tokens of them.
     auto tile = [&](uint32_t pg, int limit) {
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 #pragma unroll
           for (int i = 0; i < 4 * NG; ++i) acc[i][c] *= f, acc[i][2 + c] *= f;
 #pragma unroll
-          for (int x = 0; x < NG; ++x) zacc[x][c] *= f;
+          for (int x = 0; x < NG; ++x) zacc[x][c] *= f, psum[x][c] *= f;
         }
         scores(m[0], m[1]);
       }
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 #pragma unroll
           for (int i = 0; i < 4 * NG; ++i) acc[i][0] *= f, acc[i][1] *= f, acc[i][2] *= f, acc[i][3] *= f;
 #pragma unroll
-          for (int x = 0; x < NG; ++x) zacc[x][0] *= f, zacc[x][1] *= f;
+          for (int x = 0; x < NG; ++x) zacc[x][0] *= f, zacc[x][1] *= f, psum[x][0] *= f, psum[x][1] *= f;
         }
       }
       uint32_t bf[NG][2][2];  // P as the B operand: SIDE: of either page; else its hi and its lo
@@ -465,6 +467,8 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
         const float a0 = pa[0] * sa, a1 = pa[1] * sa, b0 = pb[0] * sb, b1 = pb[1] * sb;
         zacc[x][0] = fmaf(b0, cb, fmaf(a0, ca, zacc[x][0]));
         zacc[x][1] = fmaf(b1, cb, fmaf(a1, ca, zacc[x][1]));
+        psum[x][0] += a0 + b0;
+        psum[x][1] += a1 + b1;
         const uint32_t pha = pack_h2(a0, a1), phb = pack_h2(b0, b1);
         const uint32_t bh0 = movm_t(pha), bh1 = movm_t(phb);
         const uint32_t bl0 = movm_t(pack_h2(a0 - lo_f32(pha), a1 - hi_f32(pha)));
@@ -491,19 +495,31 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             // Of the word's nibbles e0 e2 e4 e6 e1 e3 e5 e7: k = 0: e0, e2 are rows gq, gq + 8; 1: e4, e6; 2: e1,
-            // e3; 3: e5, e7. Rows 8..15 always weigh 16, so one constant operand serves all.
+            // e3; 3: e5, e7. Rows 8..15 always weigh 16.
             const uint32_t v01 = (k & 2 ? hi01 : lo01) >> (8 * (k & 1)), v23 = (k & 2 ? hi23 : lo23) >> (8 * (k & 1));
             const uint32_t a_0 = v01 & 0x000f000fu, a_1 = v01 & 0x00f000f0u, a_2 = v23 & 0x000f000fu, a_3 = v23 & 0x00f000f0u;
             mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bf[x][s][0], bf[x][s][1]);
             if (!SIDE) mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bf[x][1][0], bf[x][1][1]);
           }
         }
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)  // -8 of each code
-            mma16816(acc[4 * x + k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, bf[x][s][0], bf[x][s][1]);
       }
+    };
+
+    auto centre = [&]() {
+#pragma unroll
+      for (int x = 0; x < NG; ++x)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float s = psum[x][c];
+#pragma unroll
+          for (int d = 4; d <= 16; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+          psum[x][c] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            acc[4 * x + k][c] = fmaf(s, -8.f / TWO24, acc[4 * x + k][c]);
+            acc[4 * x + k][2 + c] = fmaf(s, -128.f / TWO24, acc[4 * x + k][2 + c]);
+          }
+        }
     };
 
     for (int j = 0; j < pairs; ++j) {
@@ -513,6 +529,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       const uint32_t pg = ring_u + cs * (WH * SM::STAGE) + mine;
       tile(pg, min(limit, 32));
       if (!SIDE && limit > 16) tile(pg + WH * SM::PAGE, min(limit - 16, 16));
+      if ((j & (CENTRE - 1)) == CENTRE - 1 || j + 1 == pairs) centre();
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[cs]);
       if (++cs == DQ_STAGES) cs = 0, phase ^= 1;
