@@ -71,6 +71,8 @@ def parse():
     ap.add_argument("--fp8", action="store_true",
                     help="N = 1: the NON-PARITY FP8 mode (E4M3 projections); the line says so in `dtype` "
                          "and is not the headline number")
+    ap.add_argument("--kv4", action="store_true",
+                    help="the NON-PARITY 4-bit KV cache; the line says so in `dtype` and is not the headline number")
     ap.add_argument("--profiler-range", action="store_true",
                     help="bracket the device-resident timed region with cudaProfilerStart/Stop "
                          "(for `ncu --profile-from-start off`)")
@@ -216,6 +218,14 @@ def timed_contexts(plens, K, Wm):
     return np.asarray(plens, np.int64) + max(Wm, 3) + E2E_REPEATS * K + 3
 
 
+def kv_row_bytes(args, head_dim):
+    """Bytes of a cached token's K (or V) row of one KV head."""
+    if getattr(args, "kv4", False):
+        from tessel_b200.kv4 import row_bytes
+        return row_bytes(head_dim)
+    return 2 * head_dim
+
+
 def config_of(args, wl, world, seqs, plens):
     """The `config` object of the JSON line; both arms print the same one."""
     cfg = wl["cfg"]
@@ -226,7 +236,7 @@ def config_of(args, wl, world, seqs, plens):
     head_rows = cfg.vocab // world if vocab_parallel else cfg.vocab
     layer_w = cfg.layers * ((Hl + 2 * Gl) * D * cfg.dim + cfg.dim * Hl * D + 3 * Fl * cfg.dim)
     wbytes = (1.0 if getattr(args, "fp8", False) else 2.0) * layer_w + 2.0 * head_rows * cfg.dim
-    kvbytes = 4.0 * Gl * D * cfg.layers * ctx_mid * seqs
+    kvbytes = 2.0 * Gl * kv_row_bytes(args, D) * cfg.layers * ctx_mid * seqs
     par = f"tp{world}" + (f" ({args.tp_exchange} exchange)" if world > 1 else "")
     return ({"workload": wl["label"], "sequences": int(seqs), "parallelism": par,
              "l2": "inputs larger than L2 (weights + KV read per step: %.1f GB per GPU)" % ((wbytes + kvbytes) / 1e9),
@@ -383,7 +393,7 @@ def run_ours(args, wl):
     if args.fp8 and world > 1:
         raise SystemExit("--fp8 runs on one GPU")
     e = Engine(gpu, w, Limits(page=P, pages=pages, max_tokens=max_prompt, max_seq_pages=msp), rank=rank,
-               nranks=world, sharded=True, exchange=exchange, fp8=args.fp8)
+               nranks=world, sharded=True, exchange=exchange, fp8=args.fp8, kv4=args.kv4)
     e.fused = world > 1 and args.tp_exchange == "fused"
     s = Scheduler(e, reqs, seqs, packed=True, device_argmax=True)
 
@@ -441,7 +451,7 @@ def run_ours(args, wl):
     if ctx0 != timed_contexts(plens, K, Wm).tolist():
         # Not expected (no sequence ends inside this run); state what was measured.
         config["mean_context"] = float(np.mean(ctx0)) + K / 2.0
-        kvbytes = 4.0 * local.kv_heads * cfg.head_dim * cfg.layers * config["mean_context"] * n
+        kvbytes = 2.0 * local.kv_heads * kv_row_bytes(args, cfg.head_dim) * cfg.layers * config["mean_context"] * n
         config["l2"] = "inputs larger than L2 (weights + KV read per step: %.1f GB per GPU)" % ((wbytes + kvbytes) / 1e9)
     launches0 = gpu.kernel_launches()
     launches_before = launches0  # kernels launched before the device-resident timed region (a profiler's skip count)
@@ -477,13 +487,13 @@ def run_ours(args, wl):
     lyr = cfg.layers
     Gl, D, Hl = local.kv_heads, cfg.head_dim, local.heads
     sum_ctx = float(sum(ctx_prof)) + (args.profile_steps - 1) * n / 2.0
-    att_bytes = 4.0 * Gl * D * sum_ctx + 4.0 * n * Hl * D + 4.0 * sum(-(-c // P) for c in ctx_prof) + 4.0 * n
+    att_bytes = 2.0 * Gl * kv_row_bytes(args, D) * sum_ctx + 4.0 * n * Hl * D + 4.0 * sum(-(-c // P) for c in ctx_prof) + 4.0 * n
     roof = None
     if att:
         att_ms = att[0][3] / att[0][2]
         achieved = att_bytes / (att_ms * 1e-3) / 1e9
-        roof = {"kernel": "decode_attention", "bound": "hbm", "achieved": achieved, "peak": pk["hbm"], "unit": "GB/s",
-                "frac": achieved / pk["hbm"], "peak_kind": pk["kind"], "traffic": att_bytes * DRAM_PER_ALGORITHMIC_BYTE,
+        roof = {"kernel": "decode_attention_q4" if args.kv4 else "decode_attention", "bound": "hbm", "achieved": achieved, "peak": pk["hbm"], "unit": "GB/s",
+                "frac": achieved / pk["hbm"], "peak_kind": pk["kind"], "traffic": None if args.kv4 else att_bytes * DRAM_PER_ALGORITHMIC_BYTE,
                 "algorithmic_bytes_per_launch": att_bytes, "ms_per_launch": att_ms,
                 "share_of_step": att[0][3] / total_prof}
     # Whole-step HBM roofline (weights once, KV once per KV head), per GPU.
@@ -502,7 +512,8 @@ def run_ours(args, wl):
     line = {
         "metric": METRIC, "value": value, "unit": UNIT, "n_gpus": world, "steps": K, "warmup": max(Wm, 3),
         "ms_per_step": dev_step_ms, "higher_is_better": True, "scaling": "strong", "vs_baseline": None,
-        "dtype": "f8e4m3 projections, f16 elsewhere (non-parity mode)" if args.fp8 else "f16", "data": "synthetic",
+        "dtype": ("f8e4m3 projections, f16 elsewhere" if args.fp8 else "f16") + (", KV cache in 4 bits" if args.kv4 else "")
+                 + (" (non-parity mode)" if args.fp8 or args.kv4 else ""), "data": "synthetic",
         "config": config,
         "e2e": {"value": n * K / (e2e_ms * 1e-3), "unit": UNIT, "h2d_bytes_per_step": h2d, "d2h_bytes_per_step": 4 * n,
                 "ms_per_step": e2e_ms / K, "ms_per_step_min": min(e2e_all) / K, "ms_per_step_max": max(e2e_all) / K,

@@ -1,11 +1,11 @@
 """Single-kernel timings at the benchmark configurations' shapes, through the C ABI.
 
-    python -m tessel_b200.microbench decode [--seqs 256 --ctx-lo 512 --ctx-hi 2304 --heads 32 --kv-heads 8 --dim 128]
+    python -m tessel_b200.microbench decode [--seqs 256 --ctx-lo 512 --ctx-hi 2304 --heads 32 --kv-heads 8 --dim 128] [--kv4]
     python -m tessel_b200.microbench gemm   [--m 4096 --n 4096 --k 4096] [--kind matmul|linear|gate_up|linear_residual]
     python -m tessel_b200.microbench flash  [--heads 256 --seq 4096 --dim 128]
     python -m torch.distributed.run --nproc-per-node N -m tessel_b200.microbench exchange [--k-cols 4096]
     python -m tessel_b200.microbench qkv    [--m 256 --k 4096 --heads 32 --kv-heads 8 --dim 128]
-    python -m tessel_b200.microbench chunked [--prompt 4096 --chunk 512 --layers 32]
+    python -m tessel_b200.microbench chunked [--prompt 4096 --chunk 512 --layers 32] [--kv4]
     python -m tessel_b200.microbench flash --packed [--prompts 8 --seq 4096 --heads 32 --kv-heads 8 --dim 128]
 
 Each prints one JSON line: the mean device time per launch (CUDA events on the launching
@@ -62,7 +62,8 @@ class Timer:
         return float(np.mean(ms)), float(np.min(ms))
 
 
-def decode(gpu, torch, seqs=256, ctx_lo=512, ctx_hi=2304, heads=32, kv_heads=8, dim=128, iters=20, seed=0):
+def decode(gpu, torch, seqs=256, ctx_lo=512, ctx_hi=2304, heads=32, kv_heads=8, dim=128, iters=20, seed=0, q4=False):
+    from . import kv4
     from .gpu import Buf, F32
     P = 16
     g = np.random.default_rng(seed)
@@ -71,8 +72,16 @@ def decode(gpu, torch, seqs=256, ctx_lo=512, ctx_hi=2304, heads=32, kv_heads=8, 
     NP, MP = sum(pages) + 3, max(pages)
     gen = torch.Generator(device="cuda")
     gen.manual_seed(seed)
-    kc = torch.empty((NP, P, kv_heads, dim), dtype=torch.float16, device="cuda").normal_(generator=gen)
-    vc = torch.empty((NP, P, kv_heads, dim), dtype=torch.float16, device="cuda").normal_(generator=gen)
+    row = kv4.row_bytes(dim) if q4 else 2 * dim
+    if q4:
+        # Random codes, every group with the scale and zero point that normal numbers have: 0.3 and 8.
+        def cache():
+            c = torch.randint(0, 256, (NP, kv_heads, P * row), dtype=torch.uint8, device="cuda", generator=gen)
+            c.view(torch.int16)[..., P * dim // 4:] = 0x34C8
+            return c.view(NP, kv_heads, P, row)
+    else:
+        cache = lambda: torch.empty((NP, P, kv_heads, dim), dtype=torch.float16, device="cuda").normal_(generator=gen)
+    kc, vc = cache(), cache()
     q = torch.empty((seqs, heads, dim), dtype=torch.float16, device="cuda").normal_(generator=gen)
     o = torch.zeros_like(q)
     perm = g.permutation(NP).astype(np.int32)
@@ -82,18 +91,19 @@ def decode(gpu, torch, seqs=256, ctx_lo=512, ctx_hi=2304, heads=32, kv_heads=8, 
         table[b, :n] = perm[at:at + n]
         at += n
     tb, ln = torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda()
-    k = gpu.kernel("decode_attention", [list(q.shape), list(kc.shape), list(vc.shape), list(tb.shape), [seqs],
+    name = "decode_attention_q4" if q4 else "decode_attention"
+    k = gpu.kernel(name, [list(q.shape), list(kc.shape), list(vc.shape), list(tb.shape), [seqs],
                                         list(q.shape)])
     args = [Buf(t.data_ptr(), t.numel() * t.element_size()) for t in (q, kc, vc, tb, ln, o)] + [F32(1 / math.sqrt(dim))]
     t = Timer(gpu, torch)
     mean, best = t.run(lambda: gpu.launch(k, args), iters)
-    kv = 4.0 * kv_heads * dim * float(lens.sum())
+    kv = 2.0 * kv_heads * row * float(lens.sum())
     nbytes = kv + 4.0 * seqs * heads * dim + 4.0 * sum(pages) + 4.0 * seqs
     hbm, _, kind = _peaks()
     gbs = nbytes / (mean * 1e-3) / 1e9
-    return {"kernel": "decode_attention", "seqs": seqs, "ctx": [ctx_lo, ctx_hi], "heads": heads, "kv_heads": kv_heads,
+    return {"kernel": name, "seqs": seqs, "ctx": [ctx_lo, ctx_hi], "heads": heads, "kv_heads": kv_heads,
             "head_dim": dim, "ms": mean, "ms_min": best, "algorithmic_bytes": nbytes, "gbs": gbs, "peak_gbs": hbm,
-            "frac": gbs / hbm, "peak_kind": kind, "device_bytes": int(kc.numel() * 4)}
+            "frac": gbs / hbm, "peak_kind": kind, "device_bytes": 2 * kc.numel() * kc.element_size()}
 
 
 def gemm(gpu, torch, m=4096, n=4096, k=4096, kind="matmul", iters=20, seed=0):
@@ -358,7 +368,7 @@ def exchange(torch, tokens=256, dim=4096, k_cols=4096, calls=64, reps=10):
     return out if rank == 0 else None
 
 
-def chunked(gpu, torch, prompt=4096, chunk=512, layers=32, seed=0):
+def chunked(gpu, torch, prompt=4096, chunk=512, layers=32, seed=0, q4=False):
     """Prefill of one `prompt`-token prompt on a `layers`-layer Llama-3-8B-shaped model: in one
     step, and fed `chunk` tokens at a time through the mixed steps (chunk_attention over the paged
     cache). Wall-clock tokens/s of each, after a warm-up run of the same thing."""
@@ -373,9 +383,9 @@ def chunked(gpu, torch, prompt=4096, chunk=512, layers=32, seed=0):
     g = np.random.default_rng(seed)
     toks = g.integers(0, cfg.vocab, prompt).tolist()
     pages = -(-(prompt + 8) // 16) + 4
-    out = {"kernel": "chunked_prefill", "prompt": prompt, "chunk": chunk, "layers": layers}
+    out = {"kernel": "chunked_prefill", "kv4": q4, "prompt": prompt, "chunk": chunk, "layers": layers}
     for name, max_tokens, ch in (("one_step", prompt, 0), ("chunked", chunk, chunk)):
-        e = Engine(gpu, w, Limits(page=16, pages=pages, max_tokens=max_tokens, max_seq_pages=pages), sharded=True)
+        e = Engine(gpu, w, Limits(page=16, pages=pages, max_tokens=max_tokens, max_seq_pages=pages), sharded=True, kv4=q4)
         best = None
         for _ in range(3):
             gpu.sync()
@@ -397,6 +407,7 @@ def main():
     for name, default in (("seqs", 256), ("ctx-lo", 512), ("ctx-hi", 2304), ("heads", 32), ("kv-heads", 8),
                           ("dim", 128), ("iters", 20)):
         d.add_argument("--" + name, type=int, default=default)
+    d.add_argument("--kv4", action="store_true", help="over the 4-bit cache")
     gm = sub.add_parser("gemm")
     for name, default in (("m", 4096), ("n", 4096), ("k", 4096), ("iters", 20)):
         gm.add_argument("--" + name, type=int, default=default)
@@ -417,6 +428,7 @@ def main():
     ck = sub.add_parser("chunked")
     for name, default in (("prompt", 4096), ("chunk", 512), ("layers", 32)):
         ck.add_argument("--" + name, type=int, default=default)
+    ck.add_argument("--kv4", action="store_true", help="with the 4-bit cache")
     a = ap.parse_args()
     import torch
     if not torch.cuda.is_available():
@@ -429,13 +441,13 @@ def main():
     from .gpu import Gpu
     gpu = Gpu(0)
     if a.cmd == "decode":
-        r = decode(gpu, torch, a.seqs, a.ctx_lo, a.ctx_hi, a.heads, a.kv_heads, a.dim, a.iters)
+        r = decode(gpu, torch, a.seqs, a.ctx_lo, a.ctx_hi, a.heads, a.kv_heads, a.dim, a.iters, q4=a.kv4)
     elif a.cmd == "gemm":
         r = gemm(gpu, torch, a.m, a.n, a.k, a.kind, a.iters)
     elif a.cmd == "qkv":
         r = qkv_rope(gpu, torch, a.m, a.k, a.heads, a.kv_heads, a.dim, a.iters)
     elif a.cmd == "chunked":
-        r = chunked(gpu, torch, a.prompt, a.chunk, a.layers)
+        r = chunked(gpu, torch, a.prompt, a.chunk, a.layers, q4=a.kv4)
     elif a.packed:
         heads = 32 if a.heads == 256 else a.heads
         r = flash_packed(gpu, torch, a.prompts, a.seq, heads, a.kv_heads or heads, a.dim, a.iters)
