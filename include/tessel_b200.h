@@ -119,14 +119,15 @@ int tb200_host_free(tb200_ctx* ctx, void* ptr);
  * (hi - lo) / 15 rounded up to seven bits (below 2^-14 to a multiple of 2^-20),
  * zero point = rint(-lo / scale), code = rint(x / scale) + zero point, kept to
  * 0..15; a group that holds an infinity or a NaN stands for NaN throughout. D is a
- * multiple of 16, at most 256, P even; Q, K, V, O and the caches 16-byte aligned.
+ * multiple of 16, at most 256, P even; QKV, Q, K, V, O, C, S, meta and the caches
+ * 16-byte aligned.
  * rope_kv_q4 takes rope_kv's arrays with such caches (QKV, pos, slot, C, S, Q, Kc,
  * Vc, K, V; the slots of a call that lie inside the cache must differ from one
  * another). kv_unpack_q4 (Kc, Vc, slot[N], K f16[N,G,D], V f16[N,G,D]) reads rows
  * back; a slot outside the cache gives zeros. decode_attention_q4 and
  * chunk_attention_q4 are decode_attention and chunk_attention over such caches;
  * positions beyond the block table lie on page 0, a page outside the cache reads
- * as zeros.
+ * as zeros; the pieces of a call must not share rows.
  *
  * page_copy (caches i64[A], pairs i32[N,2], then the i32 scalars n, NP and bytes):
  * for each of the A caches, whose device addresses (16-byte aligned) `caches` holds,

@@ -360,6 +360,7 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
   const auto& s = op.shapes;
   auto bad = [&](const char* why) { return fail(c, op.name + ": " + why); };
   Q4Shape q;
+  TB_CUDA(c, cudaSetDevice(c->device));  // the caller's thread may have another device current
   switch (op.kind) {
     case K_ROPE_KV_Q4: {
       const int T = (int)s[0][0], H = (int)s[5][1], D = (int)s[5][2], NPOS = (int)s[3][0];
@@ -397,6 +398,7 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
       q4_shape(op, 1, D, &q);
       for (int i : {0, 1, 2, 5})
         if (!aligned_to(a[i], 16)) return bad("Q, O and the caches must be 16-byte aligned");
+      if (op.kind == K_CHUNK_ATTENTION_Q4 && !aligned_to(a[4], 16)) return bad("meta must be 16-byte aligned");
       const unsigned blocks = (unsigned)(((long long)T * H + 3) / 4);
       if (T == 0) return 0;
       if (op.p0 && op.kind == K_DECODE_ATTENTION_Q4) return launch_decode_q4(c, op, a, q);

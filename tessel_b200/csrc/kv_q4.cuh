@@ -41,7 +41,8 @@ inline const char* q4_shape(const Op& op, int i, int64_t D, Q4Shape* out) {
   if (s[3] != D / 2 + 2 * ((D + Q4_GROUP - 1) / Q4_GROUP)) return "a cache row has D/2 + 2*ceil(D/64) bytes";
   if (s[2] < 2 || s[2] % 2 || s[2] > 1024) return "the page size must be even, at most 1024";
   if (s[1] < 1) return "at least one kv head";
-  if (s[0] * s[1] > 0x7fffffffLL || s[0] * s[2] > 0x7fffffffLL) return "the cache has too many pages";
+  if (s[0] > 0x7fffffffLL / s[1] || s[0] > 0x7fffffffLL / s[2]) return "the cache has too many pages";
+  if (s[1] > 0x7fffffffLL / (s[2] * s[3])) return "a page is too large";
   *out = Q4Shape{(int)s[0], (int)s[1], (int)s[2], (int)D};
   return nullptr;
 }

@@ -117,10 +117,11 @@ def attend(q, kc, vc, row, first, scale, f16_weights=False):
     R, H, D = q.shape
     NP, G, P, _ = kc.shape
     n = first + R
-    col = np.arange(n) // P
+    col = np.arange(-(-n // P))
     page = np.where(col < len(row), row[np.minimum(col, len(row) - 1)], 0)
-    inside = ((page >= 0) & (page < NP))[:, None, None]
-    fetch = lambda c: np.where(inside, kv4.read(c, D)[np.where(inside[:, 0, 0], page, 0), np.arange(n) % P], 0).astype(f64)
+    inside = (page >= 0) & (page < NP)
+    fetch = lambda c: np.where(inside[:, None, None, None], kv4.read(c[np.where(inside, page, 0)], D),
+                               0).reshape(-1, G, D)[:n].astype(f64)
     k, v = fetch(kc), fetch(vc)
     heads = (kv4.parts(kc, D)[1] & np.uint16(0xFFF0)).view(h).astype(f64).max()
     out, tol = np.zeros((R, H, D)), np.zeros((R, H, 1))
@@ -308,6 +309,85 @@ def test_attention_agrees_between_a_decode_row_and_a_piece_of_one_row(gpu):
         near(b[r][None], want, tol)
 
 
+def spoil(rng, cache, table, rows, D, share):
+    """Marks a share of the groups of the tokens that `rows` (table row, tokens) name as NaN."""
+    head = kv4.parts(cache, D)[1]
+    for b, n in rows:
+        for t in np.nonzero(rng.random(n) < share)[0]:
+            head[table[b, t // 16], rng.integers(0, head.shape[1]), t % 16, rng.integers(0, head.shape[3])] = 0x7E00
+
+
+@pytest.mark.parametrize("H,G,D", [(32, 8, 128), (8, 8, 128), (16, 2, 64), (3, 1, 128), (10, 5, 64)])
+def test_decode_attention_q4_many_short_rows(gpu, H, G, D):
+    """Shares that run over many sequences and heads: units that lie whole in a share, cut ones, empty rows between them, and
+    spoilt values that must stay in their head, group and sequence."""
+    r = np.random.default_rng(D + H)
+    lens = np.where(r.random(300) < 0.2, 0, r.integers(1, 90, 300)).astype(i32)
+    q, kc, vc, table = attention_case(21 + H, 300, H, G, D, 16, [-(-n // 16) for n in lens])
+    spoil(r, vc, table, [(b, lens[b]) for b in range(0, 300, 3)], D, 0.02)
+    spoil(r, kc, table, [(b, lens[b]) for b in range(1, 300, 7)], D, 0.01)
+    clean = without_nans(kc, D), without_nans(vc, D)
+    got = decode_q4(gpu, q, kc, vc, table, lens, D ** -0.5)
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert np.isnan(got[b].astype(f)).all()
+            continue
+        check_with_nans(got[b][None], q[b][None], (kc, vc), clean, table[b], n - 1, D ** -0.5, False)
+
+
+def without_nans(c, D):
+    """`c` with its spoilt groups as zeros."""
+    c = c.copy()
+    head = kv4.parts(c, D)[1]
+    head[head == 0x7E00] = 0
+    return c
+
+
+def check_with_nans(got, q, caches, clean, row, first, scale, f16_weights):
+    """As `near`, where spoilt keys and values make NaNs: exactly the NaNs of the definition, and the rest near it."""
+    D, (kc, vc) = q.shape[2], caches
+    want, tol = attend(q, clean[0], clean[1], row, first, scale, f16_weights)
+    bad = np.zeros(got.shape, bool)
+    G = kc.shape[1]
+    for i in range(q.shape[0]):
+        t = np.arange(first + i + 1)
+        for g in range(G):
+            heads = slice(g * (q.shape[1] // G), (g + 1) * (q.shape[1] // G))
+            if (kv4.parts(kc, D)[1][row[t // 16], g, t % 16] == 0x7E00).any():
+                bad[i, heads] = True
+            spoilt = (kv4.parts(vc, D)[1][row[t // 16], g, t % 16] == 0x7E00).any(0)
+            bad[i, heads] |= np.repeat(spoilt, 64)
+    assert np.array_equal(np.isnan(got.astype(f)), bad)
+    ok = ~bad
+    assert (np.abs(got.astype(f64) - want)[ok] <= np.broadcast_to(tol, want.shape)[ok]).all()
+
+
+@pytest.mark.parametrize("H,G,D,most", [(32, 8, 128, 6), (8, 8, 128, 150), (16, 2, 64, 70), (128, 1, 64, 3), (100, 1, 128, 4)])
+def test_chunk_attention_q4_many_pieces(gpu, H, G, D, most):
+    """Shares that run over many pieces, heads and blocks: blocks of one tile's rows and of two, of a single key and of several
+    tiles, cut or whole, with spoilt values that later rows see and earlier ones do not."""
+    r = np.random.default_rng(D + H)
+    pieces, row = [], 0
+    for _ in range(70):
+        n = int(r.integers(1, most + 1))
+        pieces.append((row, n, int(r.choice([0, 1, 30, 63, 64, 127, 128, 300]))))
+        row += n + int(r.integers(0, 2))
+    T = row + 2
+    pages = [0] * T
+    for row0, n, pos in pieces:
+        pages[row0] = -(-(pos + n) // 16)
+    q, kc, vc, table = attention_case(T + H, T, H, G, D, 16, pages)
+    spoil(r, vc, table, [(a, n + p) for a, n, p in pieces[::2]], D, 0.01)
+    spoil(r, kc, table, [(a, n + p) for a, n, p in pieces[1::5]], D, 0.005)
+    got = chunk_q4(gpu, q, kc, vc, table, [(a, n, p, 0) for a, n, p in pieces], D ** -0.5)
+    clean = without_nans(kc, D), without_nans(vc, D)
+    rest = np.ones(T, bool)
+    for row0, n, pos in pieces:
+        check_with_nans(got[row0:row0 + n], q[row0:row0 + n], (kc, vc), clean, table[row0], pos, D ** -0.5, True)
+        rest[row0:row0 + n] = False
+    assert (got[rest] == 3).all()
+
+
 # ---- pages -------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("A,NP,words,n", [(1, 2, 1, 1), (2, 9, 34, 4), (64, 40, 2048, 13), (7, 300, 68, 149), (3, 8, 5000, 3)])
 def test_page_copy(gpu, A, NP, words, n):
@@ -378,6 +458,12 @@ def test_refusals(gpu):
         gpu.launch(k, [gpu.wrap(b.ptr + 8, 64), b, b, b, b, b, F32(1.0)])
     with pytest.raises(GpuError, match="arguments"):
         gpu.launch(k, [b, b])
+    k = gpu.kernel("chunk_attention_q4", dec()[:4] + [[2, 4], [3, 4, 128]])
+    with pytest.raises(GpuError, match="meta must be"):
+        gpu.launch(k, [b, b, b, b, gpu.wrap(b.ptr + 4, 64), b, F32(1.0)])
+    with pytest.raises(GpuError, match="too large"):
+        gpu.kernel("decode_attention_q4", [[1, 1 << 21, 128], kc(NP=1, G=1 << 21), kc(NP=1, G=1 << 21), [1, 1], [1],
+                                                                     [1, 1 << 21, 128]])
     gpu.free(b)
 
 
