@@ -133,7 +133,7 @@ int tb200_host_free(tb200_ctx* ctx, void* ptr);
  * for each of the A caches, whose device addresses (16-byte aligned) `caches` holds,
  * and each of the first n pairs (src, dst): page dst = page src, pages of `bytes`
  * bytes (a multiple of 16) in caches of NP pages. A pair with a page outside the
- * cache is skipped. All pairs run at once: a page may be the source of several
+ * cache is skipped, and so is a cache whose address is 0 or not aligned. All pairs run at once: a page may be the source of several
  * pairs, but a page that one pair writes must not be in any other pair.
  *
  * The reference's `meta` and `warps` arguments have no equivalent: tile shapes
@@ -209,7 +209,9 @@ int tb200_launch_count(tb200_ctx* ctx, uint64_t* out);
 
 /* No counterpart in the reference: run on a stream the host already owns
  * (a `cudaStream_t`), so that other libraries' work can be ordered with the
- * kernels. NULL restores the context's own stream. */
+ * kernels. NULL restores the context's own stream. A kernel handle's workspace is
+ * its context's: what was launched on the old stream must have finished, or be
+ * waited for by the new one, before the same kernels are launched there. */
 int tb200_set_stream(tb200_ctx* ctx, void* cuda_stream);
 /* The stream in use, as a `cudaStream_t`. */
 int tb200_get_stream(tb200_ctx* ctx, void** cuda_stream);

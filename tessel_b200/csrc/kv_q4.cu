@@ -291,9 +291,10 @@ __global__ void page_copy_kernel(const unsigned long long* __restrict__ caches, 
   for (long long j = blockIdx.x; j < jobs; j += gridDim.x) {
     const int pair = (int)(j / A), a = (int)(j % A);
     const int src = pairs[2 * pair], dst = pairs[2 * pair + 1];
-    if (src < 0 || src >= NP || dst < 0 || dst >= NP || src == dst) continue;
-    const uint4* from = (const uint4*)caches[a] + (size_t)src * words;
-    uint4* to = (uint4*)caches[a] + (size_t)dst * words;
+    const unsigned long long cache = caches[a];
+    if (src < 0 || src >= NP || dst < 0 || dst >= NP || src == dst || cache == 0 || cache % 16) continue;
+    const uint4* from = (const uint4*)cache + (size_t)src * words;
+    uint4* to = (uint4*)cache + (size_t)dst * words;
     for (int i = threadIdx.x; i < words; i += blockDim.x) to[i] = from[i];
   }
 }
@@ -311,7 +312,7 @@ int make_kv_q4(Ctx* c, Op& op) {
   auto bad = [&](const char* why) { return fail(c, op.name + ": " + why); };
   for (const auto& a : s)
     for (int64_t d : a)
-      if (d > 0x7fffffffLL) return bad("a dimension is beyond 2^31 - 1");
+      if (d > 0x40000000LL) return bad("a dimension is beyond 2^30");  // (loops step past the last row in 32 bits)
   Q4Shape q;
   const char* why = nullptr;
   switch (op.kind) {
@@ -371,6 +372,7 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
       const int items = (q.G * q.ng() * 8 + 31) / 32 * 32 + H * (D / 16);
       for (int i : {3, 4})
         if (!aligned_to(a[i], 16)) return bad("the rotation tables must be 16-byte aligned");
+      if (!aligned_to(a[1] | a[2], 4)) return bad("pos and slot must be 4-byte aligned");
       const unsigned y = (unsigned)((items + WRITE_THREADS - 1) / WRITE_THREADS);
       TB_CUDA(c, launch_k(c, rope_kv_q4_kernel, dim3(rows_for(T, y, c->sm_count * 16), y), dim3(WRITE_THREADS), 0, 1, (const __half*)a[0],
                           (const int*)a[1], (const int*)a[2], (const float*)a[3], (const float*)a[4], (__half*)a[5],
@@ -383,6 +385,7 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
       if (N == 0) return 0;
       for (int i : {0, 1, 3, 4})
         if (!aligned_to(a[i], 16)) return bad("K, V and the caches must be 16-byte aligned");
+      if (!aligned_to(a[2], 4)) return bad("slot must be 4-byte aligned");
       const int items = 2 * q.G * (D / 8);
       int rows = 1;
       while (rows < 16 && items * rows * 2 <= 256) rows *= 2;
@@ -399,6 +402,7 @@ int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a) {
       for (int i : {0, 1, 2, 5})
         if (!aligned_to(a[i], 16)) return bad("Q, O and the caches must be 16-byte aligned");
       if (op.kind == K_CHUNK_ATTENTION_Q4 && !aligned_to(a[4], 16)) return bad("meta must be 16-byte aligned");
+      if (!aligned_to(a[3] | a[4], 4)) return bad("the block table and lens must be 4-byte aligned");
       const unsigned blocks = (unsigned)(((long long)T * H + 3) / 4);
       if (T == 0) return 0;
       if (op.p0 && op.kind == K_DECODE_ATTENTION_Q4) return launch_decode_q4(c, op, a, q);

@@ -335,6 +335,31 @@ def test_decode_attention_q4_many_short_rows(gpu, H, G, D):
         check_with_nans(got[b][None], q[b][None], (kc, vc), clean, table[b], n - 1, D ** -0.5, False)
 
 
+@pytest.mark.parametrize("H,G,D,P", [(32, 8, 128, 16), (8, 1, 128, 16), (16, 2, 64, 16), (4, 2, 32, 8)])
+def test_attention_q4_keeps_bad_queries_to_themselves(gpu, H, G, D, P):
+    """A query with an infinity or a NaN has NaN as its result (an infinite score less an infinite maximum), and no other
+    head, row or sequence changes: bit for bit the result without it."""
+    lens = np.array([1, 40, 700, 33, 300], i32)
+    q, kc, vc, table = attention_case(31, 5, H, G, D, P, [-(-int(n) // P) for n in lens])
+    dirty = q.copy()
+    dirty[1, 1, 3], dirty[2, H - 1, D - 1], dirty[4, 0, 0] = np.inf, -np.inf, np.nan
+    bad = [(1, 1), (2, H - 1), (4, 0)]
+    clean, got = (decode_q4(gpu, x, kc, vc, table, lens, D ** -0.5) for x in (q, dirty))
+    keep = np.ones((5, H), bool)
+    for b, hh in bad:
+        assert np.isnan(got[b, hh].astype(f)).all()
+        keep[b, hh] = False
+    assert np.array_equal(got[keep].view(np.uint16), clean[keep].view(np.uint16))
+    pieces = [(0, 2, 50, 0), (2, 3, 200, 0)]
+    q, kc, vc, table = attention_case(32, 5, H, G, D, P, [-(-60 // P), 0, -(-210 // P), 0, 0])
+    dirty = q.copy()
+    dirty[1, 1, 3], dirty[2, H - 1, D - 1], dirty[4, 0, 0] = np.inf, -np.inf, np.nan
+    clean, got = (chunk_q4(gpu, x, kc, vc, table, pieces, D ** -0.5) for x in (q, dirty))
+    for b, hh in bad:
+        assert np.isnan(got[b, hh].astype(f)).all()
+    assert np.array_equal(got[keep].view(np.uint16), clean[keep].view(np.uint16))
+
+
 def without_nans(c, D):
     """`c` with its spoilt groups as zeros."""
     c = c.copy()
@@ -416,6 +441,80 @@ def test_page_copy(gpu, A, NP, words, n):
         gpu.free(b)
 
 
+def test_page_copy_skips_caches_without_an_aligned_address(gpu):
+    r = np.random.default_rng(9)
+    c = r.integers(0, 256, (4, 64)).astype(u8)
+    b = gpu.tensor(c)
+    bases = gpu.tensor(np.array([0, b.ptr + 8, b.ptr], np.uint64))
+    pairs = gpu.tensor(np.array([[0, 2], [1, 3]], i32))
+    gpu.launch(gpu.kernel("page_copy", [[3], [2, 2]]), [bases, pairs, I32(2), I32(4), I32(64)])
+    gpu.sync()
+    assert np.array_equal(gpu.fetch(b, u8, c.shape), c[[0, 1, 0, 1]])
+    for x in (b, bases, pairs):
+        gpu.free(x)
+
+
+@pytest.mark.parametrize("H,G,D,P", [(32, 8, 128, 16), (8, 4, 256, 16)])
+def test_caches_beyond_four_gigabytes(gpu, H, G, D, P):
+    """The last pages of a cache of more than 2^32 bytes: every kernel gives what it gives in a small cache, to the bit."""
+    small, pages = 70, [40, 20]
+    lens = np.array([39 * P + 3, 20 * P], i32)
+    q, kc, vc, table = attention_case(3, 2, H, G, D, P, pages)
+    kc, vc = (np.concatenate([c, np.zeros((small - len(c),) + c.shape[1:], u8)]) for c in (kc, vc))
+    size = kc[0].nbytes
+    NP = (2 ** 32 + 2 ** 28) // size
+    off = NP - small
+    big = [gpu.alloc(NP * size) for _ in range(2)]
+    for b, c in zip(big, (kc, vc)):
+        gpu.write(b, off * size, c)
+    shape = [NP] + list(kc.shape[1:])
+    T, W = 5, (H + 2 * G) * D
+    r = np.random.default_rng(4)
+    qkv, pos = r.standard_normal((T, W)).astype(h), np.arange(T, dtype=i32)
+    slot = (r.permutation(2 * P)[:T] + (small - 2) * P).astype(i32)
+    cs = [r.standard_normal((T, D // 2)).astype(f) for _ in range(2)]
+    meta = np.array([[0, 1, 38 * P, 0], [1, 1, 5, 0]], i32)
+    res = []
+    for big_one in (False, True):
+        o = off if big_one else 0
+        caches = big if big_one else [gpu.tensor(kc), gpu.tensor(vc)]
+        cshape = shape if big_one else list(kc.shape)
+        t = lambda a: gpu.tensor(a)
+        out = []
+        def call(name, arrays, shapes, scalars, outs):
+            bufs = [a if not isinstance(a, np.ndarray) else t(a) for a in arrays]
+            gpu.launch(gpu.kernel(name, shapes), bufs + scalars)
+            gpu.sync()
+            out.extend(gpu.fetch(bufs[i], h, shapes[i]).view(np.uint16) for i in outs)
+            for a, b in zip(arrays, bufs):
+                if isinstance(a, np.ndarray):
+                    gpu.free(b)
+        at = (table + o).astype(i32)
+        qs = [2, H, D]
+        call("decode_attention_q4", [q, *caches, at, lens, np.zeros(qs, h)], [qs, cshape, cshape, at.shape, [2], qs],
+             [F32(D ** -0.5)], [5])
+        call("chunk_attention_q4", [q, *caches, at, meta, np.zeros(qs, h)], [qs, cshape, cshape, at.shape, [2, 4], qs],
+             [F32(D ** -0.5)], [5])
+        kv = [T, G, D]
+        call("rope_kv_q4", [qkv, pos, (slot + o * P).astype(i32), *cs, np.zeros((T, H, D), h), *caches, np.zeros(kv, h), np.zeros(kv, h)],
+             [qkv.shape, [T], [T], cs[0].shape, cs[1].shape, [T, H, D], cshape, cshape, kv, kv], [], [5, 8, 9])
+        call("kv_unpack_q4", [*caches, (slot + o * P).astype(i32), np.zeros(kv, h), np.zeros(kv, h)], [cshape, cshape, [T], kv, kv],
+             [], [3, 4])
+        bases, pair = t(np.array([b.ptr for b in caches], np.uint64)), t(np.array([[o + small - 1, o + 1], [o, o + 2]], i32))
+        gpu.launch(gpu.kernel("page_copy", [[2], [2, 2]]), [bases, pair, I32(2), I32(cshape[0]), I32(size)])
+        gpu.sync()
+        for b in caches:
+            raw = np.empty(kc.shape, u8)
+            gpu.read(b, o * size, raw)
+            out.append(raw)
+            gpu.free(b)
+        for b in (bases, pair):
+            gpu.free(b)
+        res.append(out)
+    for a, b in zip(*res):
+        assert np.array_equal(a, b)
+
+
 # ---- refusals ----------------------------------------------------------------------------------------------------------
 def test_refusals(gpu):
     kc = lambda NP=4, G=2, P=16, D=128: [NP, G, P, kv4.row_bytes(D)]
@@ -432,6 +531,7 @@ def test_refusals(gpu):
         ([[3, 4, 24]] + [kc(D=24)] * 2 + [[3, 5], [3], [3, 4, 24]], "head_dim"),
         ([[3, 4, 272]] + [kc(D=272)] * 2 + [[3, 5], [3], [3, 4, 272]], "head_dim"),
         (dec(NP=1 << 30), "too many pages"),
+        (dec(NP=(1 << 30) + 1), "beyond"),
     ]:
         with pytest.raises(GpuError, match=what):
             gpu.kernel("decode_attention_q4", shapes)
@@ -459,6 +559,8 @@ def test_refusals(gpu):
     with pytest.raises(GpuError, match="arguments"):
         gpu.launch(k, [b, b])
     k = gpu.kernel("chunk_attention_q4", dec()[:4] + [[2, 4], [3, 4, 128]])
+    with pytest.raises(GpuError, match="4-byte"):
+        gpu.launch(k, [b, b, b, gpu.wrap(b.ptr + 2, 64), b, b, F32(1.0)])
     with pytest.raises(GpuError, match="meta must be"):
         gpu.launch(k, [b, b, b, b, gpu.wrap(b.ptr + 4, 64), b, F32(1.0)])
     with pytest.raises(GpuError, match="too large"):
