@@ -65,12 +65,37 @@ int launch_chunk_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q);
 __device__ __forceinline__ float q4_scale(uint32_t head) { return __half2float(__ushort_as_half((unsigned short)(head & 0xfff0u))); }
 __device__ __forceinline__ float q4_zero(uint32_t head) { return (float)(head & 15u); }
 
+// Two f32 at a time: one instruction where issue slots are short. (Each half rounds as the plain operation does.)
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void split2(uint64_t d, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // Element `i` (0..7) of a word of codes.
 __device__ __forceinline__ int q4_code(uint32_t word, int i) { return (word >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15; }
 
-// The header for a group with these bounds (lo <= 0 <= hi).
-__device__ __forceinline__ uint32_t q4_scale_bits(float lo, float hi) {
-  const float r = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+// The header for a group whose bounds (lo <= 0 <= hi) are this far apart. The division is a product with the rounded
+// reciprocal, corrected by its exact remainder: with a correctly rounded reciprocal that is the rounded quotient
+// (Markstein; `range` is 0 or at least 2^-24, nothing underflows).
+__device__ __forceinline__ uint32_t q4_scale_bits(float range) {
+  const float q = range * (1.0f / 15.0f), r = fmaf(fmaf(-q, 15.0f, range), 1.0f / 15.0f, q);
   float s;
   if (r < 6.103515625e-05f)  // 2^-14: f16 subnormals, four low bits of 2^-24 units kept free
     s = ceilf(r * 1048576.0f) * 9.5367431640625e-07f;
