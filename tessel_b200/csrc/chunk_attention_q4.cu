@@ -28,7 +28,7 @@
 //
 // Bound: the tensor cores by operations; measured, the softmax warps (1700 of 1870 cycles per 64 keys, 1024 of them
 // the exponentials' unit) with the unpacking in the same issue slots. 2048 rows at position 30000, 32/8 heads, D 128:
-// 890 us, 1166 TFLOP/s; 8 pieces of 1-8 rows at 700-6000: 41 us, where unpacking a tile (1650 cycles) sets the pace.
+// 890 us, 1166 TFLOP/s; 8 pieces of 1-8 rows at 700-6000: 39 us, where unpacking a tile (1650 cycles) sets the pace.
 //
 // NaN. A weight of zero times a NaN is a NaN, so a spoilt V row would reach rows that do not see it.
 // The unpacking warps store zeros for it instead and note the least such position of each 64-column
@@ -703,20 +703,34 @@ __global__ void __launch_bounds__(256) chunk_q4_join_kernel(const CqParams p) {
   const int rr = threadIdx.x, t = rr >> 7, tok = (rr & 127) / p.hq, head = (rr & 127) % p.hq;
   const int local = i * 2 * p.tm + t * p.tm + tok;
   if (tok >= p.tm || local >= r.nrows) return;
+  constexpr int U = 3;  // partials in flight
   float m = -1e30f, l = 0.f, a[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) a[e] = 0.f;
-#pragma unroll 2
-  for (int k = 0; k < pieces; ++k) {
-    const float* s = p.part + ((size_t)(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * 256 * (D + 2) + rr;
-    float v[8];
+  for (int k0 = 0; k0 < pieces; k0 += U) {
+    float v[U][8], mk[U], lk[U], m2 = m;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = s[(size_t)(blockIdx.y * 8 + e) * 256];
-    const float mk = s[D * 256], lk = s[(D + 1) * 256];
-    const float m2 = fmaxf(m, mk), f = ex2(m - m2), fk = ex2(mk - m2);
-    l = fmaf(l, f, lk * fk);
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u;
+      const bool in = k < pieces;
+      const float* s = p.part + ((size_t)(blockIdx.x + (in ? k : 0)) * 2 + (k == 0 ? 1 : 0)) * 256 * (D + 2) + rr;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = fmaf(a[e], f, v[e] * fk);
+      for (int e = 0; e < 8; ++e) v[u][e] = in ? s[(size_t)(blockIdx.y * 8 + e) * 256] : 0.f;
+      mk[u] = in ? s[D * 256] : -1e30f, lk[u] = in ? s[(D + 1) * 256] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) m2 = fmaxf(m2, mk[u]);
+    const float f = ex2(m - m2);
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] *= f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float fk = ex2(mk[u] - m2);
+      l = fmaf(lk[u], fk, l);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] = fmaf(v[u][e], fk, a[e]);
+    }
     m = m2;
   }
   uint4 y;

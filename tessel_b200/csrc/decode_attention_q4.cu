@@ -603,12 +603,12 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 
 // Joins the partials of the unit that is cut at the end of a warp's share, if there is one: that
 // warp's second slot and the first slots of the warps that follow (`wh` apart). One block per share:
-// HP heads, 8 / HP warps each, four partials in flight per warp (a long context has dozens).
+// HP heads, 8 / HP warps each, U partials in flight per warp (a long context has dozens).
 template <int D, int HP>
 __global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p, int wh) {
   pdl_wait();
   pdl_launch();
-  constexpr int NSP = 8 / HP, V = D / 32;
+  constexpr int NSP = 8 / HP, V = D / 32, U = 4;
   __shared__ float other[8][D + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hh = warp % HP, sp = warp / HP;
   const int* d = p.desc + 4 * blockIdx.x;
@@ -618,10 +618,10 @@ __global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p, i
   float m = NO_MAX, l = 0.f, a[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) a[k] = 0.f;
-  for (int i0 = sp; i0 < pieces && hh < nh; i0 += 4 * NSP) {
-    float mi[4], li[4], ai[4][V];
+  for (int i0 = sp; i0 < pieces && hh < nh; i0 += U * NSP) {
+    float mi[U], li[U], ai[U][V];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int i = i0 + u * NSP;
       const bool in = i < pieces;
       const float* s = p.part + ((size_t)(blockIdx.x + (in ? i : 0) * wh) * 2 + (in && i > 0 ? 0 : 1)) * DQ_SLOT * (D + 2);
@@ -630,12 +630,15 @@ __global__ void __launch_bounds__(256) decode_q4_join_kernel(const DqParams p, i
 #pragma unroll
       for (int k = 0; k < V; ++k) ai[u][k] = in ? s[hh * D + lane + 32 * k] : 0.f;
     }
-    const float m2 = fmaxf(fmaxf(m, fmaxf(mi[0], mi[1])), fmaxf(mi[2], mi[3])), f = ex2(m - m2);
+    float m2 = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) m2 = fmaxf(m2, mi[u]);
+    const float f = ex2(m - m2);
     l *= f;
 #pragma unroll
     for (int k = 0; k < V; ++k) a[k] *= f;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       const float fu = ex2(mi[u] - m2);
       l = fmaf(li[u], fu, l);
 #pragma unroll
