@@ -360,6 +360,50 @@ def test_attention_q4_keeps_bad_queries_to_themselves(gpu, H, G, D, P):
     assert np.array_equal(got[keep].view(np.uint16), clean[keep].view(np.uint16))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [1, 2, 3, 4])
+def test_attention_q4_of_every_head_layout(gpu, D, G):
+    """One to seventeen query heads per KV head on one to four KV heads: every way warps and tiles are laid out, with
+    sequences that end in a page, at its end, and are cut among many shares."""
+    for hq in (1, 2, 3, 4, 5, 7, 8, 9, 16, 17):
+        lens = np.array([1, 16, 0, 333, 1500], i32)
+        q, kc, vc, table = attention_case(100 * D + 10 * G + hq, 5, hq * G, G, D, 16, [-(-int(n) // 16) for n in lens])
+        got = decode_q4(gpu, q, kc, vc, table, lens, D ** -0.5)
+        for b, n in enumerate(lens):
+            if n:
+                near(got[b][None], *attend(q[b][None], kc, vc, table[b], n - 1, D ** -0.5))
+            else:
+                assert np.isnan(got[b].astype(f)).all()
+        pieces = [(0, 1, 200), (2, 40, 100), (43, 2, 1400)]
+        q, kc, vc, table = attention_case(100 * D + 10 * G + hq, 46, hq * G, G, D, 16, [13] + [0] + [9] + [0] * 40 + [88, 0, 0])
+        got = chunk_q4(gpu, q, kc, vc, table, [(a, n, at, 0) for a, n, at in pieces], D ** -0.5)
+        for a, n, at in pieces:
+            near(got[a:a + n], *attend(q[a:a + n], kc, vc, table[a], at, D ** -0.5, True))
+        assert (got[[1, 42, 45]] == 3).all()
+
+
+@pytest.mark.parametrize("H,G,D,P", [(32, 8, 128, 16), (8, 1, 64, 16), (4, 2, 32, 8)])
+def test_attention_q4_values_of_very_different_sizes(gpu, H, G, D, P):
+    """Values between 2^-20 and the largest f16, groups of zeros among them, growing and shrinking along the sequence:
+    the error stays a rounding of the largest."""
+    r = np.random.default_rng(5)
+    lens = np.array([700, 33, 1, 260], i32)
+    q, kc, vc, table = attention_case(77, 4, H, G, D, P, [-(-int(n) // P) for n in lens])
+    code, head = kv4.parts(vc, D)
+    size = 2.0 ** np.sort(r.uniform(-20, 13, (vc.shape[0], 1, P, 1)), axis=2)
+    size[::2] = size[::2, :, ::-1]                       # up along one page, down along the next
+    x = (r.standard_normal((vc.shape[0], G, P, D)) * size).clip(-65504, 65504)
+    x[r.random((vc.shape[0], G, P)) < 0.1] = 0
+    cd, hd = kv4.quantize(x.astype(h))
+    code[:], head[:] = kv4.pack(cd), hd
+    got = decode_q4(gpu, q, kc, vc, table, lens, D ** -0.5)
+    for b, n in enumerate(lens):
+        near(got[b][None], *attend(q[b][None], kc, vc, table[b], n - 1, D ** -0.5))
+    got = chunk_q4(gpu, q, kc, vc, table, [(0, 1, 600, 0), (1, 1, 32, 0), (3, 1, 255, 0)], D ** -0.5)
+    for b, n in ((0, 600), (1, 32), (3, 255)):
+        near(got[b][None], *attend(q[b][None], kc, vc, table[b], n, D ** -0.5, True))
+
+
 def without_nans(c, D):
     """`c` with its spoilt groups as zeros."""
     c = c.copy()
