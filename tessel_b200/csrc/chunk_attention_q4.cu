@@ -761,20 +761,13 @@ int launch_chunk_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
   CqParams p;
   p.T = (int)s[0][0], p.H = (int)s[0][1], p.G = q.G, p.hq = p.H / p.G, p.tm = CQ_BM / p.hq;
   p.C = (int)s[4][0], p.NP = q.NP, p.MP = (int)s[3][1];
-  const uint64_t key[4] = {a[0], 0, 0, 0};
-  const MapEntry* hit = op.find_maps(key);
-  if (!hit) {
-    // Q [T, H, D]: one box = the group's heads of tm tokens, 64 columns.
-    const uint64_t dims[3] = {(uint64_t)q.D, (uint64_t)p.H, (uint64_t)p.T};
-    const uint64_t strides[2] = {(uint64_t)q.D * 2, (uint64_t)p.H * q.D * 2};
-    const uint32_t box[3] = {64, (uint32_t)p.hq, (uint32_t)p.tm};
-    CUtensorMap m;
-    if (make_tensor_map(c, &m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (const void*)a[0], dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
-      return 1;
-    MapEntry* e = op.fresh_maps(key);
-    e->m[0] = m;
-    hit = e;
-  }
+  // Q [T, H, D]: one box = the group's heads of tm tokens, 64 columns.
+  const uint64_t dims[3] = {(uint64_t)q.D, (uint64_t)p.H, (uint64_t)p.T};
+  const uint64_t strides[2] = {(uint64_t)q.D * 2, (uint64_t)p.H * q.D * 2};
+  const uint32_t box[3] = {64, (uint32_t)p.hq, (uint32_t)p.tm};
+  CUtensorMap map;
+  if (make_tensor_map(c, &map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (const void*)a[0], dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+    return 1;
   p.Kc = (const unsigned char*)a[1];
   p.Vc = (const unsigned char*)a[2];
   p.table = (const int*)a[3];
@@ -787,10 +780,10 @@ int launch_chunk_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
   p.desc = (int*)(p.part + (size_t)op.p1 * 2 * 256 * (q.D + 2));
   const dim3 grid(op.p1), join(op.p1, q.D / 8);
   if (q.D == 128) {
-    TB_CUDA(c, launch_k(c, chunk_q4_kernel<128>, grid, dim3(CQ_THREADS), CqSmem<128>::TOTAL, 1, hit->m[0], p));
+    TB_CUDA(c, launch_k(c, chunk_q4_kernel<128>, grid, dim3(CQ_THREADS), CqSmem<128>::TOTAL, 1, map, p));
     TB_CUDA(c, launch_k(c, chunk_q4_join_kernel<128>, join, dim3(256), 0, 1, p));
   } else {
-    TB_CUDA(c, launch_k(c, chunk_q4_kernel<64>, grid, dim3(CQ_THREADS), CqSmem<64>::TOTAL, 1, hit->m[0], p));
+    TB_CUDA(c, launch_k(c, chunk_q4_kernel<64>, grid, dim3(CQ_THREADS), CqSmem<64>::TOTAL, 1, map, p));
     TB_CUDA(c, launch_k(c, chunk_q4_join_kernel<64>, join, dim3(256), 0, 1, p));
   }
   c->launches += 2;
