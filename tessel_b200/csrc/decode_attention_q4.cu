@@ -434,7 +434,8 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 #pragma unroll
           for (int x = 0; x < NG; ++x) zacc[x][c] *= f, psum[x][c] *= f;
         }
-        scores(m[0], m[1]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) xa[c] -= m[c], xb[c] -= m[c];  // (0 for the largest: a single token's weight is 1, its result its value)
       }
       const float pa[2] = {ex2(xa[0]), ex2(xa[1])}, pb[2] = {ex2(xb[0]), ex2(xb[1])};
       l[0] += pa[0] + pb[0];

@@ -404,6 +404,14 @@ def test_attention_q4_values_of_very_different_sizes(gpu, H, G, D, P):
         near(got[b][None], *attend(q[b][None], kc, vc, table[b], n, D ** -0.5, True))
 
 
+@pytest.mark.parametrize("H,G,D,P", [(32, 8, 128, 16), (16, 2, 64, 16), (5, 5, 128, 16), (4, 2, 32, 8)])
+def test_attention_q4_of_a_single_token_is_its_value(gpu, H, G, D, P):
+    q, kc, vc, table = attention_case(8, 40, H, G, D, P, [1] * 40)
+    want = np.repeat(kv4.read(vc, D)[table[:, 0], 0], H // G, axis=1)
+    assert np.array_equal(decode_q4(gpu, q, kc, vc, table, [1] * 40, D ** -0.5), want)
+    assert np.array_equal(chunk_q4(gpu, q, kc, vc, table, [(b, 1, 0, 0) for b in range(40)], D ** -0.5), want)
+
+
 def without_nans(c, D):
     """`c` with its spoilt groups as zeros."""
     c = c.copy()
