@@ -192,6 +192,7 @@ class Engine:
         self.cache_shape = [lim.pages, cfg.kv_heads, lim.page, row] if kv4 else [lim.pages, lim.page, cfg.kv_heads, cfg.head_dim]
         self.page_bytes = lim.page * cfg.kv_heads * row
         self._page_tables: Optional[tuple] = None
+        self._tables_stale = False  # pages were copied since the block tables on the device were sent
         self.layers: List[_DevLayer] = []
         self.q8: List[Dict[str, Buf]] = []
         for l in w.layers:
@@ -355,6 +356,7 @@ class Engine:
                 g.write_async(self.meta, 0, mt)
             g.write_async(self.table, 0, tb)
             g.write_async(self.lens, 0, ln)
+            self._tables_stale = False
         # Rows whose logits are wanted.
         bw = padded(len(want)) if len(want) else None
         if bw is not None:
@@ -421,8 +423,11 @@ class Engine:
         small kernel turns the picks into the next step's token, position, cache slot and length
         on the device, and the recorded step is replayed. Returns int32 ``[steps, n]``: the token
         picked by each of these steps. The sequences' block tables must already hold the pages
-        their new tokens land in (the scheduler reserves them up front)."""
-        from .gpu import I32
+        their new tokens land in (the scheduler reserves them up front). It goes on from the block
+        tables that step sent, so after ``copy_pages`` (``Scheduler.compact``) it is refused
+        (ValueError) until a decode step has sent new ones."""
+        if self._tables_stale:
+            raise ValueError("pages were copied or moved since the last decode step: run one with the new block tables first")
         t = padded(n)
         if steps < 1:
             return np.empty((0, n), np.int32)
@@ -692,10 +697,13 @@ class Engine:
         """Copies cache pages, in every layer's K and V: ``pairs`` of (source, destination). Every copy reads its
         source as it was before the call, so pages may be moved along (5 -> 2 with 9 -> 5): copies that have to wait
         for others go into launches of their own, usually there is one. A page outside the cache, a page written twice
-        and pages exchanged in a circle are refused (ValueError) before anything is copied."""
+        and pages exchanged in a circle are refused (ValueError) before anything is copied.
+        Block tables are the caller's: the ones a step sent stay as they are, and ``decode_resident``, which would go on
+        from them, is refused until the next decode step."""
         waves = kv4_format.copy_waves(pairs, self.lim.pages)
         if not waves:
             return
+        self._tables_stale = True
         g = self.gpu
         if self._page_tables is None:
             caches = np.array([b.ptr for l in self.layers for b in (l.kc, l.vc)], np.uint64)

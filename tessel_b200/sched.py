@@ -133,7 +133,8 @@ class Scheduler:
 
     def compact(self) -> int:
         """Moves the pages in use to the lowest page numbers (``Engine.copy_pages``) and points the block tables at them;
-        returns how many are in use. Call it between steps: pages from that number on hold nothing any more."""
+        returns how many are in use. Call it between steps: pages from that number on hold nothing any more. (Between this
+        scheduler's steps: where pages moved, ``Engine.decode_resident`` is refused until the next decode step.)"""
         seqs = self.running + self.feeding
         live = set(self.prefix_pages)
         for s in seqs:

@@ -166,6 +166,15 @@ class EmuGpu:
         elif name == "argmax_rows":
             x = A(0, f)
             A(1, i)[:] = [oracle.argmax(r) for r in x]
+        elif name == "decode_advance":
+            # picked, tok, pos, slot, lens, table, hist, then n, the page size and the history's row.
+            n, page, table = sc(7), sc(8), A(5, i)
+            picked, pos = A(0, i)[:n], A(2, i)[:n] + 1
+            at = pos // page
+            inside = at < table.shape[1]
+            A(1, i)[:n] = A(6, i)[sc(9), :n] = picked
+            A(2, i)[:n], A(4, i)[:n] = pos, pos + 1
+            A(3, i)[:n] = np.where(inside, table[np.arange(n), np.where(inside, at, 0)] * page + pos % page, 0x7fffffff)
         elif name == "argmax_partial":
             x, pr = A(0, f), A(1, f)
             rank, base = sc(2), sc(3)

@@ -193,3 +193,46 @@ def test_a_prefix_that_does_not_fit_is_refused():
         generate_with(tiny()(), [Request([1], 2)], 1, True, prefix=[1] * 129)
     with pytest.raises(ValueError, match="does not fit"):
         generate_with(tiny()(), [Request([1] * 100, 2)], 1, True, prefix=[1] * 40)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_resident_decoding_does_not_go_on_from_pages_that_moved(quantised):
+    from tessel_b200.sched import Request, Scheduler
+    reqs = [Request([1 + (i * 7 + j) % 250 for j in range(p)], n) for i, (p, n) in enumerate([(30, 3), (8, 20), (11, 21), (14, 22)])]
+
+    def run(compact):
+        s = Scheduler(tiny()(kv4=quantised), reqs, 4, device_argmax=True)
+        moved = False
+        while not s.done():
+            rows = [q.id for q in s.running]
+            if s.step() != "decode" or [q.id for q in s.running] != rows:
+                continue                             # (a sequence has ended: the step's rows are not the running ones)
+            before = [q.pages for q in s.running]
+            if compact:
+                s.compact()
+            n = len(s.running)
+            if [q.pages for q in s.running] != before:
+                moved = True
+                with pytest.raises(ValueError, match="moved"):
+                    s.e.decode_resident(n, 2)
+            elif min(q.left for q in s.running) > 2:
+                for picks in s.e.decode_resident(n, 2):
+                    s.absorb(picks)
+        return [o.tokens for o in s.finish()[0]], moved
+
+    (got, moved), (want, _) = run(True), run(False)
+    assert moved, "no page was moved: the test shows nothing"
+    assert got == want
+
+
+def test_resident_decoding_after_a_copy_of_pages_needs_a_step_with_its_tables():
+    from tessel_b200.engine import Decode, Prefill
+    e = tiny()()
+    e.step_greedy([3, 1, 4], [0, 1, 2], [24, 25, 26], Prefill(), [2])
+    e.step_greedy([7], [3], [27], Decode([[3]], [4]), [0])
+    e.copy_pages([(3, 5)])
+    with pytest.raises(ValueError, match="moved"):
+        e.decode_resident(1, 1)
+    e.copy_pages([])                                  # copies nothing
+    e.step_greedy([8], [4], [44], Decode([[5]], [5]), [0])
+    assert e.decode_resident(1, 2).shape == (2, 1)
