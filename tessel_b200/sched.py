@@ -153,13 +153,16 @@ class Scheduler:
 
     def _admit(self) -> List[Tuple[int, List[int]]]:
         """As many waiting prompts as the step's token budget, the batch and the free cache pages
-        allow. Pages for a whole sequence are reserved up front."""
+        allow. Pages for a whole sequence are reserved up front. A request that can never fit is
+        refused (ValueError) when it is the first to be admitted; behind others it waits for the next
+        call, so that those are not lost with it."""
         e, p = self.e, self.e.lim.page
         admit: List[Tuple[int, List[int]]] = []
         tokens = 0
         if self.prefix and not self.prefix_pages and self.waiting:
             self._feed_prefix()
         base, shared = len(self.prefix), len(self.prefix) // p
+        first = len(self.waiting)
         forks = []  # (the prefix's last, partly filled page, a sequence's copy of it)
         while self.waiting:
             rid = self.waiting[0]
@@ -167,6 +170,8 @@ class Scheduler:
             need = -(-(base + len(r.prompt) + r.max_new) // p) - shared
             long = len(r.prompt) > e.lim.max_tokens or base > 0
             if len(r.prompt) == 0 or (long and not self.chunk) or shared + need > e.lim.max_seq_pages:
+                if len(self.waiting) < first:
+                    break
                 raise ValueError(f"request {rid}: prompt of {len(r.prompt)} tokens does not fit")
             busy = len(self.running) + len(self.feeding) + len(admit)
             if long:

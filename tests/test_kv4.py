@@ -236,3 +236,30 @@ def test_resident_decoding_after_a_copy_of_pages_needs_a_step_with_its_tables():
     e.copy_pages([])                                  # copies nothing
     e.step_greedy([8], [4], [44], Decode([[5]], [5]), [0])
     assert e.decode_resident(1, 2).shape == (2, 1)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("n", [8, 13, 0])
+def test_a_request_that_does_not_fit_leaves_those_before_it_whole(n, quantised):
+    from tessel_b200.sched import Request, Scheduler
+    prefix = [1 + (i * 37 % 250) for i in range(n)]
+    good = [Request([5, 6, 7], 6), Request([9] * 12, 6)]
+    bad = Request([3] * 20, 16 * 8)
+
+    def run(reqs, drop):
+        s = Scheduler(tiny()(kv4=quantised), reqs, 4, prefix=prefix)
+        s.e.gpu.write(s.e.layers[0].kc, 0, np.full(s.e.page_bytes * s.e.lim.pages, 0x55, np.uint8))   # no page is zeros to begin with
+        refused = 0
+        while not s.done():
+            try:
+                s.step()
+            except ValueError:
+                refused += 1
+                assert s.waiting.popleft() == drop   # the caller drops the request at the head and goes on
+        assert refused == (drop is not None)
+        assert sorted(s.free + s.prefix_pages) == list(range(s.e.lim.pages)), "pages were lost"
+        return [o.tokens for o in s.finish()[0]]
+
+    want = run(good, None)
+    assert run([good[0], bad, good[1]], 1)[::2] == want
+    assert run(good + [bad], 2)[:2] == want
