@@ -53,7 +53,7 @@ __device__ __forceinline__ void quantise8(const uint4& x, uint32_t& word, uint32
   for (int o = 1; o < 8; o <<= 1) m = max_h2(m, __shfl_xor_sync(0xffffffffu, m, o));
   const bool odd = (m & 0x7c00u) == 0x7c00u || (m & 0x7c000000u) == 0x7c000000u;  // an infinity or a NaN
   const float2 bound = __half22float2(*reinterpret_cast<const __half2*>(&m));
-  head = odd ? 0x7e00u : q4_scale_bits(bound.x + bound.y);
+  head = odd ? 0x7e00u : q4_scale_bits(bound.x, bound.y);
   const float scale = q4_scale(head);
   word = 0;
   if (odd || scale == 0.f) return;

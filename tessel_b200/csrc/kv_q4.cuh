@@ -91,16 +91,20 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // Element `i` (0..7) of a word of codes.
 __device__ __forceinline__ int q4_code(uint32_t word, int i) { return (word >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15; }
 
-// The header for a group whose bounds (lo <= 0 <= hi) are this far apart. The division is a product with the rounded
-// reciprocal, corrected by its exact remainder: with a correctly rounded reciprocal that is the rounded quotient
-// (Markstein; `range` is 0 or at least 2^-24, nothing underflows).
-__device__ __forceinline__ uint32_t q4_scale_bits(float range) {
+// The header for a group whose bounds are -down <= 0 <= up. The division is a product with the rounded reciprocal,
+// corrected by its exact remainder: with a correctly rounded reciprocal that is the rounded quotient (Markstein; `range`
+// is 0 or at least 2^-24, nothing underflows). `rest` is what the sum lost (two f16 numbers may need 41 bits): it matters
+// only where the sum is 15 steps to the bit and the range is larger, which takes the next step.
+__device__ __forceinline__ uint32_t q4_scale_bits(float up, float down) {
+  const float range = up + down, part = range - up, rest = (up - (range - part)) + (down - part);
   const float q = range * (1.0f / 15.0f), r = fmaf(fmaf(-q, 15.0f, range), 1.0f / 15.0f, q);
   float s;
-  if (r < 6.103515625e-05f)  // 2^-14: f16 subnormals, four low bits of 2^-24 units kept free
+  if (r < 6.103515625e-05f)  // 2^-14: f16 subnormals, four low bits of 2^-24 units kept free (and the sum is exact)
     s = ceilf(r * 1048576.0f) * 9.5367431640625e-07f;
-  else
+  else {
     s = __uint_as_float((__float_as_uint(r) + 0x1ffffu) & ~0x1ffffu);
+    if (fmaf(-15.0f, s, range) + rest > 0.f) s = __uint_as_float(__float_as_uint(s) + 0x20000u);
+  }
   return __half_as_ushort(__float2half_rn(s));  // exact: seven bits, at most 2 * 65504 / 15 rounded up
 }
 

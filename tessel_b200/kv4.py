@@ -44,7 +44,7 @@ def quantize(x: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
         bad = ~np.isfinite(g).all(-1)
         g = np.where(bad[..., None], np.float32(0), g)
         lo, hi = np.minimum(g.min(-1), np.float32(0)), np.maximum(g.max(-1), np.float32(0))
-        r = (hi - lo) / np.float32(15)
+        r = (hi.astype(np.float64) - lo.astype(np.float64)) / 15  # (two f16 numbers may need 41 bits side by side)
         step = np.exp2(np.maximum(np.frexp(r)[1], -13) - 7.0)
         scale = (np.ceil(r / step) * step).astype(np.float32)
         div = np.where(scale > 0, scale, np.float32(1))

@@ -89,6 +89,28 @@ def test_rope_kv_q4_writes_the_host_quantisers_bytes(gpu, T, H, G, D, P, NP):
         assert np.array_equal(got, want, equal_nan=True)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_rope_kv_q4_rounds_the_scale_up_from_the_exact_range(gpu, D):
+    from test_kv4 import far_bounds
+    x = far_bounds()
+    T, G, H = len(x), 2, 1
+    x = np.stack([x, -x], 1)                                   # [T, G, 64]
+    kv = np.concatenate([x, x[::-1]], -1)[..., :D]
+    qkv = np.zeros((T, (H + 2 * G) * D), h)
+    qkv[:, H * D:(H + G) * D], qkv[:, (H + G) * D:] = kv.reshape(T, -1), kv[::-1].reshape(T, -1)
+    c, s = np.ones((1, D // 2), f), np.zeros((1, D // 2), f)   # the rotation leaves K as it is
+    NP = -(-T // 16)
+    z = lambda n: np.zeros((T, n, D), h)
+    kc, vc = new_cache(NP, G, 16, D), new_cache(NP, G, 16, D)
+    slot = np.arange(T, dtype=i32)
+    kq, vq, k, v = run(gpu, "rope_kv_q4", [qkv, np.zeros(T, i32), slot, c, s, z(H), kc, vc, z(G), z(G)], [6, 7, 8, 9])
+    assert np.array_equal(k, kv) and np.array_equal(v, kv[::-1])
+    for got, rows in ((kq, kv), (vq, kv[::-1])):
+        want = new_cache(NP, G, 16, D)
+        kv4.write(want, slot, rows)
+        assert got.tobytes() == want.tobytes()
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------
 def attention_case(seed, B, H, G, D, P, pages):
     """Queries, caches of quantised rows in scrambled pages, and a block table of `pages[b]` pages for row b."""

@@ -263,3 +263,29 @@ def test_a_request_that_does_not_fit_leaves_those_before_it_whole(n, quantised):
     want = run(good, None)
     assert run([good[0], bad, good[1]], 1)[::2] == want
     assert run(good + [bad], 2)[:2] == want
+
+
+def far_bounds():
+    """Groups of 64 whose two bounds need more than 24 bits side by side: an end of the range 15 * 2^e or 15 * scale next to a
+    much smaller number of the other sign; and, for comparison, the end alone. The ranges, and the rows f16 [n, 64]."""
+    rows = []
+    for e in (-8, 0, 5, 11):
+        for top in (15 * 2.0 ** e, 15 * 127 / 64 * 2.0 ** e, 15 * 65 / 64 * 2.0 ** e):
+            for small in (0.0, 2.0 ** -24, 2.0 ** -23, 3 * 2.0 ** -24, 2.0 ** -14, 2.0 ** -10):
+                for sign in (1, -1):
+                    rows.append([sign * top, -sign * small] + [sign * top * i / 70 for i in range(62)])
+    x = np.asarray(rows, f16)
+    assert (x[:, 0].astype(f64) == [r[0] for r in rows]).all()   # both ends are f16 numbers
+    return x
+
+
+def test_the_scale_is_rounded_up_from_the_exact_range():
+    from fractions import Fraction as F
+    x = far_bounds()
+    codes, heads = kv4.quantize(x)
+    got = (heads[:, 0] & np.uint16(0xFFF0)).view(f16).astype(f64)
+    for row, scale in zip(x.astype(f64), got):
+        r = (F(max(row.max(), 0)) - F(min(row.min(), 0))) / 15
+        step = F(2) ** (int(np.frexp(float(r))[1]) - 7)
+        want = -(-r // step) * step
+        assert F(scale) == want, (row[:2], scale, float(want))
