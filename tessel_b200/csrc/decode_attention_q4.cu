@@ -14,8 +14,14 @@
 // A code becomes an f16 operand by one AND: the nibble in the low bits of an f16 is the subnormal
 // u 2^-24, the next nibble 16 u 2^-24, and the tensor cores take subnormals as they are. For the
 // keys the 16 is taken out of q (q / 16 is exact, or off by 2^-25 where |q| < 2^-10), for the
-// values out of the accumulators. P is split in two f16 (hi + lo), so the second product keeps f32
-// accuracy.
+// values out of the accumulators.
+//
+// P is split in two f16 (hi + lo): 22 bits down to 2^-2, below that the multiples of 2^-24. A power of
+// two F for each head and group follows the largest P, up and down: not the largest scale, nor another
+// head's or group's, for a token of great weight and no value, or a group of far larger values, must not
+// push the other P off that grid. The largest P of a head and group is about 2^10 or more, so what the
+// grid cuts off a weight is less than 2^-34 of it. All sums take the P that is left on the grid: a weight
+// that falls off it is left out, where a sum of u without it and one of z with it would leave -z.
 //
 // The eight columns of a product. With four or fewer query heads per KV head (SIDE) q stands in them
 // twice and a warp takes two pages at a time: columns 0..3 of the first page's scores and 4..7 of the
@@ -51,7 +57,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float TWO24 = 16777216.0f;
 constexpr float NO_MAX = -1e30f;    // the running maximum before the first page
 constexpr float GROW = 8.0f;        // the running maximum is renewed when a score passes it by this (log2): p <= 2^8
-constexpr float SCALE_MOST = 128.f; // and the values' running scale when s F passes this: P = p s F < 2^15 fits an f16
+constexpr float P_MOST = 32768.f;   // and F when a P = p s F reaches this, to put the largest at 2^P_AIM or more
+constexpr int P_AIM = 10;
+constexpr int F_MOST = 100;         // log2 of the largest F, and the first: s F p < 2^(14 + 100 + 8) is finite
 
 constexpr int CENTRE = 8;            // pairs of pages between two centrings of the accumulators
 
@@ -347,12 +355,15 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       }
     }
     float m[2] = {NO_MAX, NO_MAX}, l[2] = {0.f, 0.f};
-    float F = 67108864.0f;  // fits the smallest scale, 2^-20: the first page sets it
+    float F[NG][2];  // of the columns' heads: the first page with a value sets it
     float acc[4 * NG][4], zacc[NG][2], psum[NG][2];  // psum: P since the last centring, of this lane's tokens
 #pragma unroll
     for (int i = 0; i < 4 * NG; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
-    for (int x = 0; x < NG; ++x) zacc[x][0] = zacc[x][1] = psum[x][0] = psum[x][1] = 0.f;
+    for (int x = 0; x < NG; ++x) {
+      zacc[x][0] = zacc[x][1] = psum[x][0] = psum[x][1] = 0.f;
+      F[x][0] = F[x][1] = __uint_as_float((127u + F_MOST) << 23);
+    }
 
     // One product's worth of tokens: a page, or (SIDE) a pair of pages at `pg`, `limit` tokens of them.
     auto tile = [&](uint32_t pg, int limit) {
@@ -426,13 +437,19 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 #pragma unroll
           for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           mx = fmaxf(m[c], mx);
-          const float f = ex2(m[c] - mx);
+          const float by = m[c] - mx;
           m[c] = mx;
-          l[c] *= f;
+          l[c] *= ex2(by);
+          // The sums lose a factor 2^by; F takes its whole powers of two, as far as it may.
 #pragma unroll
-          for (int i = 0; i < 4 * NG; ++i) acc[i][c] *= f, acc[i][2 + c] *= f;
+          for (int x = 0; x < NG; ++x) {
+            const int up = min((int)fminf(rintf(-by), 300.f), 127 + F_MOST - (int)(__float_as_uint(F[x][c]) >> 23));
+            const float f = ex2(by + (float)up);
+            F[x][c] = __uint_as_float(__float_as_uint(F[x][c]) + ((uint32_t)up << 23));
 #pragma unroll
-          for (int x = 0; x < NG; ++x) zacc[x][c] *= f, psum[x][c] *= f;
+            for (int i = 0; i < 4; ++i) acc[4 * x + i][c] *= f, acc[4 * x + i][2 + c] *= f;
+            zacc[x][c] *= f, psum[x][c] *= f;
+          }
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) xa[c] -= m[c], xb[c] -= m[c];  // (0 for the largest: a single token's weight is 1, its result its value)
@@ -440,34 +457,54 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       const float pa[2] = {ex2(xa[0]), ex2(xa[1])}, pb[2] = {ex2(xb[0]), ex2(xb[1])};
       l[0] += pa[0] + pb[0];
       l[1] += pa[1] + pb[1];
-      // P = p s F: F, a power of two, keeps it in f16's range whatever the values' size. It follows the
-      // largest scale seen.
-      float va[NG], vbs[NG];
+      // P = p s F of the two tokens, columns in pairs.
+      uint64_t wa[NG], wb[NG];
       {
         const uint32_t sa = hva & 0xfff0fff0u, sb = hvb & 0xfff0fff0u;
-        va[0] = lo_f32(sa), vbs[0] = lo_f32(sb);
-        if (NG == 2) va[NG - 1] = hi_f32(sa), vbs[NG - 1] = hi_f32(sb);
-        float most = fmaxf(va[0], vbs[0]);
-        if (NG == 2) most = fmaxf(most, fmaxf(va[NG - 1], vbs[NG - 1]));
-        if (__any_sync(0xffffffffu, most * F >= SCALE_MOST)) {
+        const uint64_t p2a = pair2(pa[0], pa[1]), p2b = pair2(pb[0], pb[1]);
+        float most = 0.f;
 #pragma unroll
-          for (int d = 1; d <= 16; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-          const float to = __uint_as_float((260u - (__float_as_uint(most) >> 23)) << 23);  // the largest scale in [64, 128)
-          const float f = to / F;
-          F = to;
+        for (int x = 0; x < NG; ++x) {
+          const float va = x ? hi_f32(sa) : lo_f32(sa), vb = x ? hi_f32(sb) : lo_f32(sb);
+          const uint64_t f2 = pair2(F[x][0], F[x][1]);
+          wa[x] = mul2(p2a, mul2(pair2(va, va), f2)), wb[x] = mul2(p2b, mul2(pair2(vb, vb), f2));
+          float a0, a1, b0, b1;
+          split2(wa[x], a0, a1);
+          split2(wb[x], b0, b1);
+          most = fmaxf(most, fmaxf(fmaxf(a0, a1), fmaxf(b0, b1)));
+        }
+        if (__any_sync(0xffffffffu, most >= P_MOST)) {
 #pragma unroll
-          for (int i = 0; i < 4 * NG; ++i) acc[i][0] *= f, acc[i][1] *= f, acc[i][2] *= f, acc[i][3] *= f;
+          for (int x = 0; x < NG; ++x) {
+            float a[2], b[2];
+            split2(wa[x], a[0], a[1]);
+            split2(wb[x], b[0], b[1]);
 #pragma unroll
-          for (int x = 0; x < NG; ++x) zacc[x][0] *= f, zacc[x][1] *= f, psum[x][0] *= f, psum[x][1] *= f;
+            for (int c = 0; c < 2; ++c) {
+              float mo = fmaxf(a[c], b[c]);
+#pragma unroll
+              for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) mo = fmaxf(mo, __shfl_xor_sync(0xffffffffu, mo, d));
+              const uint32_t down = mo >= P_MOST ? (__float_as_uint(mo) >> 23) - 127u - P_AIM : 0u;
+              const float f = __uint_as_float((127u - down) << 23);
+              F[x][c] *= f, a[c] *= f, b[c] *= f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[4 * x + i][c] *= f, acc[4 * x + i][2 + c] *= f;
+              zacc[x][c] *= f, psum[x][c] *= f;
+            }
+            wa[x] = pair2(a[0], a[1]), wb[x] = pair2(b[0], b[1]);
+          }
         }
       }
       uint32_t bf[NG][2][2];  // P as the B operand: SIDE: of either page; else its hi and its lo
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
         const uint32_t za = hva & 0x000f000fu, zb = hvb & 0x000f000fu;
-        const float sa = va[x] * F, sb = vbs[x] * F;
         const float ca = 8.f / TWO24 - (x ? hi_f32(za) : lo_f32(za)), cb = 8.f / TWO24 - (x ? hi_f32(zb) : lo_f32(zb));
-        const float a0 = pa[0] * sa, a1 = pa[1] * sa, b0 = pb[0] * sb, b1 = pb[1] * sb;
+        // To the grid: next to 0.75 a number below 0.25 keeps multiples of 2^-24 (a larger one its f32 bits, or 2^-23).
+        const uint64_t grid = pair2(0.75f, 0.75f), off = pair2(-0.75f, -0.75f);
+        float a0, a1, b0, b1;
+        split2(add2(add2(wa[x], grid), off), a0, a1);
+        split2(add2(add2(wb[x], grid), off), b0, b1);
         zacc[x][0] = fmaf(b0, cb, fmaf(a0, ca, zacc[x][0]));
         zacc[x][1] = fmaf(b1, cb, fmaf(a1, ca, zacc[x][1]));
         psum[x][0] += a0 + b0;
@@ -551,7 +588,6 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
         for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) z[x][c] += __shfl_xor_sync(0xffffffffu, z[x][c], d);
       }
     }
-    const float unit = TWO24 / F;
     const bool whole = at.page == 0 && count == w.np;
     float* part = p.part + ((size_t)worker * 2 + (at.page == 0 ? 1 : 0)) * DQ_SLOT * (D + 2);
 #pragma unroll
@@ -560,6 +596,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       const float inv = 1.0f / l[c];
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
+        const float unit = TWO24 / F[x][c];
         float v[8];  // elements 64 x + 8 gq ...
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

@@ -881,3 +881,88 @@ def test_shared_prefix_and_compaction(gpu, quantised):
                                                4, True, chunk=63)[0]]
         # A near-tie may be broken the other way by the f16 rounding of the weights; most sequences agree throughout.
         assert sum(a == b for a, b in zip(plain, cpu)) >= 4
+
+
+# ---- what little weights and small groups lose -------------------------------------------------------------------------
+# The tolerance of an element here is from its own group's values and weights, not from the largest of the head. The kernel
+# sums P = p * scale times codes of 0..15, so an error of P's own size e gives at most 15 e: with A = sum(15 p scale) / sum(p) over
+# the group's tokens, a result is off by half a step of f16, by 2 ds A (ds: the scores' error, as above), by the f32 sums,
+# 2^-16 A, and by the weights that the two f16 parts cannot hold: less than 2^-34 of the largest P for each of n tokens,
+# and so n 2^-34 A at most.
+def group_mean(q, kc, vc, row, n, scale):
+    """As `attend` for one row q [H, D] and n keys: the result and that tolerance, each [H, D]."""
+    H, D = q.shape
+    G, P = kc.shape[1:3]
+    pages = row[:-(-n // P)]
+    k = kv4.read(kc[pages], D).reshape(-1, G, D)[:n].astype(f64)
+    v = kv4.read(vc[pages], D).reshape(-1, G, D)[:n].astype(f64)
+    ks, vs = ((kv4.parts(c[pages], D)[1] & np.uint16(0xFFF0)).view(h).astype(f64).transpose(0, 2, 1, 3).reshape(-1, G, kv4.groups(D))[:n]
+              for c in (kc, vc))
+    out, tol = np.zeros((H, D)), np.zeros((H, D))
+    for hh in range(H):
+        g = hh // (H // G)
+        x = k[:, g] @ q[hh].astype(f64) * f64(f(scale))
+        p = np.exp(x - x.max())
+        p /= p.sum()
+        out[hh] = p @ v[:, g]
+        A = np.repeat(15 * (p @ vs[:, g]), 64)[:D]
+        ds = 2 * 32 * 2.0 ** -24 * abs(scale) * 15 * ks[:, g].max() * np.abs(q[hh].astype(f64)).sum()
+        tol[hh] = 2.0 ** -11 * np.abs(out[hh]) + (2 * ds + 2.0 ** -16 + n * 2.0 ** -34) * A + 2.0 ** -25
+    return out, tol
+
+
+def sink_case(seed, n, H, G, D, at, above, ratio):
+    """n keys of which `at` scores `above` more than the rest's typical one and has no value; the values' last group of 64 is
+    2^-ratio of the first."""
+    r = np.random.default_rng(seed)
+    NP = -(-n // 16) + 1
+    scale = 1 / np.sqrt(D)
+    q = r.standard_normal((H, D)).astype(h)
+    q[:, 0] = 4                                       # every head sees the sink's key alike
+    k, v = r.standard_normal((2, NP, G, 16, D))
+    k[..., 0] = 0
+    v *= 2.0 ** 12
+    v[..., 64:] *= 2.0 ** -ratio
+    page = r.permutation(NP).astype(i32)
+    for t in at:
+        k[page[t // 16], :, t % 16], v[page[t // 16], :, t % 16] = 0, 0
+        k[page[t // 16], :, t % 16, 0] = above / (4 * scale)
+    cache = []
+    for x in (k, v):
+        c = np.zeros((NP, G, 16, kv4.row_bytes(D)), u8)
+        code, head = kv4.parts(c, D)
+        cd, hd = kv4.quantize(x.astype(h))
+        code[:], head[:] = kv4.pack(cd), hd
+        cache.append(c)
+    return q, cache[0], cache[1], page[None], scale
+
+
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (12, 2, 128), (4, 1, 64), (40, 5, 64)])
+@pytest.mark.parametrize("at,above,ratio", [((0,), 14, 10), ((2000,), 14, 0), ((3999,), 14, 20), ((0,), 20, 0), ((5, 900, 3500), 20, 16),
+                                            ((3999,), 24, 10), ((), 0, 20)])
+def test_decode_weights_next_to_a_sink_without_value(gpu, H, G, D, at, above, ratio):
+    n = 4000
+    q, kc, vc, table, scale = sink_case(n + H + ratio, n, H, G, D, at, above, ratio if D == 128 else 0)
+    want, tol = group_mean(q, kc, vc, table[0], n, scale)
+    o, = run(gpu, "decode_attention_q4", [q[None], kc, vc, table, np.array([n], i32), np.zeros((1, H, D), h)], [5], [F32(scale)])
+    near(o[0], want, tol)
+
+
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (12, 2, 64)])
+def test_decode_scores_that_grow_all_along(gpu, H, G, D):
+    # Every page's scores outgrow the ones before (the running maximum is renewed again and again), and most of the weight's
+    # tokens have no value: what counts lies behind, 2^-12 and less of the maximum.
+    n = 640
+    q, kc, vc, table, scale = sink_case(H + D, n, H, G, D, (), 0, 10 if D == 128 else 0)
+    kc, vc = kc.copy(), vc.copy()
+    for i, page in enumerate(table[0][:n // 16]):
+        x = np.zeros((G, 16, D), h)
+        x[..., 0] = (9.0 * i) / (4 * scale)
+        cd, hd = kv4.quantize(x)
+        code, head = kv4.parts(kc, D)
+        code[page], head[page] = kv4.pack(cd), hd
+        if i % 3 == 2 or i == n // 16 - 1:
+            kv4.parts(vc, D)[1][page] = 0             # scale 0: no value
+    want, tol = group_mean(q, kc, vc, table[0], n, scale)
+    o, = run(gpu, "decode_attention_q4", [q[None], kc, vc, table, np.array([n], i32), np.zeros((1, H, D), h)], [5], [F32(scale)])
+    near(o[0], want, tol)
