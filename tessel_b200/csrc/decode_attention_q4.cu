@@ -4,12 +4,15 @@
 // Mathematics. With a key's code u, zero point z and scale s (64 elements share z and s), and a
 // query q: q.k = sum over groups of s (q.u - z sum(q)); so the tensor cores multiply q by the raw
 // codes and the scale and zero point come in afterwards, once per (token, head, group). For the
-// values, o = sum_t p_t s_t (u_t - z_t) = sum_t P_t (u_t - 8) + sum_t P_t (8 - z_t) with P = p s:
-// the scale rides on the weight, the second sum is one number per (head, group). Without the -8 the
-// all-positive products would make the accumulator hundreds of times larger than the result of a long
-// context, and the tensor cores' sums are not rounded to nearest. It is taken out of the accumulators
-// every CENTRE pairs of pages (8 sum P, one number per column): that costs a tenth of centring the
-// operands, and between two times the accumulator grows by the weights of 256 tokens only.
+// values, o = sum_t p_t s_t (u_t - z_t) = sum_t P_t u_t - sum_t P_t z_t with P = p s: the scale rides on
+// the weight, the second sum is one number per (head, group).
+//
+// The tensor cores cut products and sums off towards zero, and products that are never negative would
+// grow hundreds of times larger than the result of a long context, all of them cut down. So the tokens
+// of the second half of a page enter as (-P)(15 - u), with P (15 - z) in the other sum: the complement
+// costs no instruction, products of both signs nearly cancel, and so do their cuts. What the other sum
+// still holds is taken out of the accumulators every CENTRE pairs of pages. (Four of 131072 tokens, 32/8
+// heads: 2.11e-4 off in all, of which 2.108e-4 by rounding to f16; 2.8e-4 without the complement.)
 //
 // A code becomes an f16 operand by one AND: the nibble in the low bits of an f16 is the subnormal
 // u 2^-24, the next nibble 16 u 2^-24, and the tensor cores take subnormals as they are. For the
@@ -356,12 +359,12 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
     }
     float m[2] = {NO_MAX, NO_MAX}, l[2] = {0.f, 0.f};
     float F[NG][2];  // of the columns' heads: the first page with a value sets it
-    float acc[4 * NG][4], zacc[NG][2], psum[NG][2];  // psum: P since the last centring, of this lane's tokens
+    float acc[4 * NG][4], zsum[NG][2];  // zsum: P z, or P (z - 15), since the last centring, of this lane's tokens
 #pragma unroll
     for (int i = 0; i < 4 * NG; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
     for (int x = 0; x < NG; ++x) {
-      zacc[x][0] = zacc[x][1] = psum[x][0] = psum[x][1] = 0.f;
+      zsum[x][0] = zsum[x][1] = 0.f;
       F[x][0] = F[x][1] = __uint_as_float((127u + F_MOST) << 23);
     }
 
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
             F[x][c] = __uint_as_float(__float_as_uint(F[x][c]) + ((uint32_t)up << 23));
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[4 * x + i][c] *= f, acc[4 * x + i][2 + c] *= f;
-            zacc[x][c] *= f, psum[x][c] *= f;
+            zsum[x][c] *= f;
           }
         }
 #pragma unroll
@@ -457,10 +460,10 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       const float pa[2] = {ex2(xa[0]), ex2(xa[1])}, pb[2] = {ex2(xb[0]), ex2(xb[1])};
       l[0] += pa[0] + pb[0];
       l[1] += pa[1] + pb[1];
-      // P = p s F of the two tokens, columns in pairs.
+      // P = p s F of the first token and -P of the second, columns in pairs.
       uint64_t wa[NG], wb[NG];
       {
-        const uint32_t sa = hva & 0xfff0fff0u, sb = hvb & 0xfff0fff0u;
+        const uint32_t sa = hva & 0xfff0fff0u, sb = (hvb & 0xfff0fff0u) | 0x80008000u;
         const uint64_t p2a = pair2(pa[0], pa[1]), p2b = pair2(pb[0], pb[1]);
         float most = 0.f;
 #pragma unroll
@@ -471,7 +474,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
           float a0, a1, b0, b1;
           split2(wa[x], a0, a1);
           split2(wb[x], b0, b1);
-          most = fmaxf(most, fmaxf(fmaxf(a0, a1), fmaxf(b0, b1)));
+          most = fmaxf(most, fmaxf(fmaxf(a0, a1), fmaxf(-b0, -b1)));
         }
         if (__any_sync(0xffffffffu, most >= P_MOST)) {
 #pragma unroll
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
             split2(wb[x], b[0], b[1]);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float mo = fmaxf(a[c], b[c]);
+              float mo = fmaxf(a[c], -b[c]);
 #pragma unroll
               for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) mo = fmaxf(mo, __shfl_xor_sync(0xffffffffu, mo, d));
               const uint32_t down = mo >= P_MOST ? (__float_as_uint(mo) >> 23) - 127u - P_AIM : 0u;
@@ -489,7 +492,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
               F[x][c] *= f, a[c] *= f, b[c] *= f;
 #pragma unroll
               for (int i = 0; i < 4; ++i) acc[4 * x + i][c] *= f, acc[4 * x + i][2 + c] *= f;
-              zacc[x][c] *= f, psum[x][c] *= f;
+              zsum[x][c] *= f;
             }
             wa[x] = pair2(a[0], a[1]), wb[x] = pair2(b[0], b[1]);
           }
@@ -499,16 +502,15 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
         const uint32_t za = hva & 0x000f000fu, zb = hvb & 0x000f000fu;
-        const float ca = 8.f / TWO24 - (x ? hi_f32(za) : lo_f32(za)), cb = 8.f / TWO24 - (x ? hi_f32(zb) : lo_f32(zb));
+        // z, and 15 - z where P is negative, 2^-24 each as the codes are.
+        const float ca = x ? hi_f32(za) : lo_f32(za), cb = 15.f / TWO24 - (x ? hi_f32(zb) : lo_f32(zb));
         // To the grid: next to 0.75 a number below 0.25 keeps multiples of 2^-24 (a larger one its f32 bits, or 2^-23).
         const uint64_t grid = pair2(0.75f, 0.75f), off = pair2(-0.75f, -0.75f);
         float a0, a1, b0, b1;
         split2(add2(add2(wa[x], grid), off), a0, a1);
-        split2(add2(add2(wb[x], grid), off), b0, b1);
-        zacc[x][0] = fmaf(b0, cb, fmaf(a0, ca, zacc[x][0]));
-        zacc[x][1] = fmaf(b1, cb, fmaf(a1, ca, zacc[x][1]));
-        psum[x][0] += a0 + b0;
-        psum[x][1] += a1 + b1;
+        split2(add2(add2(wb[x], off), grid), b0, b1);
+        zsum[x][0] = fmaf(b0, cb, fmaf(a0, ca, zsum[x][0]));
+        zsum[x][1] = fmaf(b1, cb, fmaf(a1, ca, zsum[x][1]));
         const uint32_t pha = pack_h2(a0, a1), phb = pack_h2(b0, b1);
         const uint32_t bh0 = movm_t(pha), bh1 = movm_t(phb);
         const uint32_t bl0 = movm_t(pack_h2(a0 - lo_f32(pha), a1 - hi_f32(pha)));
@@ -537,7 +539,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
             // Of the word's nibbles e0 e2 e4 e6 e1 e3 e5 e7: k = 0: e0, e2 are rows gq, gq + 8; 1: e4, e6; 2: e1,
             // e3; 3: e5, e7. Rows 8..15 always weigh 16.
             const uint32_t v01 = (k & 2 ? hi01 : lo01) >> (8 * (k & 1)), v23 = (k & 2 ? hi23 : lo23) >> (8 * (k & 1));
-            const uint32_t a_0 = v01 & 0x000f000fu, a_1 = v01 & 0x00f000f0u, a_2 = v23 & 0x000f000fu, a_3 = v23 & 0x00f000f0u;
+            const uint32_t a_0 = v01 & 0x000f000fu, a_1 = v01 & 0x00f000f0u, a_2 = ~v23 & 0x000f000fu, a_3 = ~v23 & 0x00f000f0u;
             mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bf[x][s][0], bf[x][s][1]);
             if (!SIDE) mma16816(acc[4 * x + k], a_0, a_1, a_2, a_3, bf[x][1][0], bf[x][1][1]);
           }
@@ -550,14 +552,14 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
       for (int x = 0; x < NG; ++x)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float s = psum[x][c];
+          float z = zsum[x][c];
 #pragma unroll
-          for (int d = 4; d <= 16; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-          psum[x][c] = 0.f;
+          for (int d = 4; d <= 16; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+          zsum[x][c] = 0.f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            acc[4 * x + k][c] = fmaf(s, -8.f / TWO24, acc[4 * x + k][c]);
-            acc[4 * x + k][2 + c] = fmaf(s, -128.f / TWO24, acc[4 * x + k][2 + c]);
+            acc[4 * x + k][c] -= z;
+            acc[4 * x + k][2 + c] = fmaf(z, -16.f, acc[4 * x + k][2 + c]);
           }
         }
     };
@@ -576,18 +578,10 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
     }
 
     // ---- the segment's result ---------------------------------------------------------------------------
-    float z[NG][2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) l[c] += __shfl_xor_sync(0xffffffffu, l[c], d);
-#pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        z[x][c] = zacc[x][c];
-#pragma unroll
-        for (int d = SIDE ? 2 : 4; d <= 16; d = d == 2 ? 4 : d * 2) z[x][c] += __shfl_xor_sync(0xffffffffu, z[x][c], d);
-      }
-    }
     const bool whole = at.page == 0 && count == w.np;
     float* part = p.part + ((size_t)worker * 2 + (at.page == 0 ? 1 : 0)) * DQ_SLOT * (D + 2);
 #pragma unroll
@@ -603,7 +597,7 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
           const int upper = (i >> 1) & 1;  // the nibble's weight; its product: see above
           float a = acc[4 * x + 2 * (i & 1) + (i >> 2)][2 * upper + c];
           if (SIDE) a += __shfl_xor_sync(0xffffffffu, a, 2);  // columns h and h + 4 are the same head
-          v[i] = fmaf(a, upper ? 0.0625f * unit : unit, z[x][c] * unit);
+          v[i] = a * (upper ? 0.0625f * unit : unit);
         }
         // SIDE: both lanes of a pair hold the sums; they take a group each.
         if (hh < nh && (!SIDE || (t >> 1) == x)) {

@@ -966,3 +966,17 @@ def test_decode_scores_that_grow_all_along(gpu, H, G, D):
     want, tol = group_mean(q, kc, vc, table[0], n, scale)
     o, = run(gpu, "decode_attention_q4", [q[None], kc, vc, table, np.array([n], i32), np.zeros((1, H, D), h)], [5], [F32(scale)])
     near(o[0], want, tol)
+
+
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (12, 2, 128), (16, 4, 64)])
+def test_decode_of_a_long_context_has_no_bias(gpu, H, G, D):
+    # The tensor cores cut products and sums off towards zero. Cuts of one sign do not average out: they stay the same share of
+    # A (see above) at every length, while the result becomes smaller with it. Here a result is about A 2^-11 (64 normal numbers
+    # span some fifteen steps of 0.35, and 131072 of them average to 1 / 362), half a step of f16 2^-22 A. The mean error must
+    # not pass a quarter of that, 2^-24 A; rounding to f16, 2^-23 A each over 1024 elements or more, leaves 2^-28 A.
+    n = 131072
+    q, kc, vc, table, scale = sink_case(H, n, H, G, D, (), 0, 0)
+    want, _ = group_mean(q, kc, vc, table[0], n, scale)
+    o, = run(gpu, "decode_attention_q4", [q[None], kc, vc, table, np.array([n], i32), np.zeros((1, H, D), h)], [5], [F32(scale)])
+    A = 15 * 2.0 ** 12 * 0.35
+    assert abs((o[0].astype(f64) - want).mean()) <= 2.0 ** -24 * A
