@@ -16,8 +16,9 @@
 //
 // A code becomes an f16 operand by one AND: the nibble in the low bits of an f16 is the subnormal
 // u 2^-24, the next nibble 16 u 2^-24, and the tensor cores take subnormals as they are. For the
-// keys the 16 is taken out of q (q / 16 is exact, or off by 2^-25 where |q| < 2^-10), for the
-// values out of the accumulators.
+// keys the 16 is in q: 16 q meets the low nibbles, q the high ones, both exact. (Where a head group holds
+// a |q| of 4096 or more, 16 q may pass the largest f16: there q and q / 16, which loses bits of numbers
+// below 2^-22 of that one.) For the values it is taken out of the accumulators.
 //
 // P is split in two f16 (hi + lo): 22 bits down to 2^-2, below that the multiples of 2^-24. A power of
 // two F for each head and group follows the largest P, up and down: not the largest scale, nor another
@@ -315,7 +316,6 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
   // Rows of the K tile (and columns of the V tile) are the page's tokens in the order that lets a
   // lane's four V tokens be t, 4 + t, 8 + t, 12 + t: row r is token (r & 7) / 2 + 4 (r & 1) + (r & 8).
   const int tok_a = (gq >> 1) + 4 * (gq & 1), tok_b = tok_a + 8;
-  const float sc2 = p.scale * LOG2E * TWO24;
   const uint32_t ring_u = smem_u32(ring);
   const int side = SIDE ? t >> 1 : 0;  // the page of a pair whose scores this lane holds
   int cs = 0, phase = 0;               // the slot that is read next, and its phase
@@ -331,8 +331,9 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
     // Q as the B operand: column gq is head gq (SIDE: head gq & 3), the rows of step k of group x are elements 64 x + 16 t + 2 k, + 1 and the same + 8, as the words of
     // codes hold them; odd steps' nibbles weigh 16.
     uint32_t qf[NG][4][2];
-    float qsum[NG][2];
+    float qsum[NG][2], sc2 = p.scale * LOG2E * TWO24;
     {
+      bool large = false;  // some |q| is 4096 or more
       const int hc = SIDE ? gq & 3 : gq;
       const bool live = hc < nh;
       const __half* q = p.Q + ((size_t)at.b * p.H + h0 + (live ? hc : 0)) * D + 16 * t;
@@ -343,19 +344,34 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
           lo = *reinterpret_cast<const uint4*>(q + 64 * x);
           hi = *reinterpret_cast<const uint4*>(q + 64 * x + 8);
         }
-        uint32_t w[4][2] = {{lo.x, hi.x}, {lo.y, hi.y}, {lo.z, hi.z}, {lo.w, hi.w}};
+        const uint32_t w[4][2] = {{lo.x, hi.x}, {lo.y, hi.y}, {lo.z, hi.z}, {lo.w, hi.w}};
         float s = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           s += lo_f32(w[k][0]) + hi_f32(w[k][0]) + lo_f32(w[k][1]) + hi_f32(w[k][1]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) qf[x][k][e] = (k & 1) ? mul_h2(w[k][e], 0x2c002c00u) : w[k][e];  // 1/16
+          for (int e = 0; e < 2; ++e) {
+            qf[x][k][e] = w[k][e];
+            large = large || (w[k][e] & 0x7fffu) >= 0x6c00u || (w[k][e] & 0x7fff0000u) >= 0x6c000000u;
+          }
         }
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
         qsum[x][0] = __shfl_sync(0xffffffffu, s, 8 * t);      // of column 2t
         qsum[x][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);  // of column 2t + 1
       }
+      large = __any_sync(0xffffffffu, large);
+      const uint32_t by = large ? 0x2c002c00u : 0x4c004c00u;  // 1 / 16, 16
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (((k & 1) != 0) == large) qf[x][k][e] = mul_h2(qf[x][k][e], by);
+        if (!large) qsum[x][0] *= 16.f, qsum[x][1] *= 16.f;
+      }
+      if (!large) sc2 *= 0.0625f;
     }
     float m[2] = {NO_MAX, NO_MAX}, l[2] = {0.f, 0.f};
     float F[NG][2];  // of the columns' heads: the first page with a value sets it

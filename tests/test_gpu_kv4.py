@@ -980,3 +980,20 @@ def test_decode_of_a_long_context_has_no_bias(gpu, H, G, D):
     o, = run(gpu, "decode_attention_q4", [q[None], kc, vc, table, np.array([n], i32), np.zeros((1, H, D), h)], [5], [F32(scale)])
     A = 15 * 2.0 ** 12 * 0.35
     assert abs((o[0].astype(f64) - want).mean()) <= 2.0 ** -24 * A
+
+
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (12, 2, 128), (5, 5, 64)])
+@pytest.mark.parametrize("q_size,k_size", [(2.0 ** -18, 2e4), (2.0 ** -12, 300.0), (1000.0, 0.01), (1.2e4, 2e-3)])
+def test_decode_scores_of_small_and_large_queries(gpu, H, G, D, q_size, k_size):
+    n = 40
+    _, _, vc, table, _ = sink_case(D + H, n, H, G, D, (), 0, 0)
+    r = np.random.default_rng(H)
+    q = (q_size * r.standard_normal((H, D)).clip(-3, 3)).astype(h)
+    kc = np.zeros(vc.shape, u8)
+    code, head = kv4.parts(kc, D)
+    cd, hd = kv4.quantize((k_size * r.standard_normal(code.shape[:3] + (D,)).clip(-3, 3)).astype(h))
+    code[:], head[:] = kv4.pack(cd), hd
+    scale = 2 / (q_size * k_size * np.sqrt(D))
+    want, tol = group_mean(q, kc, vc, table[0], n, scale)
+    o, = run(gpu, "decode_attention_q4", [q[None], kc, vc, table, np.array([n], i32), np.zeros((1, H, D), h)], [5], [F32(scale)])
+    near(o[0], want, tol)
