@@ -7,7 +7,8 @@
 // when a row's maximum grew by more than 2^8; P is rounded to f16 for the second product (as
 // chunk_attention and prefill_attention round it; its relative error, 2^-11 at most and independent
 // from key to key, adds to the result about what the result's own rounding to f16 does), its sum is
-// kept in f32. K and V enter as f16 tiles; every value of the cache is an f16 number, so unpacking
+// kept in f32. The largest weight is 2^7 to 2^15, so that relative error holds for weights down to 2^-21
+// of it; smaller ones are off by up to 2^-32 of it. K and V enter as f16 tiles; every value of the cache is an f16 number, so unpacking
 // rounds nothing.
 //
 // Roles of a CTA's sixteen warps: warp 0 brings Q (TMA) and the pages' 4-bit records (bulk copies);
@@ -46,6 +47,7 @@ constexpr int CQ_THREADS = 512;  // warps 0 TMA, 1-2 MMA, (3 idle), 4-7 unpack, 
 constexpr int CQ_LEAST = 1;      // tiles a CTA takes at least
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.0f;
+constexpr float P_AIM = 7.0f;  // log2 of a row's largest weight when its reference is set: up to 2^15 later, an f16 holds 2^16
 
 // What a table entry outside the cache reads as.
 __device__ __align__(128) unsigned char g_zero_record[2048];
@@ -557,7 +559,7 @@ __global__ void __launch_bounds__(CQ_THREADS, 1) chunk_q4_kernel(const __grid_co
             mx = fmaxf(mx, x);
           }
         }
-        mx *= sc2;  // log2 domain (the scale is positive)
+        mx = fmaf(mx, sc2, -P_AIM);  // log2 domain (the scale is positive)
         const float m_new = fmaxf(m_ref, mx);
         const bool grow = m_new > m_ref + RESCALE_STEP;
         if (n == 0) {

@@ -997,3 +997,32 @@ def test_decode_scores_of_small_and_large_queries(gpu, H, G, D, q_size, k_size):
     want, tol = group_mean(q, kc, vc, table[0], n, scale)
     o, = run(gpu, "decode_attention_q4", [q[None], kc, vc, table, np.array([n], i32), np.zeros((1, H, D), h)], [5], [F32(scale)])
     near(o[0], want, tol)
+
+
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (5, 5, 64)])
+@pytest.mark.parametrize("rows", [1, 3, 200])
+@pytest.mark.parametrize("at,above", [((0,), 14), ((299,), 14), ((100,), 12), ((), 0)])
+def test_chunk_weights_next_to_a_sink_without_value(gpu, H, G, D, rows, at, above):
+    # Per element: half a step of f16; the weights' rounding to f16, 2^-11 of each, or half the spacing of the smallest f16
+    # numbers, 2^-25 where the row's largest weight is 2^7 or more: 2^-32 of that one; the scores' errors, each 64 roundings of
+    # 2^-24 of its products' sum, which move a weight's share of v and of the weights' sum; the f32 sums, 2^-16.
+    n = 300
+    _, kc, vc, table, scale = sink_case(n + H, n + rows, H, G, D, at, above, 0)
+    q = np.random.default_rng(rows).standard_normal((rows, H, D)).astype(h)
+    q[..., 0] = 4
+    meta = np.array([[0, rows, n, 0]], i32)
+    tables = np.zeros((rows, table.shape[1]), i32)
+    tables[0] = table[0]
+    o, = run(gpu, "chunk_attention_q4", [q, kc, vc, tables, meta, np.zeros((rows, H, D), h)], [5], [F32(scale)])
+    k, v = (kv4.read(c[table[0]], D).reshape(-1, G, D).astype(f64) for c in (kc, vc))
+    for i in range(rows):
+        for hh in range(H):
+            kk, vv = (x[:n + i + 1, hh // (H // G)] for x in (k, v))
+            qq = q[i, hh].astype(f64)
+            p = np.exp(kk @ qq * scale)
+            p /= p.sum()
+            want = p @ vv
+            ds = 64 * 2.0 ** -24 * scale * (np.abs(kk) @ np.abs(qq))
+            tol = 2.0 ** -11 * np.abs(want) + 2.0 ** -25 + (2.0 ** -11 + 2.0 ** -16) * (p @ np.abs(vv)) \
+                + 2.0 ** -32 * p.max() * np.abs(vv).sum(0) + (p * ds) @ (np.abs(vv) + np.abs(want))
+            near(o[i, hh], want, tol)
