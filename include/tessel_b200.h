@@ -210,8 +210,10 @@ int tb200_launch_count(tb200_ctx* ctx, uint64_t* out);
 /* No counterpart in the reference: run on a stream the host already owns
  * (a `cudaStream_t`), so that other libraries' work can be ordered with the
  * kernels. NULL restores the context's own stream. A kernel handle's workspace is
- * its context's: what was launched on the old stream must have finished, or be
- * waited for by the new one, before the same kernels are launched there. */
+ * its context's, and decode_attention_q4 and chunk_attention_q4 share one for all
+ * their handles: what was launched on the old stream must have finished, or be
+ * waited for by the new one, before the same kernels (of these two: either) are
+ * launched there. The same holds for graphs that were captured with them. */
 int tb200_set_stream(tb200_ctx* ctx, void* cuda_stream);
 /* The stream in use, as a `cudaStream_t`. */
 int tb200_get_stream(tb200_ctx* ctx, void** cuda_stream);

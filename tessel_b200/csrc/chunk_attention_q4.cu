@@ -747,10 +747,10 @@ bool chunk_q4_takes(const Q4Shape& q, int T, int H, int C, int MP) {
   return q.P == 16 && (q.D == 64 || q.D == 128) && q.NP > 0 && MP > 0 && T > 0 && C > 0 && H / q.G <= CQ_BM;
 }
 
+size_t chunk_q4_workspace(const Ctx* c, int D) { return (size_t)c->sm_count * (2 * 256 * (D + 2) * sizeof(float) + 16); }
+
 int make_chunk_q4(Ctx* c, Op& op, const Q4Shape& q) {
   op.p1 = c->sm_count;
-  op.scratch_bytes = (size_t)op.p1 * (2 * 256 * (q.D + 2) * sizeof(float) + 16);
-  TB_CUDA(c, cudaMalloc(&op.scratch, op.scratch_bytes));
   if (q.D == 128)
     TB_CUDA(c, cudaFuncSetAttribute(chunk_q4_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, CqSmem<128>::TOTAL));
   else
@@ -778,7 +778,7 @@ int launch_chunk_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
   p.scale = bits_f32(a[6]);
   p.least = CQ_LEAST;
   p.status = c->status;
-  p.part = (float*)op.scratch;
+  p.part = (float*)c->q4_work[q.D == 128];
   p.desc = (int*)(p.part + (size_t)op.p1 * 2 * 256 * (q.D + 2));
   const dim3 grid(op.p1), join(op.p1, q.D / 8);
   if (q.D == 128) {

@@ -129,6 +129,9 @@ struct Ctx {
   uint64_t launches = 0;
   // Device word the kernels raise when a bounded wait runs out: 0 = healthy.
   unsigned int* status = nullptr;
+  // The partials of the 4-bit attention kernels for head_dim 64 and 128: one workspace each for all ops of a
+  // context, whose launches follow one another. Made with the first op that needs it.
+  void* q4_work[2] = {nullptr, nullptr};
   // cuTensorMapEncodeTiled, resolved through the runtime (no link to libcuda).
   void* encode_tiled = nullptr;
   // Tensor-parallel communicator (NCCL, loaded at run time), or null.

@@ -193,6 +193,8 @@ void tb200_destroy(tb200_ctx* h) {
     if (g) cudaGraphExecDestroy(g);
   for (auto& op : c->ops)
     if (op.scratch) cudaFree(op.scratch);
+  for (void* w : c->q4_work)
+    if (w) cudaFree(w);
   for (auto& a : c->allocs) cudaFree((void*)a.first);
   if (c->status) cudaFree(c->status);
   if (c->ev0) cudaEventDestroy(c->ev0);

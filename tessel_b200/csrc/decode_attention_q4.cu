@@ -733,6 +733,10 @@ bool decode_q4_takes(const Q4Shape& q, int B, int MP) {
   return q.P == 16 && (q.D == 64 || q.D == 128) && q.NP > 0 && B > 0 && MP > 0;
 }
 
+size_t decode_q4_workspace(const Ctx* c, int D) {
+  return (size_t)c->sm_count * DQ_CTAS * DQ_WARPS * (2 * DQ_SLOT * (D + 2) * sizeof(float) + 16);
+}
+
 int make_decode_q4(Ctx* c, Op& op, const Q4Shape& q) {
   const int B = (int)op.shapes[0][0], H = (int)op.shapes[0][1];
   const int units = q.G * ((H / q.G + 7) / 8);
@@ -741,8 +745,6 @@ int make_decode_q4(Ctx* c, Op& op, const Q4Shape& q) {
   const long long most = ((long long)B * units * op.shapes[3][1] + DQ_LEAST * DQ_WARPS - 1) / (DQ_LEAST * DQ_WARPS);
   const long long fit = (long long)c->sm_count * DQ_CTAS;
   op.p1 = (int)(most < fit ? most : fit);
-  op.scratch_bytes = (size_t)op.p1 * DQ_WARPS * (2 * DQ_SLOT * (q.D + 2) * sizeof(float) + 16);
-  TB_CUDA(c, cudaMalloc(&op.scratch, op.scratch_bytes));
   TB_CUDA(c, cudaFuncSetAttribute(kernel_of(q.D, H / q.G, set_of(units)), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   q.D == 128 ? DqSmem<128>::TOTAL : DqSmem<64>::TOTAL));
   return 0;
@@ -763,7 +765,7 @@ int launch_decode_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
   p.units = p.G * p.hgroups / wh;
   p.least = DQ_LEAST;
   p.status = c->status;
-  p.part = (float*)op.scratch;
+  p.part = (float*)c->q4_work[q.D == 128];
   p.desc = (int*)(p.part + (size_t)op.p1 * DQ_WARPS * 2 * DQ_SLOT * (q.D + 2));
   const bool few = p.H / p.G <= 4;
   TB_CUDA(c, launch_k(c, kernel_of(q.D, p.H / p.G, wh), dim3(op.p1), dim3(DQ_THREADS),

@@ -405,7 +405,12 @@ int make_kv_q4(Ctx* c, Op& op) {
       if (chunk && s[4][0] > 65535) return bad("at most 65535 chunks");
       const int T = (int)s[0][0], H = (int)s[0][1], MP = (int)s[3][1];
       op.p0 = chunk ? chunk_q4_takes(q, T, H, (int)s[4][0], MP) : decode_q4_takes(q, T, MP);
-      return !op.p0 ? 0 : chunk ? make_chunk_q4(c, op, q) : make_decode_q4(c, op, q);
+      if (!op.p0) return 0;
+      if (void** work = &c->q4_work[q.D == 128]; !*work) {
+        const size_t d = decode_q4_workspace(c, q.D), k = chunk_q4_workspace(c, q.D);
+        TB_CUDA(c, cudaMalloc(work, d > k ? d : k));
+      }
+      return chunk ? make_chunk_q4(c, op, q) : make_decode_q4(c, op, q);
     }
     case K_PAGE_COPY:
       if (s[0].size() != 1 || s[1].size() != 2 || s[1][1] != 2) return bad("shapes are caches i64[A], pairs[N,2]");

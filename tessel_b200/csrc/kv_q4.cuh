@@ -53,10 +53,12 @@ int make_kv_q4(Ctx* c, Op& op);
 int launch_kv_q4(Ctx* c, Op& op, const uint64_t* a);
 // The tensor-core kernels behind decode_attention_q4 (decode_attention_q4.cu), for the shapes they take.
 bool decode_q4_takes(const Q4Shape& q, int B, int MP);
+size_t decode_q4_workspace(const Ctx* c, int D);  // bytes that a launch of any size needs at most
 int make_decode_q4(Ctx* c, Op& op, const Q4Shape& q);
 int launch_decode_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q);
 // And behind chunk_attention_q4 (chunk_attention_q4.cu).
 bool chunk_q4_takes(const Q4Shape& q, int T, int H, int C, int MP);
+size_t chunk_q4_workspace(const Ctx* c, int D);
 int make_chunk_q4(Ctx* c, Op& op, const Q4Shape& q);
 int launch_chunk_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q);
 

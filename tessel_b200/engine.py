@@ -191,6 +191,10 @@ class Engine:
         # The cache as the attention kernels see it, and bytes of one page of K (or V) of one layer.
         self.cache_shape = [lim.pages, cfg.kv_heads, lim.page, row] if kv4 else [lim.pages, lim.page, cfg.kv_heads, cfg.head_dim]
         self.page_bytes = lim.page * cfg.kv_heads * row
+        if kv4:
+            # Made here, with the cache, so that the attention kernels' workspace is not first asked for while serving.
+            q, mp = [1, cfg.heads, cfg.head_dim], lim.max_seq_pages
+            gpu.kernel("decode_attention_q4", [q, self.cache_shape, self.cache_shape, [1, mp], [1], q])
         self._page_tables: Optional[tuple] = None
         self._tables_stale = False  # pages were copied since the block tables on the device were sent
         self.layers: List[_DevLayer] = []

@@ -764,6 +764,56 @@ def test_two_contexts_at_once_and_a_foreign_stream(gpu):
         gpu.free(b)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_of_many_shapes_shares_one_workspace(gpu, D):
+    """A handle for each of many step sizes must not hold memory of its own; and launches of different sizes and of both kinds,
+    back to back without waiting, do not disturb one another."""
+    import torch
+    from tessel_b200.gpu import Gpu
+    H, G, P = 8, 2, 16
+    other = Gpu(0)                                    # a context of its own: nothing is made yet
+    sizes = [(1, 40), (4, 300), (9, 33), (16, 8), (2, 700), (64, 5)]
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for T, MP in sizes + [(T, MP + i) for T, MP in sizes for i in range(1, 6)]:
+        row, cache = [T, H, D], [4096, G, P, kv4.row_bytes(D)]
+        other.kernel("decode_attention_q4", [row, cache, cache, [T, MP], [T], row])
+        other.kernel("chunk_attention_q4", [row, cache, cache, [T, MP], [1, 4], row])
+    held = free - torch.cuda.mem_get_info()[0]
+    assert held < 96 << 20, f"72 handles hold {held >> 20} MB"
+
+    cases, want = [], []
+    for i, (T, MP) in enumerate(sizes):
+        q, kc, vc, table = attention_case(i + D, T, H, G, D, P, [MP] * T)
+        lens = np.random.default_rng(i).integers(1, MP * P + 1, T).astype(i32)
+        meta = np.array([[0, T, MP * P - T, 0]], i32)
+        for name, last in (("decode_attention_q4", lens), ("chunk_attention_q4", meta)):
+            a = [q, kc, vc, table, last, np.zeros((T, H, D), h)]
+            want.append(run(other, name, a, [5], [F32(0.1)])[0].tobytes())
+            cases.append((other.kernel(name, [x.shape for x in a]), [other.tensor(x) for x in a], a[5]))
+    for order in (cases, cases[::-1], cases[1::2] + cases[::2]):
+        for _, b, o in cases:
+            other.write(b[5], 0, o)
+        for k, b, _ in order:
+            other.launch(k, b + [F32(0.1)])
+        other.sync()
+        assert [other.fetch(b[5], h, o.shape).tobytes() for _, b, o in cases] == want
+    # The same as two graphs that take turns.
+    graphs = []
+    for half in (cases[::2], cases[1::2]):
+        other.capture_begin()
+        for k, b, _ in half:
+            other.launch(k, b + [F32(0.1)])
+        graphs.append(other.capture_end())
+    for _, b, o in cases:
+        other.write(b[5], 0, o)
+    for g in graphs * 3:
+        other.replay(g)
+    other.sync()
+    assert [other.fetch(b[5], h, o.shape).tobytes() for _, b, o in cases] == want
+    other.close()
+
+
 # ---- the engine and the scheduler --------------------------------------------------------------------------------------
 CFG = Config(dim=256, layers=2, heads=8, kv_heads=2, head_dim=64, ffn=512, vocab=1000, eps=1e-5, rope_theta=10000.0, max_pos=512,
              bos=1, eos=-1)

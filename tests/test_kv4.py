@@ -289,3 +289,10 @@ def test_the_scale_is_rounded_up_from_the_exact_range():
         step = F(2) ** (int(np.frexp(float(r))[1]) - 7)
         want = -(-r // step) * step
         assert F(scale) == want, (row[:2], scale, float(want))
+
+
+def test_the_attention_kernels_workspace_is_asked_for_with_the_cache():
+    # On a device the library allocates it with the first handle; here the handles are looked at.
+    make = tiny()
+    assert "decode_attention_q4" in [name for name, _ in make(kv4=True).gpu._kernels]
+    assert "decode_attention_q4" not in [name for name, _ in make().gpu._kernels]
