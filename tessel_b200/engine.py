@@ -196,6 +196,7 @@ class Engine:
             q, mp = [1, cfg.heads, cfg.head_dim], lim.max_seq_pages
             gpu.kernel("decode_attention_q4", [q, self.cache_shape, self.cache_shape, [1, mp], [1], q])
         self._page_tables: Optional[tuple] = None
+        self._pairs_staged = 0  # pairs of earlier copy_pages calls that the device may not have taken yet
         self._tables_stale = False  # pages were copied since the block tables on the device were sent
         self.layers: List[_DevLayer] = []
         self.q8: List[Dict[str, Buf]] = []
@@ -399,6 +400,7 @@ class Engine:
         ``[len(want), vocab]`` (a view of page-locked memory, valid until the next step)."""
         n, t, bw, prefill = self._upload(tokens, pos, slots, attn, want)
         self._run(t, prefill, bw, False)
+        self._pairs_staged = 0  # (what follows waits for the device)
         if not len(want):
             self.gpu.sync()
             return np.empty((0, self.cfg.vocab), np.float32)
@@ -414,6 +416,7 @@ class Engine:
         device: returns int32 ``[len(want)]`` token ids."""
         n, t, bw, prefill = self._upload(tokens, pos, slots, attn, want)
         self._run(t, prefill, bw, True)
+        self._pairs_staged = 0
         if not len(want):
             self.gpu.sync()
             return np.empty((0,), np.int32)
@@ -711,10 +714,20 @@ class Engine:
         g = self.gpu
         if self._page_tables is None:
             caches = np.array([b.ptr for l in self.layers for b in (l.kc, l.vc)], np.uint64)
-            self._page_tables = (g.tensor(caches), len(caches), g.alloc(self.lim.pages * 8))
-        caches, n, buf = self._page_tables
+            # (A wave's pairs begin anywhere in the first half: the kernel's array of them fits behind.)
+            self._page_tables = (g.tensor(caches), len(caches), g.alloc(2 * self.lim.pages * 8),
+                                 g.host_array((2 * self.lim.pages, 2), np.int32))
+        caches, n, buf, stage = self._page_tables
         copy = g.kernel("page_copy", [[n], [self.lim.pages, 2]])
-        g.write(buf, 0, np.array([p for w in waves for p in w], np.int32))
+        # The pairs go up as a step's inputs do, without waiting; a step's end makes room again.
+        count = sum(len(w) for w in waves)
+        if self._pairs_staged + count > len(stage):
+            g.sync()
+            self._pairs_staged = 0
+        pairs = stage[self._pairs_staged:self._pairs_staged + count]
+        pairs[:] = [p for w in waves for p in w]
+        self._pairs_staged += count
+        g.write_async(buf, 0, pairs)
         at = 0
         for w in waves:
             g.launch(copy, [caches, Buf(buf.ptr + at * 8, buf.bytes - at * 8), I32(len(w)), I32(self.lim.pages), I32(self.page_bytes)])

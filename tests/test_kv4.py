@@ -296,3 +296,74 @@ def test_the_attention_kernels_workspace_is_asked_for_with_the_cache():
     make = tiny()
     assert "decode_attention_q4" in [name for name, _ in make(kv4=True).gpu._kernels]
     assert "decode_attention_q4" not in [name for name, _ in make().gpu._kernels]
+
+
+def test_copying_pages_does_not_wait_for_the_device():
+    """On a stand-in whose device is behind the host: copies to it and launches happen when somebody waits for it, and an array
+    handed to `write_async` is read only then."""
+    from emu import EmuGpu
+    from tessel_b200.engine import Decode, Engine, Limits, Prefill
+    from tessel_b200.model import Config, Weights
+
+    class Late(EmuGpu):
+        def __init__(self):
+            super().__init__()
+            self.queue, self.waits = [], 0
+
+        def sync(self):
+            self.waits += bool(self.queue)
+            queue, self.queue = self.queue, []
+            for call in queue:
+                call()
+
+        def write(self, b, offset, data):
+            self.sync()
+            super().write(b, offset, data)
+
+        def read(self, b, offset, out):
+            self.sync()
+            return super().read(b, offset, out)
+
+        def write_async(self, b, offset, a):
+            assert offset + a.nbytes <= b.bytes
+            self.queue.append(lambda: EmuGpu.write(self, b, offset, a))
+
+        def launch(self, k, args):
+            args = list(args)
+            self.queue.append(lambda: EmuGpu.launch(self, k, args))
+
+    w = Weights.random(Config.tiny(), 9)
+    e = Engine(Late(), w, Limits(page=4, pages=40, max_tokens=16, max_seq_pages=8))
+    e.graphs = False
+    e.copy_pages([(0, 1)])                            # (the first call makes its tables)
+    e.gpu.sync()
+    rng = np.random.default_rng(1)
+    shape = (40, e.page_bytes // 2)
+    want = []
+    for l in e.layers:
+        for b in (l.kc, l.vc):
+            x = rng.standard_normal(shape).astype(f16)
+            e.gpu.write(b, 0, x)
+            want.append(x)
+    e.step_greedy([3, 1], [0, 1], [0, 1], Prefill(), [1])
+    want = [e.gpu.fetch(b, f16, shape) for l in e.layers for b in (l.kc, l.vc)]
+    before = e.gpu.waits
+    calls = [[(0, 9), (0, 10), (3, 11)], [(9, 20)], [(20, 30), (11, 20)], [(i, i + 1) for i in range(39)], [(5, 6)]]
+    for pairs in calls[:3]:
+        e.copy_pages(pairs)
+    assert e.gpu.waits == before and e.gpu.queue, "the host waited for the device"
+    for i in range(60):                               # many more than fit side by side, whatever that takes
+        e.copy_pages(calls[3 + i % 2])
+    e.gpu.sync()
+    for x, b in zip(want, (b for l in e.layers for b in (l.kc, l.vc))):
+        for pairs in calls[:3] + [calls[3 + i % 2] for i in range(60)]:
+            old = x.copy()
+            for s, d in pairs:
+                x[d] = old[s]
+        assert np.array_equal(e.gpu.fetch(b, f16, shape), x)
+    # A step's end has waited for the device in any case: from there on the room is free again.
+    for i in range(100):
+        e.step_greedy([7], [2 + i % 4], [2 + i % 4], Decode([[0]], [3 + i % 4]), [0])
+        before = e.gpu.waits
+        e.copy_pages([(i % 40, (i + 1) % 40), ((i + 2) % 40, (i + 3) % 40)])
+        assert e.gpu.waits == before
