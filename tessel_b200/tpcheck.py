@@ -46,15 +46,16 @@ def chunk_requests(cfg: Config) -> List[Request]:
     return [Request(g.integers(0, cfg.vocab, n).tolist(), CHUNK_NEW) for n in (9, 100)]
 
 
-def run(gpu, rank: int, nranks: int, exchange: Optional[Callable] = None) -> Dict[str, np.ndarray]:
+def run(gpu, rank: int, nranks: int, exchange: Optional[Callable] = None, kv4: bool = False) -> Dict[str, np.ndarray]:
     """Two packed prompts, one decode step, a 3-request greedy generation of 1 + 32 tokens, and a
     2-request generation with one prompt fed in chunks, on rank ``rank`` of ``nranks``. Returns
     the prefill logits ``pre`` [2, vocab], the decode step's logits ``dec`` [2, vocab], layer 1's
     cache shard ``kc``/``vc``, the real rows of x and h after the decode step, ``tokens`` [3, 33]
-    and ``chunk_tokens`` [2, 8]."""
+    and ``chunk_tokens`` [2, 8]. ``kv4``: the engines keep their cache in 4 bits (``kc``/``vc``
+    are then the values it stands for)."""
     cfg, w = model()
     lim = Limits(page=16, pages=40, max_tokens=128, max_seq_pages=8)
-    e = Engine(gpu, w, lim, rank=rank, nranks=nranks, exchange=exchange)
+    e = Engine(gpu, w, lim, rank=rank, nranks=nranks, exchange=exchange, kv4=kv4)
     g = np.random.default_rng(1)
     p1, p2 = g.integers(0, cfg.vocab, 37).tolist(), g.integers(0, cfg.vocab, 20).tolist()
     toks, pos = p1 + p2, list(range(37)) + list(range(20))
@@ -66,10 +67,10 @@ def run(gpu, rank: int, nranks: int, exchange: Optional[Callable] = None) -> Dic
     x = gpu.fetch(e.x, np.float32, (e.tmax, cfg.dim))[:2].copy()
     h = gpu.fetch(e.h, np.float16, (e.tmax, cfg.dim))[:2].copy()
     e2 = Engine(gpu, w, Limits(page=16, pages=64, max_tokens=128, max_seq_pages=8), rank=rank, nranks=nranks,
-                exchange=exchange)
+                exchange=exchange, kv4=kv4)
     outs, _ = generate_with(e2, requests(cfg), 3, True, device_argmax=True)
     e3 = Engine(gpu, w, Limits(page=16, pages=64, max_tokens=64, max_seq_pages=8), rank=rank, nranks=nranks,
-                exchange=exchange)
+                exchange=exchange, kv4=kv4)
     couts, _ = generate_with(e3, chunk_requests(cfg), 2, True, device_argmax=True, chunk=CHUNK)
     return dict(pre=pre, dec=dec, kc=kc, vc=vc, x=x, h=h, tokens=np.asarray([o.tokens for o in outs]),
                 chunk_tokens=np.asarray([o.tokens for o in couts]))

@@ -99,3 +99,45 @@ def test_ranks_on_gpus(tmp_path, world):
     compare(one, launch("gpu", world, str(tmp_path)))
     # The same with the sum, the residual add and the RMSNorm fused into one kernel over NVLink.
     compare(one, launch("gpufused", world, str(tmp_path)))
+
+
+# ---- the same with the cache in 4 bits ---------------------------------------------------------------------------------
+def compare_kv4(one, many):
+    """A prompt's own step attends to f16 rows: its logits agree as above. What is cached is quantised from rows that agree to
+    TOL of the largest only, so a code may be its neighbour, or a group's scale the next one: a value is off by a step at most
+    (a sixtieth more, and TOL for the row's own difference). A step of 1/15 of a group's span in some elements of some keys
+    moves the next step's logits little, but by more than TOL; the greedy tokens may part, yet never between ranks."""
+    a, b = one[0], many[0]
+    assert tpcheck.rel_err(b["pre"], a["pre"]) <= TOL
+    assert tpcheck.rel_err(b["dec"], a["dec"]) <= 0.05
+    for name in ("kc", "vc"):
+        full, got = a[name].astype(np.float64), tpcheck.gathered_cache(many, name).astype(np.float64)
+        assert got.shape == full.shape
+        used = np.abs(full).sum(axis=(1, 2, 3)) > 0
+        assert np.array_equal(np.abs(got).sum(axis=(1, 2, 3)) > 0, used), "the same pages are written"
+        assert all(len(np.unique(row)) <= 16 for row in full.reshape(-1, full.shape[-1])), "not a 4-bit cache"
+        span = np.maximum(full.max(-1), 0) - np.minimum(full.min(-1), 0)   # (head_dim 64: one group)
+        off = np.abs(got - full).max(-1)
+        assert (off <= span / 15 * (1 + 2.0 ** -5) + TOL * np.abs(full).max()).all()
+        assert (got == full)[used].mean() > 0.8
+    assert len({tpcheck.digest(r) for r in many}) == 1, "x and h differ between ranks"
+    for r in many:
+        for name in ("tokens", "chunk_tokens"):
+            assert np.array_equal(r[name], b[name])
+            assert r[name].shape == a[name].shape
+
+
+@pytest.mark.parametrize("world", [2, 4, 8])
+def test_ranks_on_cpu_with_a_4bit_cache(tmp_path, world):
+    compare_kv4(single("cpu4", str(tmp_path)), launch("cpu4", world, str(tmp_path)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("world", [2, 4, 8])
+def test_ranks_on_gpus_with_a_4bit_cache(tmp_path, world):
+    import torch
+    if torch.cuda.device_count() < world:
+        pytest.skip(f"needs {world} GPUs")
+    one = single("gpu4", str(tmp_path))
+    compare_kv4(one, launch("gpu4", world, str(tmp_path)))
+    compare_kv4(one, launch("gpufused4", world, str(tmp_path)))

@@ -1,10 +1,11 @@
 """One rank of a tensor-parallel engine run (launched by the tests, 1 to 8 ranks).
 
-    python tests/tp_worker.py cpu|gpu|gpufused <rank> <world> <port> <out.npz>
+    python tests/tp_worker.py cpu|gpu|gpufused[4] <rank> <world> <port> <out.npz>
 
 cpu: the engine on the oracle stand-in, the allreduce over gloo. gpu: the engine on the
 library, the allreduce over NCCL (NVLS off, plain peer transport). gpufused: the cross-rank sum
-fused with residual add and RMSNorm over peer memory (tp_reduce_norm). Every rank writes what
+fused with residual add and RMSNorm over peer memory (tp_reduce_norm). A 4 behind the mode: the
+cache in 4 bits. Every rank writes what
 ``tessel_b200.tpcheck.run`` returns: the prefill logits, one decode step's logits, the greedy
 tokens of a 32-step generation, its KV cache shard, and its x and h after the decode step.
 """
@@ -20,6 +21,7 @@ sys.path.insert(0, HERE)
 
 def main():
     mode, rank, world, port, out = sys.argv[1], int(sys.argv[2]), int(sys.argv[3]), sys.argv[4], sys.argv[5]
+    mode, kv4 = mode.rstrip("4"), mode.endswith("4")
     import torch
     import torch.distributed as dist
     from tessel_b200 import tpcheck
@@ -49,7 +51,7 @@ def main():
             everyone = [None] * world
             dist.all_gather_object(everyone, mine)
             return everyone
-    np.savez(out, **tpcheck.run(gpu, rank, world, exchange))
+    np.savez(out, **tpcheck.run(gpu, rank, world, exchange, kv4))
     if world > 1:
         dist.barrier()
         dist.destroy_process_group()
