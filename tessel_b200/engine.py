@@ -704,12 +704,15 @@ class Engine:
         """Copies cache pages, in every layer's K and V: ``pairs`` of (source, destination). Every copy reads its
         source as it was before the call, so pages may be moved along (5 -> 2 with 9 -> 5): copies that have to wait
         for others go into launches of their own, usually there is one. A page outside the cache, a page written twice
-        and pages exchanged in a circle are refused (ValueError) before anything is copied.
+        and pages exchanged in a circle are refused (ValueError) before anything is copied, and so is a cache whose pages
+        are no multiple of 16 bytes (a few tokens of a small head_dim).
         Block tables are the caller's: the ones a step sent stay as they are, and ``decode_resident``, which would go on
         from them, is refused until the next decode step."""
         waves = kv4_format.copy_waves(pairs, self.lim.pages)
         if not waves:
             return
+        if self.page_bytes % 16:
+            raise ValueError(f"pages of {self.page_bytes} bytes cannot be copied: a multiple of 16 is needed")
         self._tables_stale = True
         g = self.gpu
         if self._page_tables is None:

@@ -87,6 +87,8 @@ class Scheduler:
         self.chunk = max(0, min(chunk, e.lim.max_tokens - 1))
         if self.prefix and not self.chunk:
             raise ValueError("a shared prefix needs steps of at least two tokens")
+        if len(self.prefix) % e.lim.page and e.page_bytes % 16:
+            raise ValueError("a prefix that ends inside a page needs pages of a multiple of 16 bytes, to be copied")
         self.prefix_pages: List[int] = []  # the prefix's pages, once it is in the cache
         self.feeding: List[_Seq] = []  # sequences whose (long) prompt is still being fed in chunks
         self.start = time.perf_counter()

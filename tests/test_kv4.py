@@ -367,3 +367,23 @@ def test_copying_pages_does_not_wait_for_the_device():
         before = e.gpu.waits
         e.copy_pages([(i % 40, (i + 1) % 40), ((i + 2) % 40, (i + 3) % 40)])
         assert e.gpu.waits == before
+
+
+def test_pages_that_cannot_be_copied_are_refused_before_anything_is_admitted():
+    # head_dim 16 in 4 bits: 10 bytes a row and head, so two tokens of two heads are a page of 40 bytes.
+    from tessel_b200.sched import Request, Scheduler
+    e = tiny(page=2)(kv4=True)
+    assert e.page_bytes % 16
+    with pytest.raises(ValueError, match="multiple of 16"):
+        e.copy_pages([(0, 1)])
+    with pytest.raises(ValueError, match="multiple of 16"):
+        Scheduler(e, [Request([1], 2)], 1, prefix=[1, 2, 3])
+    s = Scheduler(e, [Request([1], 2), Request([7, 8], 2)], 2, prefix=[1, 2])   # ends with a page: nothing is forked
+    while not s.done():
+        assert s.step() != "idle"
+    with pytest.raises(ValueError, match="multiple of 16"):
+        s = Scheduler(e, [Request([1, 2, 3], 2), Request([7, 8], 6)], 2)
+        while not s.done():
+            s.step()
+            s.compact()
+    assert s.running and [q.pages for q in s.running] == [[3, 4, 5, 6]], "the tables are as they were"
