@@ -61,7 +61,7 @@ struct CqParams {
   float* part;  // [CTA][2][D + 2][256]: a row's numerator, maximum and sum, rows side by side
   int* desc;    // [CTA][4]: piece, KV head, block, CTAs that hold a part of the unit cut at this CTA's end (0: none)
   float scale;
-  int T, H, G, hq, tm, C, NP, MP, least;  // tm: tokens of a tile
+  int T, H, G, hq, tm, C, NP, MP;  // tm: tokens of a tile
   unsigned int* status;
 };
 
@@ -85,28 +85,8 @@ struct CqSmem {
   static_assert((CQ_THREADS + 8) * 8 <= KV_BYTES, "the prefix sums use the first K / V slot");
 };
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"((uint64_t)src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  unsigned short v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
-}
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // A piece of the step, empty if its descriptor does not lie inside it.
@@ -189,7 +169,7 @@ __device__ __forceinline__ bool find_walk(const CqParams& p, long long* scan, Wa
   }
   __syncthreads();
   const long long all = scan[CQ_THREADS] * p.G;
-  const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)p.least);
+  const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)CQ_LEAST);
   const long long start = blockIdx.x * share;
   if (start >= all) return false;  // uniform for the CTA
   long long at = scan[threadIdx.x] * p.G;
@@ -776,7 +756,6 @@ int launch_chunk_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
   p.meta = (const int*)a[4];
   p.O = (__half*)a[5];
   p.scale = bits_f32(a[6]);
-  p.least = CQ_LEAST;
   p.status = c->status;
   p.part = (float*)c->q4_work[q.D == 128];
   p.desc = (int*)(p.part + (size_t)op.p1 * 2 * 256 * (q.D + 2));

@@ -80,7 +80,7 @@ struct DqParams {
   float* part;  // [warp][2][8][D + 2]: accumulators [8][D], then maxima [8] and sums [8]
   int* desc;    // [warp][4]: sequence, head group, warps that hold a piece of the unit cut at this warp's end (0: none)
   float scale;
-  int B, H, G, NP, MP, hgroups, least;
+  int B, H, G, NP, MP, hgroups;
   int units;  // sets of WH head groups, which neighbouring warps take side by side, in a sequence
   unsigned int* status;
 };
@@ -96,11 +96,6 @@ struct DqSmem {
   static constexpr int TOTAL = SCAN + (DQ_THREADS + 1 + 2 * DQ_WARPS) * 8 + 128;
 };
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"((uint64_t)src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ uint32_t movm_t(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -113,24 +108,9 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  unsigned short v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
   return v;
 }
 __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
@@ -175,7 +155,7 @@ __device__ __forceinline__ Place find_place(const DqParams& p, long long* scan, 
     pages += scan[w];
   }
   const long long all = pages * units, workers = (long long)gridDim.x * owners;
-  const long long s = max((all + workers - 1) / workers, (long long)p.least);
+  const long long s = max((all + workers - 1) / workers, (long long)DQ_LEAST);
   *total = all;
   *share = s;
   // The thread whose sequences hold a warp's start says which one.
@@ -763,7 +743,6 @@ int launch_decode_q4(Ctx* c, Op& op, const uint64_t* a, const Q4Shape& q) {
   p.hgroups = (p.H / p.G + 7) / 8;
   const int wh = set_of(p.G * p.hgroups);
   p.units = p.G * p.hgroups / wh;
-  p.least = DQ_LEAST;
   p.status = c->status;
   p.part = (float*)c->q4_work[q.D == 128];
   p.desc = (int*)(p.part + (size_t)op.p1 * DQ_WARPS * 2 * DQ_SLOT * (q.D + 2));
