@@ -127,14 +127,17 @@ int tb200_host_free(tb200_ctx* ctx, void* ptr);
  * back; a slot outside the cache gives zeros. decode_attention_q4 and
  * chunk_attention_q4 are decode_attention and chunk_attention over such caches;
  * positions beyond the block table lie on page 0, a page outside the cache reads
- * as zeros; the pieces of a call must not share rows.
+ * as zeros; the pieces of a call must not share rows. Pages of 16 tokens with D 64
+ * or 128 (and at most 128 query heads per KV head, for chunk_attention_q4) run on
+ * the tensor cores, other shapes on one warp per row and head.
  *
  * page_copy (caches i64[A], pairs i32[N,2], then the i32 scalars n, NP and bytes):
  * for each of the A caches, whose device addresses (16-byte aligned) `caches` holds,
  * and each of the first n pairs (src, dst): page dst = page src, pages of `bytes`
  * bytes (a multiple of 16) in caches of NP pages. A pair with a page outside the
- * cache is skipped, and so is a cache whose address is 0 or not aligned. All pairs run at once: a page may be the source of several
- * pairs, but a page that one pair writes must not be in any other pair.
+ * cache is skipped, and so is a cache whose address is 0 or not aligned. All pairs
+ * run at once: a page may be the source of several pairs, but a page that one pair
+ * writes must not be in any other pair.
  *
  * The reference's `meta` and `warps` arguments have no equivalent: tile shapes
  * are chosen inside. */

@@ -29,7 +29,8 @@
 //
 // Bound: the tensor cores by operations; measured, the softmax warps (1700 of 1870 cycles per 64 keys, 1024 of them
 // the exponentials' unit) with the unpacking in the same issue slots. 2048 rows at position 30000, 32/8 heads, D 128:
-// 890 us, 1166 TFLOP/s; 8 pieces of 1-8 rows at 700-6000: 39 us, where unpacking a tile (1650 cycles) sets the pace.
+// 888 us at 1965 MHz, 1170 TFLOP/s; 1023-1034 us at the 1695 MHz that the power cap leaves. 8 pieces of 1-8 rows at
+// 700-6000: 39 us, where unpacking a tile (1650 cycles) sets the pace.
 //
 // NaN. A weight of zero times a NaN is a NaN, so a spoilt V row would reach rows that do not see it.
 // The unpacking warps store zeros for it instead and note the least such position of each 64-column

@@ -33,9 +33,10 @@
 // product, side by side. With five to eight heads a page fills the columns,
 // and lo is a second product.
 //
-// Bound: by bytes 2 (D/2 + 2 D/64) per token and KV head, from HBM; measured, the half-rate integer pipe and
-// dependent issue on fewer than three warps per scheduler come first (four ANDs and a shift per word of codes).
-// 256 sequences of 512-2304 tokens, 32/8 heads, D 128: 91 us, 4.2 TB/s; 4 of 100000-131072: 109 us, 4.5 TB/s.
+// Bound: by bytes 2 (D/2 + 2 D/64) per token and KV head, from HBM. Measured, nothing is saturated (HBM 0.64 of the copy
+// rate, integer pipe 58 %, issue slots 51 %): what is left is latency that fewer than three warps per scheduler
+// do not hide. 256 sequences of 512-2304 tokens, 32/8 heads, D 128: 97 us as calls on changing inputs, 3.9 TB/s
+// (93 with the same launches back to back); 4 of 100000-131072: 118 us, 4.2 TB/s (110). SM clock 1965 MHz.
 //
 // Work split. Every warp works on its own: it takes an equal share of the step's (sequence, KV head,
 // page) list, whatever the lengths are, finds its place from the lengths, brings its pages through a
@@ -308,8 +309,8 @@ __global__ void __launch_bounds__(DQ_THREADS, DQ_CTAS) decode_q4_kernel(const Dq
     const uint32_t mine = (hg / p.hgroups - at.hg * WH / p.hgroups) * SM::REC;  // this head's record in a slot
     const int h0 = hg / p.hgroups * hq + (hg % p.hgroups) * 8, nh = min(8, hq - (hg % p.hgroups) * 8);
 
-    // Q as the B operand: column gq is head gq (SIDE: head gq & 3), the rows of step k of group x are elements 64 x + 16 t + 2 k, + 1 and the same + 8, as the words of
-    // codes hold them; odd steps' nibbles weigh 16.
+    // Q as the B operand: column gq is head gq (SIDE: head gq & 3), the rows of step k of group x are elements
+    // 64 x + 16 t + 2 k, + 1 and the same + 8, as the words of codes hold them; odd steps' nibbles weigh 16.
     uint32_t qf[NG][4][2];
     float qsum[NG][2], sc2 = p.scale * LOG2E * TWO24;
     {

@@ -148,7 +148,9 @@ class Engine:
         ``kv4``: a separate, NON-PARITY mode (any number of ranks, with or without ``fp8``): the cache
         holds K and V in 4 bits with one scale and zero point for 64 elements (``tessel_b200.kv4``),
         0.27 of the f16 cache's bytes. Decode steps and prompts fed in chunks attend to the
-        quantised keys and values; a prompt's own prefill step attends to its rows in f16."""
+        quantised keys and values; a prompt's own prefill step attends to its rows in f16. Attention
+        is fast with pages of 16 tokens and a head_dim of 64 or 128; other shapes run on kernels of
+        one warp per row and head, tens of times slower and more."""
         full = w.cfg
         if fp8 and nranks != 1:
             raise ValueError("the FP8 mode runs on a single rank")
