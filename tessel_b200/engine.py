@@ -435,11 +435,11 @@ class Engine:
         their new tokens land in (the scheduler reserves them up front). It goes on from the block
         tables that step sent, so after ``copy_pages`` (``Scheduler.compact``) it is refused
         (ValueError) until a decode step has sent new ones."""
-        if self._tables_stale:
-            raise ValueError("pages were copied or moved since the last decode step: run one with the new block tables first")
         t = padded(n)
         if steps < 1:
             return np.empty((0, n), np.int32)
+        if self._tables_stale:
+            raise ValueError("pages were copied or moved since the last decode step: run one with the new block tables first")
         if self._hist is None or self._hist_rows < steps:
             self._hist_rows = max(steps, 512)
             self._hist = self.gpu.alloc(self._hist_rows * self.tmax * 4)

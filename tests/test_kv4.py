@@ -231,6 +231,7 @@ def test_resident_decoding_after_a_copy_of_pages_needs_a_step_with_its_tables():
     e.step_greedy([3, 1, 4], [0, 1, 2], [24, 25, 26], Prefill(), [2])
     e.step_greedy([7], [3], [27], Decode([[3]], [4]), [0])
     e.copy_pages([(3, 5)])
+    assert e.decode_resident(1, 0).shape == (0, 1)
     with pytest.raises(ValueError, match="moved"):
         e.decode_resident(1, 1)
     e.copy_pages([])                                  # copies nothing
